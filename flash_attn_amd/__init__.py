@@ -24,3 +24,13 @@ from .binding import (  # noqa: F401
     FLASH_MAX_SPLITS,
     lib,
 )
+from .paged import (  # noqa: F401
+    PagedParams,
+    RotaryParams,
+    flash_append_paged,
+    flash_forward_paged,
+    flash_rotary,
+    paged_resolve_splits,
+    paged_workspace_bytes,
+    rotary_frequencies,
+)

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstring>
 
+#include "api_common.h"
 #include "combine.h"
 #include "common.h"
 #include "decode_kernels.h"
@@ -16,17 +17,18 @@
 static_assert(FLASH_MAX_SPLITS == FLASH_MAX_SPLITS_K, "split limits out of sync");
 
 namespace {
-
 thread_local char g_hip_error[256] = "";
+}  // namespace
 
+namespace fa {
+
+// (declared in api_common.h: the other entry points' files use them too)
 int record_hip(int e)
 {
     if (e == (int)hipSuccess) return FLASH_OK;
     std::snprintf(g_hip_error, sizeof(g_hip_error), "%s", hipGetErrorString((hipError_t)e));
     return FLASH_ELAUNCH;
 }
-
-constexpr int kNumCU = 256;  // MI355X
 
 // The library carries gfx950 code only: on any other device the first launch would fail with a HIP error that says
 // little.  Checked once per device (0 = not yet, 1 = gfx950, 2 = something else).
@@ -46,7 +48,15 @@ int device_usable()
     return st == 1 ? FLASH_OK : FLASH_ENODEVICE;
 }
 
-inline bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+}  // namespace fa
+
+namespace {
+
+using fa::device_usable;
+using fa::misaligned;
+using fa::record_hip;
+
+constexpr int kNumCU = 256;  // MI355X
 
 // shape / scalar checks shared by every entry point; *empty is set when there is nothing to compute
 int validate_shape(const flash_params* p, bool* empty)

@@ -1,0 +1,280 @@
+// C entry points of rotary positions and of the paged cache (include/flash_attn_mi355.h): argument checks, split count, launches.
+#include "flash_attn_mi355.h"
+
+#include <cmath>
+#include <cstring>
+
+#include "api_common.h"
+#include "paged_kernel.h"
+#include "rotary_kernels.h"
+
+namespace {
+
+using fa::device_usable;
+using fa::misaligned;
+using fa::record_hip;
+
+constexpr int kNumCU = 256;  // MI355X
+
+// strides of rows that are moved 16 bytes at a time
+inline bool odd_stride(int64_t s) { return (s & 7) != 0; }
+
+// ---------------------------------------------------------------------------------------------- rotary
+
+int run_rotary(const flash_rotary_params* p, hipStream_t st)
+{
+    if (!p) return FLASH_EINVAL;
+    if (p->dtype != FLASH_FP16 && p->dtype != FLASH_BF16 && p->dtype != FLASH_FP32) return FLASH_EINVAL;
+    if (p->B < 0 || p->H < 0 || p->N < 0 || p->d <= 0) return FLASH_EINVAL;
+    if (p->rot < 2 || (p->rot & 1) || p->rot > p->d || p->rot > 512) return FLASH_EINVAL;
+    if ((long long)p->B * p->N > 0x7fffffffLL / 4 || (long long)p->H * p->d > 0x7fffffffLL) return FLASH_EINVAL;
+    if (!std::isfinite(p->factor)) return FLASH_EINVAL;
+    for (int64_t s : {p->x_batch, p->x_head, p->x_row, p->y_batch, p->y_head, p->y_row, p->positions_batch})
+        if (s < 0) return FLASH_EINVAL;
+    if (p->B == 0 || p->H == 0 || p->N == 0) return FLASH_OK;
+    if (!p->X || !p->Y || !p->positions || !p->inv_freq) return FLASH_EINVAL;
+    // (in place: the same rows, not others of the same memory)
+    if (p->X == p->Y && ((p->B > 1 && p->x_batch != p->y_batch) || (p->H > 1 && p->x_head != p->y_head) || (p->N > 1 && p->x_row != p->y_row)))
+        return FLASH_EINVAL;
+    const size_t size = p->dtype == FLASH_FP32 ? 4 : 2;
+    if (misaligned(p->X, size) || misaligned(p->Y, size) || misaligned(p->positions, p->positions_64 ? 8 : 4) || misaligned(p->inv_freq, 4))
+        return FLASH_EALIGN;
+    if (const int rc = device_usable(); rc != FLASH_OK) return rc;
+    int wide = 8;  // elements at once, as far as addresses and strides allow
+    while (wide > 1) {
+        bool fits = !misaligned(p->X, wide * size) && !misaligned(p->Y, wide * size);
+        for (int64_t s : {p->B > 1 ? p->x_batch : 0, p->B > 1 ? p->y_batch : 0, p->H > 1 ? p->x_head : 0, p->H > 1 ? p->y_head : 0, p->N > 1 ? p->x_row : 0,
+                          p->N > 1 ? p->y_row : 0})
+            fits = fits && s % wide == 0;
+        if (fits) break;
+        wide /= 2;
+    }
+    fa::RotaryArgs a{};
+    a.X = p->X, a.Y = p->Y, a.positions = p->positions, a.inv_freq = p->inv_freq;
+    a.x_batch = p->x_batch, a.x_head = p->x_head, a.x_row = p->x_row;
+    a.y_batch = p->y_batch, a.y_head = p->y_head, a.y_row = p->y_row, a.positions_batch = p->positions_batch;
+    a.factor = p->factor;
+    a.B = p->B, a.H = p->H, a.N = p->N, a.d = p->d, a.rot = p->rot;
+    a.positions_64 = p->positions_64 != 0, a.interleaved = p->interleaved != 0, a.inverse = p->inverse != 0;
+    return record_hip(fa::launch_rotary(a, p->dtype, wide, st));
+}
+
+// ---------------------------------------------------------------------------------------------- paged cache
+
+// sizes, types and strides that both entry points share; *empty: nothing to do
+int validate_paged(const flash_paged_params* p, bool* empty)
+{
+    *empty = false;
+    if (!p) return FLASH_EINVAL;
+    if (p->dtype != FLASH_FP16 && p->dtype != FLASH_BF16) return FLASH_EINVAL;
+    if (p->B < 0 || p->H <= 0 || p->H_kv <= 0 || p->H % p->H_kv != 0 || p->d <= 0) return FLASH_EINVAL;
+    if (p->d > FLASH_MAX_HEAD_DIM) return FLASH_EHEADDIM;
+    if (p->d % 8 != 0) return FLASH_EINVAL;
+    if (p->total_q < 0 || p->num_pages < 0 || p->max_pages < 0 || p->page_size <= 0 || p->page_size % 16 != 0) return FLASH_EINVAL;
+    if (p->max_seqlen_q < 0 || p->max_seqlen_k < 0 || p->block_table_stride < 0) return FLASH_EINVAL;
+    // (positions and keys stay far below 2^31 in the kernels' int arithmetic)
+    if ((long long)p->page_size * p->max_pages > (1LL << 30) || p->total_q > (1 << 30) || p->B > (1 << 24)) return FLASH_EINVAL;
+    if ((long long)p->total_q * p->H > 0x7fffffffLL - 0x1000000) return FLASH_EINVAL;
+    if (p->num_splits > FLASH_MAX_SPLITS) return FLASH_ESPLITS;
+    if (p->B == 0 || p->total_q == 0) *empty = true;
+    return FLASH_OK;
+}
+
+// the cache's strides, bases and index tensors; `launch` alone has pointers
+int validate_cache(const flash_paged_params* p)
+{
+    for (int64_t s : {p->kc_page, p->kc_head, p->kc_row, p->vc_page, p->vc_head, p->vc_row})
+        if (s < 0 || odd_stride(s)) return FLASH_EINVAL;
+    if (p->kc_row > (1 << 26) || p->vc_row > (1 << 26)) return FLASH_EINVAL;  // (the 16 rows of a request are addressed with 32 bits)
+    if (!p->seqlens_k || !p->cu_seqlens_q) return FLASH_EINVAL;
+    if (p->max_pages > 0 && !p->block_table) return FLASH_EINVAL;
+    if (misaligned(p->seqlens_k, 4) || misaligned(p->cu_seqlens_q, 4) || misaligned(p->block_table, 4)) return FLASH_EALIGN;
+    if (p->num_pages > 0) {
+        if (!p->K_cache || !p->V_cache) return FLASH_EINVAL;
+        if (misaligned(p->K_cache, 16) || misaligned(p->V_cache, 16)) return FLASH_EALIGN;
+    }
+    return FLASH_OK;
+}
+
+int rows_strides(int64_t token, int64_t head, const void* base)
+{
+    if (token < 0 || head < 0 || odd_stride(token) || odd_stride(head)) return FLASH_EINVAL;
+    if (!base) return FLASH_EINVAL;
+    return misaligned(base, 16) ? FLASH_EALIGN : FLASH_OK;
+}
+
+int group_of(const flash_paged_params* p) { return p->H / p->H_kv; }
+int longest_chunk(const flash_paged_params* p) { return p->max_seqlen_q > 0 && p->max_seqlen_q < p->total_q ? p->max_seqlen_q : p->total_q; }
+int capacity_of(const flash_paged_params* p) { return p->num_pages > 0 ? p->page_size * p->max_pages : 0; }
+
+// Up to 32 rows per K/V head and sequence: the waves of a work-group share out the tiles.
+bool few_rows(const flash_paged_params* p) { return (long long)longest_chunk(p) * group_of(p) <= fa::kPagedFewRows; }
+
+// row blocks of all sequences, at most
+long long row_blocks(const flash_paged_params* p)
+{
+    const int br = few_rows(p) ? fa::kPagedFewRows : fa::kPagedTallRows, G = group_of(p);
+    const long long each = ((long long)longest_chunk(p) * G + br - 1) / br;
+    const long long all = (long long)p->total_q * G / br + p->B;
+    return each * p->B < all ? each * p->B : all;
+}
+
+int window_left_of(const flash_paged_params* p) { return p->window_left >= capacity_of(p) ? -1 : p->window_left; }
+int window_right_of(const flash_paged_params* p) { return p->window_right >= (long long)capacity_of(p) + p->total_q ? -1 : p->window_right; }
+
+// tiles of 64 keys that a row block sees, at most
+int most_tiles(const flash_paged_params* p)
+{
+    const int cap = capacity_of(p), br = few_rows(p) ? fa::kPagedFewRows : fa::kPagedTallRows;
+    long long keys = p->max_seqlen_k > 0 && p->max_seqlen_k < cap ? p->max_seqlen_k : cap;
+    const int wl = window_left_of(p), wr = window_right_of(p);
+    if (wl >= 0 && (p->is_causal || wr >= 0)) {
+        const long long span = (long long)wl + 1 + (p->is_causal || wr < 0 ? 0 : wr) + (br + group_of(p) - 1) / group_of(p) + 63;
+        if (span < keys) keys = span;
+    }
+    return (int)((keys + 63) / 64);
+}
+
+int splits_of(const flash_paged_params* p)
+{
+    const int nt = most_tiles(p);
+    if (nt <= 1 || (long long)p->total_q * p->H >= 1LL << 26) return 1;  // (the merge has a wave per row: 2^32 threads)
+    long long s = p->num_splits;
+    if (s <= 0) {
+        const long long groups = row_blocks(p) * p->H_kv;
+        s = groups >= kNumCU ? 1 : kNumCU / groups;
+        const int least = few_rows(p) ? 2 : 4;  // tiles per split
+        if (s > nt / least) s = nt / least;
+    }
+    if (s > nt) s = nt;
+    if (s > FLASH_MAX_SPLITS) s = FLASH_MAX_SPLITS;
+    if (s < 1) s = 1;
+    const int per = (int)((nt + s - 1) / s);
+    return (nt + per - 1) / per;
+}
+
+int run_forward(const flash_paged_params* p, hipStream_t st)
+{
+    bool empty;
+    int rc = validate_paged(p, &empty);
+    if (rc != FLASH_OK) return rc;
+    if (!(p->softmax_scale > 0.0f) || std::isinf(p->softmax_scale)) return FLASH_EINVAL;
+    if (empty) return FLASH_OK;
+    if ((rc = validate_cache(p)) != FLASH_OK) return rc;
+    if ((rc = rows_strides(p->q_token, p->q_head, p->Q)) != FLASH_OK || (rc = rows_strides(p->o_token, p->o_head, p->O)) != FLASH_OK) return rc;
+    if (!p->LSE) return FLASH_EINVAL;
+    if (misaligned(p->LSE, 4)) return FLASH_EALIGN;
+    const int splits = splits_of(p), nt = most_tiles(p);
+    if (splits > 1) {
+        if (!p->O_partial || !p->LSE_partial) return FLASH_EWORKSPACE;
+        if (misaligned(p->O_partial, 16) || misaligned(p->LSE_partial, 4)) return FLASH_EALIGN;
+    }
+    const bool few = few_rows(p);
+    const long long blocks = row_blocks(p) * p->H_kv * splits;
+    if (blocks * (few ? 256 : 512) >= 1LL << 32) return FLASH_EINVAL;
+    if ((rc = device_usable()) != FLASH_OK) return rc;
+    fa::PagedArgs a{};
+    a.Q = static_cast<const char*>(p->Q), a.K = static_cast<const char*>(p->K_cache), a.V = static_cast<const char*>(p->V_cache);
+    a.O = static_cast<char*>(p->O), a.LSE = p->LSE, a.O_partial = p->O_partial, a.LSE_partial = p->LSE_partial;
+    a.table = p->block_table, a.lens = p->seqlens_k, a.cu = p->cu_seqlens_q;
+    a.q_token = 2 * p->q_token, a.q_head = 2 * p->q_head, a.o_token = 2 * p->o_token, a.o_head = 2 * p->o_head;
+    a.k_page = 2 * p->kc_page, a.k_head = 2 * p->kc_head, a.v_page = 2 * p->vc_page, a.v_head = 2 * p->vc_head;
+    a.k_row = (uint32_t)(2 * p->kc_row), a.v_row = (uint32_t)(2 * p->vc_row);
+    a.table_stride = p->block_table_stride;
+    a.B = p->B, a.H = p->H, a.Hk = p->H_kv, a.G = group_of(p), a.d = p->d, a.tokens = p->total_q, a.num_pages = p->num_pages, a.page = p->page_size;
+    a.capacity = capacity_of(p);
+    a.causal = p->is_causal != 0, a.wl = window_left_of(p), a.wr = window_right_of(p);
+    a.scale_log2 = p->softmax_scale * fa::kLog2e;
+    a.num_splits = splits, a.tiles_per_split = (nt + splits - 1) / splits;
+    a.direct = (long long)longest_chunk(p) * a.G <= (few ? fa::kPagedFewRows : fa::kPagedTallRows);
+    a.by_unit = fa::fast_div((long long)a.Hk * splits), a.by_heads = fa::fast_div(a.Hk), a.by_group = fa::fast_div(a.G), a.by_page = fa::fast_div(a.page);
+    a.by_splits = fa::fast_div(splits);
+    const bool bf16 = p->dtype == FLASH_BF16;
+    rc = record_hip(p->d <= 64 ? fa::launch_paged_d64(a, bf16, few, blocks, st) : fa::launch_paged_d128(a, bf16, few, blocks, st));
+    if (rc != FLASH_OK || splits == 1) return rc;
+    return record_hip(fa::launch_paged_merge(a, bf16, st));
+}
+
+int run_append(const flash_paged_params* p, hipStream_t st)
+{
+    bool empty;
+    int rc = validate_paged(p, &empty);
+    if (rc != FLASH_OK) return rc;
+    const bool turns = p->inv_freq != nullptr, queries = turns && p->Q != nullptr;
+    if (turns) {
+        if (p->rot < 2 || (p->rot & 1) || p->rot > p->d || !std::isfinite(p->factor)) return FLASH_EINVAL;
+        if (misaligned(p->inv_freq, 4)) return FLASH_EALIGN;
+        if (p->positions && misaligned(p->positions, p->positions_64 ? 8 : 4)) return FLASH_EALIGN;
+    }
+    if (empty) return FLASH_OK;
+    if ((rc = validate_cache(p)) != FLASH_OK) return rc;
+    if ((rc = rows_strides(p->k_token, p->k_head, p->K)) != FLASH_OK || (rc = rows_strides(p->v_token, p->v_head, p->V)) != FLASH_OK) return rc;
+    if (queries) {
+        if ((rc = rows_strides(p->q_token, p->q_head, p->Q)) != FLASH_OK || (rc = rows_strides(p->o_token, p->o_head, p->O)) != FLASH_OK) return rc;
+        if (p->Q == p->O && ((p->total_q > 1 && p->q_token != p->o_token) || (p->H > 1 && p->q_head != p->o_head))) return FLASH_EINVAL;
+    }
+    if ((rc = device_usable()) != FLASH_OK) return rc;
+    fa::AppendArgs a{};
+    a.Q = p->Q, a.K = p->K, a.V = p->V, a.O = p->O, a.K_cache = p->K_cache, a.V_cache = p->V_cache, a.positions = p->positions;
+    a.table = p->block_table, a.lens = p->seqlens_k, a.cu = p->cu_seqlens_q, a.inv_freq = p->inv_freq;
+    a.q_token = p->q_token, a.q_head = p->q_head, a.o_token = p->o_token, a.o_head = p->o_head;
+    a.k_token = p->k_token, a.k_head = p->k_head, a.v_token = p->v_token, a.v_head = p->v_head;
+    a.kc_page = p->kc_page, a.kc_head = p->kc_head, a.kc_row = p->kc_row, a.vc_page = p->vc_page, a.vc_head = p->vc_head, a.vc_row = p->vc_row;
+    a.table_stride = p->block_table_stride;
+    a.factor = p->factor;
+    a.B = p->B, a.H = queries ? p->H : 0, a.Hk = p->H_kv, a.d = p->d, a.rot = turns ? p->rot : 0, a.tokens = p->total_q, a.num_pages = p->num_pages;
+    a.page = p->page_size, a.capacity = capacity_of(p), a.positions_64 = p->positions_64 != 0, a.interleaved = turns && p->interleaved != 0;
+    return record_hip(fa::launch_append(a, p->dtype, st));
+}
+
+}  // namespace
+
+#define FLASH_EXPORT __attribute__((visibility("default")))
+
+extern "C" {
+
+FLASH_EXPORT int flash_rotary(const flash_rotary_params* p, void* stream) { return run_rotary(p, static_cast<hipStream_t>(stream)); }
+
+FLASH_EXPORT int flash_append_paged(const flash_paged_params* p, void* stream) { return run_append(p, static_cast<hipStream_t>(stream)); }
+
+FLASH_EXPORT int flash_forward_paged(const flash_paged_params* p, void* stream) { return run_forward(p, static_cast<hipStream_t>(stream)); }
+
+FLASH_EXPORT int flash_forward_paged_resolve_splits(const flash_paged_params* p)
+{
+    bool empty;
+    const int rc = validate_paged(p, &empty);
+    if (rc != FLASH_OK) return rc;
+    return empty ? 1 : splits_of(p);
+}
+
+FLASH_EXPORT int flash_forward_paged_workspace_bytes(const flash_paged_params* p, size_t* o_partial_bytes, size_t* lse_partial_bytes)
+{
+    bool empty;
+    const int rc = validate_paged(p, &empty);
+    if (rc != FLASH_OK) return rc;
+    const int splits = empty ? 1 : splits_of(p);
+    const size_t rows = splits > 1 ? (size_t)p->total_q * p->H * splits : 0;
+    if (o_partial_bytes) *o_partial_bytes = rows * p->d * sizeof(float);
+    if (lse_partial_bytes) *lse_partial_bytes = rows * sizeof(float);
+    return FLASH_OK;
+}
+
+FLASH_EXPORT void flash_rotary_params_init(flash_rotary_params* p)
+{
+    if (!p) return;
+    std::memset(p, 0, sizeof(*p));
+    p->factor = 1.0f;
+}
+
+FLASH_EXPORT void flash_paged_params_init(flash_paged_params* p)
+{
+    if (!p) return;
+    std::memset(p, 0, sizeof(*p));
+    p->window_left = p->window_right = -1;
+    p->factor = 1.0f;
+}
+
+FLASH_EXPORT size_t flash_rotary_params_size(void) { return sizeof(flash_rotary_params); }
+FLASH_EXPORT size_t flash_paged_params_size(void) { return sizeof(flash_paged_params); }
+
+}  // extern "C"

@@ -1,0 +1,1055 @@
+// Attention of ragged chunks of new tokens over a paged K/V cache (flash_forward_paged), fp16 and bf16, d a multiple of 8 up to 128.
+//
+//   O_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys j that row i sees, LSE_i = log sum_j exp(scale q_i . k_j)
+//
+// Sequence b has the query rows cu[b] ... cu[b + 1] - 1 of Q [tokens, H, d] and lens[b] keys; key j lies in row j % page of page
+// table[b][j / page].  The chunk's rows are the last of the sequence: row i stands at position i + len - rows.
+// The G query heads of a K/V head are the rows of one problem over it: row r is query r / G of head r % G, so that K and V
+// are read once per K/V head, whatever G is.
+//
+// Pages.  A request of the tile loads (global_load_lds_dwordx4, one KiB) covers 4 rows of 256 bytes or 8 of 128.  Tiles begin at multiples of
+// 64 keys and pages hold multiples of 16, so the rows of a request lie in one page: its place is worked out on the scalar unit (an
+// entry of the table by s_load, one tile ahead of its use) and the lanes' own offsets never change.  No vector instruction goes
+// into paging, and with it no page size costs more than another.
+//
+// Two forms share the mathematics of fwd_kernel.h (S^T = K Q^T and O^T += V^T P^T on 32x32x16 MFMA, one query row per lane, scores
+// scaled inside the exponent, a running maximum that is raised only when some row outgrows it by 2^8):
+//   paged_tall_kernel  256 rows per work-group, eight waves that share the tiles, the schedule of fwd_pp_kernel.h: on every SIMD one
+//                      wave is at its MFMAs while the other is at its softmax.  Bound by MFMA and softmax.
+//   paged_few_kernel   up to 32 rows, four waves that share out the tiles, each with LDS stages of its own and no barrier in the loop;
+//                      the four results are merged through LDS.  Bound by HBM.
+// Either form may split the key range (num_splits): partial results in fp32, merged by paged_merge_kernel.
+//
+// What is not in the sequence must not reach the result: keys past its end are not read (their rows repeat the last key's), columns
+// d ... D - 1 of the tiles in LDS are zeroed once and never requested, and a product of a masked probability, 0, with a V that is
+// not finite is taken back out at the end (rescue).
+#pragma once
+#include <type_traits>
+
+#include "common.h"
+
+namespace fa {
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+constexpr int kPagedTallRows = 256, kPagedFewRows = 32;
+
+struct PagedArgs {
+    const char *Q, *K, *V;
+    char* O;
+    float* LSE;                        // [tokens, H]
+    float *O_partial, *LSE_partial;    // [tokens, H, S, d] and [tokens, H, S]
+    const int32_t *table, *lens, *cu;
+    int64_t q_token, q_head, o_token, o_head, k_page, k_head, v_page, v_head, table_stride;  // bytes (table_stride: entries)
+    uint32_t k_row, v_row;             // bytes
+    int B, H, Hk, G, d, tokens, num_pages, page, capacity;  // capacity: keys that a row of the table can name
+    int causal, wl, wr;                // wl / wr < 0: unbounded
+    float scale_log2;
+    int num_splits, tiles_per_split;
+    int direct;                        // every sequence has one row block: work-group u is sequence u
+    FastDiv by_unit, by_heads, by_group, by_page, by_splits;
+};
+
+// What the merge needs of them (short arguments launch faster: common.h)
+struct PagedMergeArgs {
+    char* O;
+    float* LSE;
+    const float *O_partial, *LSE_partial;
+    const int32_t* cu;
+    int64_t o_token, o_head;
+    int B, H, d, tokens, num_splits;
+};
+
+// An int that nobody writes during the launch at an address that is the same in all lanes: a load of the scalar unit.
+__device__ __forceinline__ int read_uniform_int(const int32_t* p)
+{
+    return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
+}
+
+template <bool kBf16>
+struct Elem {
+    static __device__ __forceinline__ v16f mfma(v8h a, v8h b, v16f c)
+    {
+        if constexpr (kBf16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    // two floats rounded to nearest even, packed
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        const v2f t = {a, b};
+        if constexpr (kBf16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(t, v2bf));
+        else return __builtin_bit_cast(uint32_t, __builtin_convertvector(t, v2h));
+    }
+    static __device__ __forceinline__ float low(uint32_t u)
+    {
+        if constexpr (kBf16) return __uint_as_float(u << 16);
+        else return (float)__builtin_bit_cast(v2h, u)[0];
+    }
+    static __device__ __forceinline__ float high(uint32_t u)
+    {
+        if constexpr (kBf16) return __uint_as_float(u & 0xffff0000u);
+        else return (float)__builtin_bit_cast(v2h, u)[1];
+    }
+    // whether one of the two is infinite or not a number
+    static __device__ __forceinline__ bool not_finite(uint32_t u)
+    {
+        constexpr uint32_t e = kBf16 ? 0x7f80u : 0x7c00u;
+        return (u & e) == e || (u >> 16 & e) == e;
+    }
+};
+
+// ---------------------------------------------------------------------------------------------- work of a work-group
+
+struct PagedItem {
+    int b, hk, split;
+    int tok0, rows;   // first token of the chunk; query rows of the problem (tokens times heads per K/V head)
+    int row0;         // first row of the work-group
+    int len, shift;   // keys; position of query 0
+};
+
+// Lengths come from device memory: whatever they hold, nothing outside the tensors is touched.
+__device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// Work-group -> (sequence, row block, split, K/V head); false where there is nothing to do.  K/V heads vary fastest, splits next, so
+// that with a multiple of 8 of them the row blocks of a K/V head find its keys in one XCD's L2; row blocks of a sequence come last
+// first, which under a causal mask is heaviest first.
+template <int BR>
+__device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedItem* it)
+{
+    const int block = blockIdx.x;
+    const int u = a.by_unit.quotient(block), rest = block - u * (a.Hk * a.num_splits);
+    it->split = a.by_heads.quotient(rest);
+    it->hk = rest - it->split * a.Hk;
+    int b = u, m = 0;
+    if (!a.direct) {
+        // row blocks of 64 sequences at a time, a lane each
+        int before = 0;
+        bool found = false;
+        for (int b0 = 0; b0 < a.B; b0 += 64) {
+            const int mine = b0 + lane;
+            int n = 0;
+            if (mine < a.B) {
+                const int c0 = clamp_int(a.cu[mine], 0, a.tokens), c1 = clamp_int(a.cu[mine + 1], c0, a.tokens);
+                n = ((c1 - c0) * a.G + BR - 1) / BR;
+            }
+            int upto = n;
+#pragma unroll
+            for (int s = 1; s < 64; s <<= 1) {
+                const int other = __shfl_up(upto, s);
+                if (lane >= s) upto += other;
+            }
+            const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > u);
+            if (past != 0) {
+                const int at = __builtin_ctzll(past);
+                b = b0 + at;
+                m = before + __builtin_amdgcn_readlane(upto, at) - 1 - u;
+                found = true;
+                break;
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+        }
+        if (!found) return false;
+        b = wave_uniform(b);
+        m = wave_uniform(m);
+    }
+    const int c0 = clamp_int(read_uniform_int(a.cu + b), 0, a.tokens), c1 = clamp_int(read_uniform_int(a.cu + b + 1), c0, a.tokens);
+    it->b = b;
+    it->tok0 = c0;
+    it->rows = (c1 - c0) * a.G;
+    it->row0 = m * BR;
+    it->len = clamp_int(read_uniform_int(a.lens + b), 0, a.capacity);
+    it->shift = it->len - (c1 - c0);
+    return it->row0 < it->rows;
+}
+
+// keys [kmin, kmax) that some row of the work-group sees, of those its split's share: the range of the row block is cut, not the
+// sequence, so that windows and short chunks in long caches divide evenly
+template <int BR>
+__device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedItem& it, int* kmin, int* kmax)
+{
+    const int last = it.row0 + BR < it.rows ? it.row0 + BR - 1 : it.rows - 1;
+    const int p0 = a.by_group.quotient(it.row0) + it.shift, p1 = a.by_group.quotient(last) + it.shift;
+    int lo = 0, hi = it.len;
+    if (a.wl >= 0) lo = max(0, p0 - a.wl);
+    if (a.causal) hi = min(hi, p1 + 1);
+    if (a.wr >= 0) hi = min(hi, p1 + a.wr + 1);
+    if (a.num_splits > 1) {
+        // as many tiles per split as the launch was sized for, or more, should the range be longer than the caller said
+        const int t0 = lo >> 6, nt = hi > lo ? ((hi + 63) >> 6) - t0 : 0;
+        const int per = max(a.tiles_per_split, a.by_splits.quotient(nt + a.num_splits - 1));
+        const int64_t s0 = ((int64_t)t0 + (int64_t)it.split * per) * 64, s1 = s0 + (int64_t)per * 64;
+        lo = (int)max((int64_t)lo, min(s0, (int64_t)hi));
+        hi = (int)min((int64_t)hi, s1);
+    }
+    *kmin = lo;
+    *kmax = hi;
+}
+
+// first and last key that row r (of the problem) sees; [lo, hi] may be empty
+__device__ __forceinline__ void paged_bounds(const PagedArgs& a, const PagedItem& it, int r, int kmin, int kmax, int* lo, int* hi)
+{
+    const int p = a.by_group.quotient(r < it.rows ? r : it.rows - 1) + it.shift;
+    int l = kmin, h = kmax - 1;
+    if (a.wl >= 0) l = max(l, p - a.wl);
+    if (a.causal) h = min(h, p);
+    if (a.wr >= 0) h = min(h, p + a.wr);
+    *lo = l;
+    *hi = h;
+}
+
+__device__ __forceinline__ int row_token(const PagedArgs& a, const PagedItem& it, int r, int* head)
+{
+    const int i = a.by_group.quotient(r);
+    *head = it.hk * a.G + (r - i * a.G);
+    return it.tok0 + i;
+}
+
+// Entry of the page that key j of the sequence lies in, kept inside the cache whatever the table holds.
+__device__ __forceinline__ int paged_entry(const PagedArgs& a, const int32_t* table_row, int len, int j)
+{
+    return read_uniform_int(table_row + a.by_page.quotient(j < len ? j : len - 1));
+}
+__device__ __forceinline__ int64_t inside(const PagedArgs& a, int entry) { return (uint32_t)entry < (uint32_t)a.num_pages ? entry : 0; }
+
+// rows of the work-group that see no key: O = 0, LSE = -inf, or the same as partial results
+template <int BR, int kThreads>
+__device__ __forceinline__ void paged_store_empty(const PagedArgs& a, const PagedItem& it, int tid)
+{
+    const int n = min(BR, it.rows - it.row0);
+    for (int k = tid; k < n * 16; k += kThreads) {
+        const int r = it.row0 + (k >> 4), c = k & 15;
+        int head;
+        const int tok = row_token(a, it, r, &head);
+        const size_t row = (size_t)tok * a.H + head;
+        if (a.num_splits > 1) {  // (a partial result of weight 0 is not read)
+            if (c == 0) a.LSE_partial[row * a.num_splits + it.split] = -INFINITY;
+        } else {
+            const v4u z = {0u, 0u, 0u, 0u};
+            if (c * 8 < a.d) *reinterpret_cast<v4u*>(a.O + (size_t)tok * a.o_token + (size_t)head * a.o_head + c * 16) = z;
+            if (c == 0) a.LSE[row] = -INFINITY;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- tiles in LDS
+//
+// A stage holds 64 keys row-major, D * 2 bytes each, with the 16-byte chunks of a row permuted so that the fragment reads are free of
+// bank conflicts:
+//   K: chunk c of key r in slot c ^ (r % 16) (256-byte rows) or c ^ (r / 2 % 8) (128-byte rows)
+//   V: 32-byte chunk c in slot c ^ (2 (r % 4) + r / 4 % 2), or the two halves of a 128-byte row exchanged in rows 2, 3 mod 4
+template <int D>
+struct PagedTile {
+    static constexpr int BC = 64, KS = D / 16, MB = D / 32, ROW = D * 2, BUF = BC * ROW;
+    static constexpr int RPB = 1024 / ROW;   // rows of a request
+    static constexpr int REQ = BUF / 1024;   // requests of a tile
+    static constexpr int CPR = ROW / 16;     // chunks of a row
+    static __device__ __forceinline__ int k_chunk(int slot, int r) { return D == 128 ? slot ^ (r & 15) : slot ^ ((r >> 1) & 7); }
+    static __device__ __forceinline__ int v_chunk(int slot, int r)
+    {
+        return D == 128 ? ((((slot >> 1) ^ (2 * (r & 3) + ((r >> 2) & 1))) << 1) | (slot & 1)) : slot ^ (((r >> 1) & 1) << 2);
+    }
+    // lane part of a K fragment's address: key l32, chunk 2 ks + g -> k_lane ^ (ks << 5), + BUF / 2 for the second 32 keys
+    static __device__ __forceinline__ int k_lane(int lane)
+    {
+        const int l32 = lane & 31, g = lane >> 5, z = D == 128 ? l32 & 15 : (l32 >> 1) & 7;
+        return l32 * ROW + ((g ^ (z & 1)) << 4) + ((z >> 1) << 5);
+    }
+    // of a V fragment's: keys 16 st + 8 h + 4 (lane / 32) + e, columns 32 mb + 16 (lane / 16 % 2) + 4 j ... + 3
+    // -> v_lane ^ (mb << 6), + (16 st + 8 h) ROW
+    static __device__ __forceinline__ int v_lane(int lane)
+    {
+        const int G = lane >> 4, e = (lane >> 2) & 3, j = lane & 3;
+        if (D == 128) return (4 * (G >> 1) + e) * ROW + (((G & 1) ^ (G >> 1)) << 5) + 8 * j + (e << 6);
+        return (4 * (G >> 1) + e) * ROW + ((G & 1) << 5) + 8 * j + ((e >> 1) << 6);
+    }
+};
+
+__device__ __forceinline__ FA_LDS const char* lds_at(uint32_t addr) { return reinterpret_cast<FA_LDS const char*>(static_cast<uintptr_t>(addr)); }
+
+// The sum of the register and the lane part, kept as one register (written out, the compiler keeps one per fragment).
+__device__ __forceinline__ uint32_t fragment_base(FA_LDS const char* stage, int lane_part)
+{
+    uint32_t v = (uint32_t)(uintptr_t)stage + (uint32_t)lane_part;
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+template <int D>
+__device__ __forceinline__ v8h v_fragment(uint32_t vbase, int st, int mb)
+{
+    FA_LDS const char* p0 = lds_at(vbase ^ (uint32_t)(mb << 6)) + st * 16 * PagedTile<D>::ROW;
+    union { v4hp p[2]; v8h v; } f;
+    f.p[0] = __builtin_amdgcn_ds_read_tr16_b64_v4f16((FA_LDS v4hp*)(p0));
+    f.p[1] = __builtin_amdgcn_ds_read_tr16_b64_v4f16((FA_LDS v4hp*)(p0 + 8 * PagedTile<D>::ROW));
+    return f.v;
+}
+template <int D>
+__device__ __forceinline__ v8h k_fragment(uint32_t kbase, int ks, int kb)
+{
+    return *reinterpret_cast<FA_LDS const v8h*>(lds_at(kbase ^ (uint32_t)(ks << 5)) + kb * (PagedTile<D>::BUF / 2));
+}
+
+constexpr float kPagedTau = 8.0f;                       // powers of two by which a row may outgrow its running maximum
+constexpr float kPagedNothing = -3.402823466e38f;       // running maximum of a row that has seen no key
+
+// Online softmax of one tile: scores in s (unscaled), P^T packed into p as the B operand of the second product.
+template <bool kBf16, int MB>
+struct PagedSoftmax {
+    float m_ref = kPagedNothing, m_thr = -INFINITY, l_run = 0.0f;
+    __device__ __forceinline__ void tile(v16f (&s)[2], v16f (&oacc)[MB], uint32_t (&p)[2][2][4], float c2, float inv_c2, int sides, int lo_rel, int hi_rel)
+    {
+        if (__builtin_expect(sides != 0, 0)) mask_tile<false>(s[0], s[1], wave_uniform(mask_modes_general(sides)), lo_rel, hi_rel, -INFINITY);
+        float mk[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) mk[kb] = fmaxf(mk[kb], s[kb][r]);
+        const float mx = fmaxf(mk[0], mk[1]);
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m_thr) != 0ull, 0)) {
+            const float m_new = fmaxf(m_ref, xhalf_max(mx) * c2);  // c2 > 0
+            float alpha = fast_exp2(m_ref - m_new);
+            asm volatile("; raise running max" : "+v"(alpha));
+            m_ref = m_new;
+            m_thr = (m_new + kPagedTau) * inv_c2;
+            l_run *= alpha;
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) oacc[mb][r] *= alpha;
+        }
+        float rs = 0.0f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const float p0 = fast_exp2(__builtin_fmaf(s[kb][r], c2, -m_ref)), p1 = fast_exp2(__builtin_fmaf(s[kb][r + 1], c2, -m_ref));
+                rs = kb == 0 && r == 0 ? p0 + p1 : rs + p0 + p1;
+                p[kb][r >> 3][(r & 7) >> 1] = Elem<kBf16>::pack(p0, p1);
+            }
+        l_run += rs;
+    }
+};
+
+__device__ __forceinline__ v8h as_fragment(const uint32_t (&p)[4])
+{
+    const v4u t = {p[0], p[1], p[2], p[3]};
+    return __builtin_bit_cast(v8h, t);
+}
+
+// Q fragments (B operand): lane holds row r's columns 16 ks + 8 g ... + 7; zeroes past d
+template <int KS>
+__device__ __forceinline__ void load_q(const PagedArgs& a, const PagedItem& it, int r, int g, v8h (&qf)[KS])
+{
+    int head;
+    const int tok = row_token(a, it, r < it.rows ? r : it.rows - 1, &head);
+    const char* const q = a.Q + (size_t)tok * a.q_token + (size_t)head * a.q_head;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int c = 16 * ks + 8 * g;
+        v4u v = *reinterpret_cast<const v4u*>(q + 2 * (c < a.d ? c : 0));
+        const v4u z = {0u, 0u, 0u, 0u};
+        v = c < a.d ? v : z;
+        qf[ks] = __builtin_bit_cast(v8h, v);
+    }
+}
+
+// A masked probability is 0, and 0 times a V that is not finite is not: such a product has spoilt the row's sum if V has one in a tile of
+// which the row sees a part, or none.  Called once per wave, behind its loop, where some sum is not finite: looks for such
+// values among the wave's partly masked tiles and, if there are any, works out the rows in question once more key by key, visible
+// keys alone.  (Tiles first, first + step, ... of the range from key kb_first on.)
+template <int D, int MB, bool kBf16>
+__device__ __forceinline__ void paged_rescue(const PagedArgs& a, const PagedItem& it, int r, int kmin, int kmax, int tile0, int ntiles, int first,
+                                                       int step, float m_ref, v16f (&oacc)[MB])
+{
+    const int lane = threadIdx.x & 63, g = lane >> 5;
+    const int32_t* const table_row = a.table + (size_t)it.b * a.table_stride;
+    int lo, hi;
+    paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
+    auto row_of = [&](const char* base, int64_t page_bytes, int64_t head_bytes, uint32_t row_bytes, int j) {
+        const int pg = a.by_page.quotient(j);
+        return base + inside(a, table_row[pg]) * page_bytes + it.hk * head_bytes + (int64_t)(j - pg * a.page) * row_bytes;
+    };
+    // lane j: key j of the tile; masked for some row of the wave, and not finite somewhere?
+    bool spoilt = false;
+    for (int t = first; t < ntiles; t += step) {
+        const int kb0 = (tile0 + t) * 64, j = kb0 + lane;
+        bool some = false;  // of the lanes' rows does one not see key j?  (the key is told to all rows in turn)
+        for (int q = 0; q < 32; ++q) {
+            const int l = __builtin_amdgcn_readlane(lo, q), h = __builtin_amdgcn_readlane(hi, q);
+            some |= j < l || j > h;
+        }
+        if (some && j < it.len) {
+            const char* const v = row_of(a.V, a.v_page, a.v_head, a.v_row, j);
+            for (int c = 0; c < a.d; c += 2) spoilt |= Elem<kBf16>::not_finite(*reinterpret_cast<const uint32_t*>(v + 2 * c));
+        }
+    }
+    if (__builtin_amdgcn_ballot_w64(spoilt) == 0) return;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[mb][e] = 0.0f;
+    int head;
+    const int tok = row_token(a, it, r < it.rows ? r : it.rows - 1, &head);
+    const char* const q = a.Q + (size_t)tok * a.q_token + (size_t)head * a.q_head;
+    for (int t = first; t < ntiles; t += step) {
+        const int kb0 = (tile0 + t) * 64;
+        const int j0 = max(kb0, lo), j1 = min(kb0 + 63, hi);
+        for (int j = j0; j <= j1; ++j) {
+            const char* const k = row_of(a.K, a.k_page, a.k_head, a.k_row, j);
+            const char* const v = row_of(a.V, a.v_page, a.v_head, a.v_row, j);
+            float s = 0.0f;
+            for (int c = 0; c < a.d; c += 2) {
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(q + 2 * c), y = *reinterpret_cast<const uint32_t*>(k + 2 * c);
+                s = __builtin_fmaf(Elem<kBf16>::low(x), Elem<kBf16>::low(y), s);
+                s = __builtin_fmaf(Elem<kBf16>::high(x), Elem<kBf16>::high(y), s);
+            }
+            const float e = fast_exp2(__builtin_fmaf(s, a.scale_log2, -m_ref)), p = Elem<kBf16>::low(Elem<kBf16>::pack(e, e));
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int rg = 0; rg < 4; ++rg) {
+                    const int c = 32 * mb + 8 * rg + 4 * g;
+                    if (c < a.d) {
+                        const v2u w = *reinterpret_cast<const v2u*>(v + 2 * c);
+                        oacc[mb][4 * rg] = __builtin_fmaf(p, Elem<kBf16>::low(w[0]), oacc[mb][4 * rg]);
+                        oacc[mb][4 * rg + 1] = __builtin_fmaf(p, Elem<kBf16>::high(w[0]), oacc[mb][4 * rg + 1]);
+                        oacc[mb][4 * rg + 2] = __builtin_fmaf(p, Elem<kBf16>::low(w[1]), oacc[mb][4 * rg + 2]);
+                        oacc[mb][4 * rg + 3] = __builtin_fmaf(p, Elem<kBf16>::high(w[1]), oacc[mb][4 * rg + 3]);
+                    }
+                }
+        }
+    }
+}
+
+template <int MB>
+__device__ __forceinline__ bool any_not_finite(const v16f (&oacc)[MB])
+{
+    float z = 0.0f;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z = __builtin_fmaf(oacc[mb][r], 0.0f, z);
+    return __builtin_amdgcn_ballot_w64(!(z == 0.0f)) != 0ull;
+}
+
+// ---------------------------------------------------------------------------------------------- few rows
+
+template <int D>
+struct FewCfg {
+    static constexpr int kWaves = 4, NST = D == 128 ? 1 : 2;
+    static constexpr int WAVE = NST * 2 * PagedTile<D>::BUF;  // LDS of a wave's stages
+    static constexpr int OROW = D + 4;                        // floats of a row of partial O
+    static constexpr int SMEM = kWaves * WAVE;
+    static_assert(kWaves * (32 * OROW + 64) * 4 <= SMEM, "the merge takes the stages' place");
+};
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(256, 1) paged_few_kernel(const PagedArgs a)
+{
+    using T = PagedTile<D>;
+    using C = FewCfg<D>;
+    constexpr int KS = T::KS, MB = T::MB, REQ = T::REQ, NST = C::NST;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6), l32 = lane & 31, g = lane >> 5;
+
+    PagedItem it;
+    if (!paged_item<kPagedFewRows>(a, lane, &it)) return;
+    int kmin, kmax;
+    paged_range<kPagedFewRows>(a, it, &kmin, &kmax);
+    if (kmax <= kmin) {
+        paged_store_empty<kPagedFewRows, 256>(a, it, tid);
+        return;
+    }
+    const int tile0 = kmin >> 6, ntiles = ((kmax + 63) >> 6) - tile0;
+    const int len = it.len;
+    const int32_t* const table_row = a.table + (size_t)it.b * a.table_stride;
+
+    FA_LDS char* const mine = (FA_LDS char*)smem + wave * C::WAVE;
+    if (a.d != D) {  // columns that no request writes
+        const v4u z = {0u, 0u, 0u, 0u};
+        for (int k = lane; k < C::WAVE / 16; k += 64) *reinterpret_cast<FA_LDS v4u*>(mine + 16 * k) = z;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+
+    // ---- requests: request x of a tile covers its rows RPB x ... ; four table entries per tile, one for each 16 keys
+    const int lrow = lane / T::CPR, slot = lane % T::CPR;
+    constexpr int kPer = REQ / 4;  // requests per 16 keys
+    uint32_t koff[kPer], voff[kPer];
+    bool kok[kPer], vok[kPer];
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+        const int r = T::RPB * x + lrow, ck = T::k_chunk(slot, r), cv = T::v_chunk(slot, r);
+        koff[x] = (uint32_t)r * a.k_row + ck * 16;
+        voff[x] = (uint32_t)r * a.v_row + cv * 16;
+        kok[x] = ck * 8 < a.d;
+        vok[x] = cv * 8 < a.d;
+    }
+    int entry[4];
+    auto ask_entries = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) entry[s] = paged_entry(a, table_row, len, (tile0 + t) * 64 + 16 * s);
+    };
+    // the 64 rows of tile t (its entries given) of K or V
+    auto request = [&](int t, const int (&entries)[4], const char* base, int64_t page_bytes, int64_t head_bytes, uint32_t row_bytes,
+                       const uint32_t (&off)[kPer], const bool (&ok)[kPer], FA_LDS char* dst) __attribute__((always_inline)) {
+        const int kb0 = (tile0 + t) * 64;
+        const bool whole = kb0 + 64 <= len;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int j = kb0 + 16 * s, jj = j < len ? j : len - 1;
+            const int in_page = jj - a.by_page.quotient(jj) * a.page;
+            const char* const at = base + inside(a, entries[s]) * page_bytes + it.hk * head_bytes + (int64_t)in_page * row_bytes;
+#pragma unroll
+            for (int x = 0; x < kPer; ++x) {
+                uint32_t o = off[x];
+                if (!whole) {  // rows past the last key repeat it
+                    const int r = T::RPB * x + lrow, most = len - 1 - jj;
+                    if (r > most) o -= (uint32_t)(r - most) * row_bytes;
+                }
+                if (ok[x]) dma_kib_nt(at, o, dst + (s * kPer + x) * 1024);
+            }
+        }
+    };
+    auto k_stage = [&](int n) { return mine + (n % NST) * T::BUF; };
+    auto v_stage = [&](int n) { return mine + NST * T::BUF + (n % NST) * T::BUF; };
+    auto request_k = [&](int t, const int (&e)[4], int n) { request(t, e, a.K, a.k_page, a.k_head, a.k_row, koff, kok, k_stage(n)); };
+    auto request_v = [&](int t, const int (&e)[4], int n) { request(t, e, a.V, a.v_page, a.v_head, a.v_row, voff, vok, v_stage(n)); };
+
+    const int r = it.row0 + l32;
+    v8h qf[KS];
+    v16f oacc[MB];
+    PagedSoftmax<kBf16, MB> soft;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[mb][e] = 0.0f;
+
+    int lo, hi;
+    paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
+    int lo_max = lo, hi_min = hi;
+    if (wave < ntiles) {
+        ask_entries(wave);
+        load_q<KS>(a, it, r, g, qf);
+        request_k(wave, entry, 0);
+        request_v(wave, entry, 0);
+        lo_max = __builtin_amdgcn_readlane(lo, 31);  // (bounds do not fall from row to row)
+        hi_min = __builtin_amdgcn_readlane(hi, 0);
+    }
+    const float c2 = a.scale_log2, inv_c2 = __builtin_amdgcn_rcpf(c2);
+    const int k_rd = T::k_lane(lane), v_rd = T::v_lane(lane);
+    int n = 0;
+    for (int t = wave; t < ntiles; t += 4, ++n) {
+        const int kb0 = (tile0 + t) * 64;
+        const bool more = t + 4 < ntiles;
+        if (more) ask_entries(t + 4);
+        if constexpr (NST == 2) {
+            if (more) {
+                request_k(t + 4, entry, n + 1);
+                request_v(t + 4, entry, n + 1);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * REQ) : "memory");  // K of this tile is there
+            } else {
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");
+            }
+        } else {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");
+        }
+        if (n == 0) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
+        }
+        v16f s[2];
+        {
+            const uint32_t kbase = fragment_base(k_stage(n), k_rd);
+            const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) s[kb] = Elem<kBf16>::mfma(k_fragment<D>(kbase, ks, kb), qf[ks], ks == 0 ? z : s[kb]);
+        }
+        if constexpr (NST == 1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the fragments have been read
+            if (more) request_k(t + 4, entry, n + 1);
+        }
+        uint32_t p[2][2][4];
+        soft.tile(s, oacc, p, c2, inv_c2, mask_sides(kb0, lo_max, hi_min), lo - kb0 - 4 * g, hi - kb0 - 4 * g);
+        if constexpr (NST == 2) {
+            if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * REQ) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else {
+            if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        {
+            const uint32_t vbase = fragment_base(v_stage(n), v_rd);
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb) oacc[mb] = Elem<kBf16>::mfma(v_fragment<D>(vbase, st, mb), as_fragment(p[st >> 1][st & 1]), oacc[mb]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if constexpr (NST == 1) {
+            if (more) request_v(t + 4, entry, n + 1);
+        }
+    }
+    if (wave < ntiles && __builtin_expect(any_not_finite<MB>(oacc), 0))
+        paged_rescue<D, MB, kBf16>(a, it, r, kmin, kmax, tile0, ntiles, wave, 4, soft.m_ref, oacc);
+
+    // ---- merge of the four waves: reference of a row = the largest of theirs
+    const int nrows = min(kPagedFewRows, it.rows - it.row0);
+    FA_LDS float* const xo = (FA_LDS float*)smem;                       // [4][32][OROW]
+    FA_LDS float* const xm = xo + 4 * 32 * C::OROW;                     // [4][32] reference, then [4][32] sum
+    __syncthreads();  // every wave is done with its stages
+    {
+        const float l = xhalf_sum(soft.l_run);
+        if (l32 < nrows) {
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int rg = 0; rg < 4; ++rg) {
+                    const v4f o = {oacc[mb][4 * rg], oacc[mb][4 * rg + 1], oacc[mb][4 * rg + 2], oacc[mb][4 * rg + 3]};
+                    *reinterpret_cast<FA_LDS v4f*>(xo + (wave * 32 + l32) * C::OROW + 32 * mb + 8 * rg + 4 * g) = o;
+                }
+            if (g == 0) {
+                xm[wave * 32 + l32] = soft.m_ref;
+                xm[128 + wave * 32 + l32] = l;
+            }
+        }
+    }
+    __syncthreads();
+    constexpr int CO = D / 8;  // eight columns per thread
+    for (int k = tid; k < nrows * CO; k += 256) {
+        const int row = k / CO, c = (k % CO) * 8;
+        float m = xm[row];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) m = fmaxf(m, xm[w * 32 + row]);
+        float l = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float lw = xm[128 + w * 32 + row], f = lw == 0.0f ? 0.0f : fast_exp2(xm[w * 32 + row] - m);
+            l += f * lw;
+            const FA_LDS float* const src = xo + (w * 32 + row) * C::OROW + c;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf(f, src[e], o[e]);
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float lse = l == 0.0f ? -INFINITY : __builtin_fmaf(m, kLn2, fast_log2(l) * kLn2);
+        int head;
+        const int tok = row_token(a, it, it.row0 + row, &head);
+        const size_t at = (size_t)tok * a.H + head;
+        if (c >= a.d) continue;
+        if (a.num_splits > 1) {
+            const size_t part = at * a.num_splits + it.split;
+            float* const op = a.O_partial + part * a.d + c;
+            const v4f o0 = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv}, o1 = {o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv};
+            *reinterpret_cast<v4f*>(op) = o0;
+            *reinterpret_cast<v4f*>(op + 4) = o1;
+            if (c == 0) a.LSE_partial[part] = lse;
+        } else {
+            const v4u w = {Elem<kBf16>::pack(o[0] * inv, o[1] * inv), Elem<kBf16>::pack(o[2] * inv, o[3] * inv),
+                           Elem<kBf16>::pack(o[4] * inv, o[5] * inv), Elem<kBf16>::pack(o[6] * inv, o[7] * inv)};
+            *reinterpret_cast<v4u*>(a.O + (size_t)tok * a.o_token + (size_t)head * a.o_head + c * 2) = w;
+            if (c == 0) a.LSE[at] = lse;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- many rows
+
+template <int D>
+struct TallCfg {
+    static constexpr int kWaves = 8, NST = 4;                 // LDS stages per tensor
+    static constexpr int SMEM = NST * 2 * PagedTile<D>::BUF;  // 128 or 64 KiB
+    static constexpr int NL = PagedTile<D>::REQ / kWaves;     // requests per wave and tile, K and V each
+};
+
+// LDS-only barrier: requests in flight are not waited for, and nothing moves across.
+__device__ __forceinline__ void paged_barrier()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// The same with the last kReads reads of LDS left in flight.
+template <int kReads>
+__device__ __forceinline__ void paged_barrier_keep()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(%0)\n\ts_barrier" ::"n"(kReads < 15 ? kReads : 15) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Waves 0-3 and 4-7 run half an iteration apart (the second group passes one more barrier in front of the loop): while one wave of a
+// SIMD is at its softmax, the other is at its MFMAs.  V(t + 2) is requested at the start of iteration t and waited for at its end, K(t + 3) at
+// its end and waited for at the next one's; their slots were last read two barriers before.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(512, 2) paged_tall_kernel(const PagedArgs a)
+{
+    using T = PagedTile<D>;
+    using C = TallCfg<D>;
+    using E = Elem<kBf16>;
+    constexpr int KS = T::KS, MB = T::MB, NST = C::NST, NL = C::NL, BC = T::BC;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    FA_LDS char* const Ks = (FA_LDS char*)smem;
+    FA_LDS char* const Vs = Ks + NST * T::BUF;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6), grp = wave >> 2, l32 = lane & 31, g = lane >> 5;
+
+    PagedItem it;
+    if (!paged_item<kPagedTallRows>(a, lane, &it)) return;
+    int kmin, kmax;
+    paged_range<kPagedTallRows>(a, it, &kmin, &kmax);
+    if (kmax <= kmin) {
+        paged_store_empty<kPagedTallRows, 512>(a, it, tid);
+        return;
+    }
+    const int tile0 = kmin >> 6, ntiles = ((kmax + 63) >> 6) - tile0;
+    const int len = it.len;
+    const int32_t* const table_row = a.table + (size_t)it.b * a.table_stride;
+
+    if (a.d != D) {  // columns that no request writes
+        const v4u z = {0u, 0u, 0u, 0u};
+        for (int k = tid; k < C::SMEM / 16; k += 512) *reinterpret_cast<FA_LDS v4u*>(Ks + 16 * k) = z;
+        paged_barrier();
+    }
+
+    // (row blocks s and 7 - s on SIMD s: evens out the diagonal)
+    const int rblk = wave < 4 ? wave : 11 - wave;
+    const int first_row = it.row0 + rblk * 32, r = first_row + l32;
+
+    // ---- requests of this wave: KiB blocks wave and (256-byte rows) wave + 8 of a tile
+    const int lrow = lane / T::CPR, slot = lane % T::CPR;
+    const int brow = T::RPB * wave;  // first row of block `wave`; the other one's is 32 further on
+    const int ck = T::k_chunk(slot, brow + lrow), cv = T::v_chunk(slot, brow + lrow);
+    const uint32_t koff = (uint32_t)lrow * a.k_row + ck * 16, voff = (uint32_t)lrow * a.v_row + cv * 16;
+    const bool kok = ck * 8 < a.d, vok = cv * 8 < a.d;
+    int kent[NL], vent[NL];  // table entries of the next tiles of K and V to request
+    auto ask_entries = [&](int t, int (&e)[NL]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < NL; ++x) e[x] = paged_entry(a, table_row, len, (tile0 + t) * BC + brow + 32 * x);
+    };
+    auto request = [&](int t, const int (&e)[NL], const char* base, int64_t page_bytes, int64_t head_bytes, uint32_t row_bytes, uint32_t off, bool ok,
+                       FA_LDS char* stage) __attribute__((always_inline)) {
+        const int kb0 = (tile0 + t) * BC;
+        const bool whole = kb0 + BC <= len;
+#pragma unroll
+        for (int x = 0; x < NL; ++x) {
+            const int j = kb0 + brow + 32 * x, jj = j < len ? j : len - 1;
+            const int in_page = jj - a.by_page.quotient(jj) * a.page;
+            const char* const at = base + inside(a, e[x]) * page_bytes + it.hk * head_bytes + (int64_t)in_page * row_bytes;
+            uint32_t o = off;
+            if (!whole) {  // rows past the last key repeat it
+                const int most = j < len ? len - 1 - j : 0;
+                if (lrow > most) o -= (uint32_t)(lrow - most) * row_bytes;
+            }
+            if (ok) dma_kib(at, o, stage + (wave + 8 * x) * 1024);
+        }
+    };
+    auto load_k = [&](int t, const int (&e)[NL], FA_LDS char* stage) { request(t, e, a.K, a.k_page, a.k_head, a.k_row, koff, kok, stage); };
+    auto load_v = [&](int t, const int (&e)[NL], FA_LDS char* stage) { request(t, e, a.V, a.v_page, a.v_head, a.v_row, voff, vok, stage); };
+
+    // ---- what the rows of this wave see
+    int lo, hi, lo_max, hi_min, lo_min, hi_max;
+    paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
+    lo_min = __builtin_amdgcn_readlane(lo, 0);
+    hi_min = __builtin_amdgcn_readlane(hi, 0);
+    lo_max = __builtin_amdgcn_readlane(lo, 31);  // (bounds do not fall from row to row)
+    hi_max = __builtin_amdgcn_readlane(hi, 31);
+
+    v8h qf[KS];
+    v16f oacc[MB], s[2];
+    uint32_t p[2][2][4];
+    PagedSoftmax<kBf16, MB> soft;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[mb][e] = 0.0f;
+    const float c2 = a.scale_log2, inv_c2 = __builtin_amdgcn_rcpf(c2);
+    const int k_rd = T::k_lane(lane), v_rd = T::v_lane(lane);
+
+    // ---- fragments of the MFMA phase, one software-pipelined stream of LDS reads and MFMAs (fwd_pp_kernel.h)
+    v8h vf[4][MB];
+    constexpr int KPD = KS < 3 ? KS : 3;  // K k-steps in flight
+    v8h kf[KS][2];
+    auto v_read = [&](uint32_t vbase, int st) {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) vf[st][mb] = v_fragment<D>(vbase, st, mb);
+    };
+    auto k_read = [&](uint32_t kbase, int ks) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) kf[ks][kb] = k_fragment<D>(kbase, ks, kb);
+    };
+    auto pv_mfma = [&](int st) {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) oacc[mb] = E::mfma(vf[st][mb], as_fragment(p[st >> 1][st & 1]), oacc[mb]);
+    };
+    auto qk_mfma = [&](int ks) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) s[kb] = E::mfma(kf[ks][kb], qf[ks], s[kb]);
+    };
+    auto s_clear = [&]() {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kb][e] = 0.0f;
+    };
+    auto mfma_phase = [&](auto last_c, uint32_t vbase, uint32_t kbase) __attribute__((always_inline)) {
+        constexpr bool kLast = decltype(last_c)::value;
+        pv_mfma(0);
+        __builtin_amdgcn_sched_barrier(0);
+        v_read(vbase, 2);
+        pv_mfma(1);
+        v_read(vbase, 3);
+        pv_mfma(2);
+        if constexpr (!kLast) {
+#pragma unroll
+            for (int ks = 0; ks < KPD; ++ks) k_read(kbase, ks);
+        }
+        pv_mfma(3);
+        if constexpr (!kLast) {
+            s_clear();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + KPD < KS) k_read(kbase, ks + KPD);
+                qk_mfma(ks);
+            }
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * MB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, MB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * MB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, MB, 0);
+        if constexpr (!kLast) __builtin_amdgcn_sched_group_barrier(0x100, 2 * KPD, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, MB, 0);
+        if constexpr (!kLast) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + KPD < KS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            }
+        }
+    };
+    // what has to have landed at the end of iteration t, and the requests for what is to come
+    auto tail_requests = [&](int t, FA_LDS char* wrk) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < NL; ++x) vent[x] = kent[x];  // K(t + 3)'s entries are V(t + 3)'s
+        if (t + 3 < ntiles) {
+            load_k(t + 3, kent, wrk);
+            ask_entries(t + 4, kent);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+    };
+    auto iteration = [&](auto last_c, FA_LDS const char* __restrict__ rdv, FA_LDS const char* __restrict__ rdk, FA_LDS char* __restrict__ wrk,
+                         FA_LDS char* __restrict__ wrv, int t) __attribute__((always_inline)) {
+        const int kb0 = (tile0 + t) * BC;
+        if (t + 2 < ntiles) load_v(t + 2, vent, wrv);
+        soft.tile(s, oacc, p, c2, inv_c2, mask_sides(kb0, lo_max, hi_min), lo - kb0 - 4 * g, hi - kb0 - 4 * g);
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t vbase = fragment_base(rdv, v_rd);
+        const uint32_t kbase = fragment_base(rdk, k_rd);
+        v_read(vbase, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        v_read(vbase, 1);
+        paged_barrier_keep<4 * MB>();
+        __builtin_amdgcn_s_setprio(1);
+        mfma_phase(last_c, vbase, kbase);
+        __builtin_amdgcn_s_setprio(0);
+        tail_requests(t, wrk);
+        paged_barrier();
+    };
+
+    // ---- prologue
+    load_q<KS>(a, it, r, g, qf);
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {
+        if (t < ntiles) {
+            ask_entries(t, kent);
+            load_k(t, kent, Ks + t * T::BUF);
+            if (t < 2) load_v(t, kent, Vs + t * T::BUF);
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < NL; ++x) vent[x] = kent[x];  // of tile 2
+    ask_entries(3, kent);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
+    paged_barrier();
+    {
+        const uint32_t kbase = fragment_base(Ks, k_rd);
+#pragma unroll
+        for (int ks = 0; ks < KPD; ++ks) k_read(kbase, ks);
+        s_clear();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if (ks + KPD < KS) k_read(kbase, ks + KPD);
+            qk_mfma(ks);
+        }
+    }
+    if (grp == 1) paged_barrier();
+
+    // Tiles of which no row of this wave sees a key: only the wave's share of the requests and the barriers.
+    auto idle_iteration = [&](int t) {
+        if (t + 2 < ntiles) load_v(t + 2, vent, Vs + ((t + 2) % NST) * T::BUF);
+        paged_barrier();
+        tail_requests(t, Ks + ((t + 3) % NST) * T::BUF);
+        paged_barrier();
+    };
+    int t_lo = 0, t_hi = 0;
+    if (first_row < it.rows && hi_max >= lo_min) {
+        t_lo = max(0, (lo_min >> 6) - tile0 - 1);  // (the tile in front of the first visible one brings that one's scores)
+        t_hi = min(ntiles, (hi_max >> 6) - tile0 + 1);
+        t_lo = min(t_lo, t_hi);
+    }
+    int t = 0;
+    for (; t < t_lo; ++t) idle_iteration(t);
+    for (; t < t_hi - 1; ++t)
+        iteration(std::false_type{}, Vs + (t % NST) * T::BUF, Ks + ((t + 1) % NST) * T::BUF, Ks + ((t + 3) % NST) * T::BUF, Vs + ((t + 2) % NST) * T::BUF, t);
+    if (t < t_hi) {
+        iteration(std::true_type{}, Vs + (t % NST) * T::BUF, Ks + ((t + 1) % NST) * T::BUF, Ks + ((t + 3) % NST) * T::BUF, Vs + ((t + 2) % NST) * T::BUF, t);
+        ++t;
+    }
+    for (; t < ntiles; ++t) idle_iteration(t);
+    if (grp == 0) paged_barrier();
+    if (first_row >= it.rows) return;
+
+    // ---- epilogue
+    if (__builtin_expect(any_not_finite<MB>(oacc), 0)) paged_rescue<D, MB, kBf16>(a, it, r, kmin, kmax, tile0, ntiles, 0, 1, soft.m_ref, oacc);
+    const float l = xhalf_sum(soft.l_run);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float lse = l == 0.0f ? -INFINITY : __builtin_fmaf(soft.m_ref, kLn2, fast_log2(l) * kLn2);
+    int head;
+    const int tok = row_token(a, it, r < it.rows ? r : it.rows - 1, &head);
+    const size_t at = (size_t)tok * a.H + head;
+    if (a.num_splits > 1) {
+        if (r < it.rows) {
+            const size_t part = at * a.num_splits + it.split;
+            if (g == 0) a.LSE_partial[part] = lse;
+            float* const op = a.O_partial + part * a.d;
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int rg = 0; rg < 4; ++rg) {
+                    const int c = 32 * mb + 8 * rg + 4 * g;
+                    const v4f o = {oacc[mb][4 * rg] * inv, oacc[mb][4 * rg + 1] * inv, oacc[mb][4 * rg + 2] * inv, oacc[mb][4 * rg + 3] * inv};
+                    if (c < a.d) *reinterpret_cast<v4f*>(op + c) = o;
+                }
+        }
+        return;
+    }
+    if (r < it.rows && g == 0) a.LSE[at] = lse;
+    // O^T is turned round in LDS of the wave's own (every read of the tiles is behind the last barrier) and leaves as whole rows
+    FA_LDS char* const ost = Ks + wave * (32 * T::ROW);
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int rg = 0; rg < 4; ++rg) {
+            const v2u w = {E::pack(oacc[mb][4 * rg] * inv, oacc[mb][4 * rg + 1] * inv), E::pack(oacc[mb][4 * rg + 2] * inv, oacc[mb][4 * rg + 3] * inv)};
+            *reinterpret_cast<FA_LDS v2u*>(ost + l32 * T::ROW + T::k_chunk(4 * mb + rg, l32) * 16 + g * 8) = w;
+        }
+#pragma unroll
+    for (int x = 0; x < 32 / T::RPB; ++x) {
+        const int rl = T::RPB * x + lrow, c = T::k_chunk(slot, rl);
+        const v4u val = *reinterpret_cast<FA_LDS const v4u*>(ost + x * 1024 + lane * 16);
+        if (first_row + rl < it.rows && c * 8 < a.d) {
+            int oh;
+            const int ot = row_token(a, it, first_row + rl, &oh);
+            __builtin_nontemporal_store(val, reinterpret_cast<v4u*>(a.O + (size_t)ot * a.o_token + (size_t)oh * a.o_head + c * 16));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- merge of splits
+
+// O = sum_s w_s O_s, LSE = log sum_s exp LSE_s with w_s = exp(LSE_s - LSE): one or (kWaves = 4, few rows with many splits) four waves per
+// row.  Half a wave reads one split's row, 16 bytes per lane.  Splits of weight 0 are not read, nor written by who found nothing there.
+template <bool kBf16, int kWaves>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMergeArgs a)
+{
+    __shared__ float xs[kWaves == 4 ? 4 * 2 * 32 * 5 : 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6), half = lane >> 5, l32 = lane & 31;
+    const int64_t row = kWaves == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    const int tok = (int)(row / a.H);
+    // rows in front of the first sequence and behind the last one are nobody's
+    if (tok >= a.tokens || tok < read_uniform_int(a.cu) || tok >= read_uniform_int(a.cu + a.B)) return;
+    const int head = (int)(row - (int64_t)tok * a.H), S = a.num_splits, d = a.d;
+    const float* const lse = a.LSE_partial + (size_t)row * S;
+    const float l0 = lane < S ? lse[lane] : -INFINITY, l1 = lane + 64 < S ? lse[lane + 64] : -INFINITY;
+    float m = fmaxf(l0, l1);
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    const float m0 = m == -INFINITY ? 0.0f : m;
+    const float w0 = fast_exp2((l0 - m0) * kLog2e), w1 = fast_exp2((l1 - m0) * kLog2e);
+    float sum = w0 + w1;
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float* const op = a.O_partial + (size_t)row * S * d + 4 * l32;
+    const int first = kWaves == 4 ? 2 * wave : 0, step = 2 * kWaves;
+    // four reads at a time, whose weights are known
+    for (int s0 = first; s0 < S; s0 += 4 * step) {
+        float w[4];
+        v4f x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int s = s0 + k * step + half;
+            const float wk = s < 64 ? __shfl(w0, s & 63) : __shfl(w1, s & 63);
+            const bool there = s < S && !(wk == 0.0f) && 4 * l32 < d;
+            const v4f z = {0.0f, 0.0f, 0.0f, 0.0f};
+            w[k] = there ? wk : 0.0f;
+            x[k] = z;
+            if (there) x[k] = *reinterpret_cast<const v4f*>(op + (size_t)s * d);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w[k], x[k][e], o[e]);
+    }
+    if constexpr (kWaves == 4) {
+        float* const mine = xs + ((wave * 2 + half) * 32 + l32) * 5;  // (five words apart: no bank conflicts)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mine[e] = o[e];
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            o[e] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[e] += xs[((k * 2 + half) * 32 + l32) * 5 + e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = xhalf_sum(o[e]);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (half == 0 && 4 * l32 < d) {
+        const v2u w = {Elem<kBf16>::pack(o[0] * inv, o[1] * inv), Elem<kBf16>::pack(o[2] * inv, o[3] * inv)};
+        *reinterpret_cast<v2u*>(a.O + (size_t)tok * a.o_token + (size_t)head * a.o_head + 8 * l32) = w;
+    }
+    if (lane == 0) a.LSE[row] = sum == 0.0f ? -INFINITY : m0 + fast_log2(sum) * kLn2;
+}
+
+// ---------------------------------------------------------------------------------------------- launches
+
+template <int D, bool kBf16, bool kFew>
+inline hipError_t launch_paged_instance(const PagedArgs& a, long long blocks, hipStream_t st)
+{
+    const auto kern = kFew ? paged_few_kernel<D, kBf16> : paged_tall_kernel<D, kBf16>;
+    constexpr int smem = kFew ? FewCfg<D>::SMEM : TallCfg<D>::SMEM;
+    static DeviceFlags attr_done;  // per instantiation and device
+    if (hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), smem, attr_done); e != hipSuccess) return e;
+    return launch_kernel(kern, dim3((unsigned)blocks), dim3(kFew ? 256 : 512), smem, st, a);
+}
+
+template <int D>
+inline int launch_paged_bucket(const PagedArgs& a, bool bf16, bool few, long long blocks, hipStream_t st)
+{
+    if (bf16) return (int)(few ? launch_paged_instance<D, true, true>(a, blocks, st) : launch_paged_instance<D, true, false>(a, blocks, st));
+    return (int)(few ? launch_paged_instance<D, false, true>(a, blocks, st) : launch_paged_instance<D, false, false>(a, blocks, st));
+}
+
+int launch_paged_d64(const PagedArgs& a, bool bf16, bool few, long long blocks, hipStream_t st);
+int launch_paged_d128(const PagedArgs& a, bool bf16, bool few, long long blocks, hipStream_t st);
+int launch_paged_merge(const PagedArgs& a, bool bf16, hipStream_t st);
+
+}  // namespace fa

@@ -200,6 +200,88 @@ void flash_params_init(flash_params *p);
  * header would hand over a struct of another size (fields are only ever appended): compare before the first call. */
 size_t flash_params_size(void);
 
+/* ---- Rotary positions and a paged K/V cache.  No counterpart in the reference, which has contiguous K and V of one length per
+ * batch and leaves positions to ALiBi.  All strides are in elements, the last dimension of every tensor is contiguous, and all pointers are
+ * device pointers.  Lengths, page tables and positions are read on the device, so that a captured graph follows them. */
+enum { FLASH_FP16 = 0, FLASH_BF16 = 1, FLASH_FP32 = 2 };
+
+/* Y = factor * R(position) X on the leading `rot` elements of every row, X itself behind them.  Pair i of a row is (X[i], X[i + rot / 2]), or
+ * (X[2 i], X[2 i + 1]) if interleaved, and turns by the angle position * inv_freq[i]:
+ *     (a, b) -> factor * (a cos - b sin, a sin + b cos)
+ * `inverse` turns the other way, which is the transposed map: the gradient of X from the gradient of Y.
+ * The angle is worked out in 64 bits and more: positions up to 2^53 lose nothing.  X and Y may be the same rows (same pointer and strides); rows
+ * that overlap otherwise are the caller's error. */
+typedef struct flash_rotary_params {
+    const void *X;
+    void *Y;
+    int dtype;            /* FLASH_FP16, FLASH_BF16 or FLASH_FP32 */
+    int B, H, N, d;       /* rows of d elements, [B,H,N,d] */
+    int rot;              /* even, 2 ... min(d, 512) */
+    int64_t x_batch, x_head, x_row, y_batch, y_head, y_row;
+    const void *positions;     /* of row n of batch b: positions[b * positions_batch + n] */
+    int positions_64;          /* 0: int32, 1: int64 */
+    int64_t positions_batch;   /* 0: the same for every batch */
+    const float *inv_freq;     /* [rot / 2] */
+    float factor;
+    int interleaved, inverse;
+} flash_rotary_params;
+
+int flash_rotary(const flash_rotary_params *p, void *stream);
+
+/* Arguments of flash_append_paged and flash_forward_paged.  B sequences share a call: their new tokens lie one after the other, sequence b in
+ * rows cu_seqlens_q[b] ... cu_seqlens_q[b + 1] - 1 of Q, K, V and O.  seqlens_k[b] counts its keys with the new ones, which are the last: new token
+ * i of n stands at position seqlens_k[b] - n + i.  Key j lies in row j % page_size of page block_table[b * block_table_stride + j / page_size].
+ * What is read on the device is kept inside the tensors: lengths are cut to what the table can name, entries outside 0 ... num_pages - 1
+ * are read as page 0 (the results of that sequence are then meaningless) and never written.  Entries behind a sequence's last page are not read.
+ * Rows of Q, K, V and O in front of cu_seqlens_q[0] and from cu_seqlens_q[B] on are neither read nor written. */
+typedef struct flash_paged_params {
+    const void *Q;        /* [total_q, H, d] */
+    void *O;              /* forward: the result; append: Q turned (may be Q itself) */
+    const void *K, *V;    /* append: new rows [total_q, H_kv, d] */
+    void *K_cache, *V_cache;   /* [num_pages, H_kv, page_size, d], any strides */
+    const int32_t *block_table, *seqlens_k, *cu_seqlens_q;
+    int dtype;            /* FLASH_FP16 or FLASH_BF16 */
+    int B, H, H_kv, d;    /* H a multiple of H_kv; d a multiple of 8 up to FLASH_MAX_HEAD_DIM */
+    int total_q, num_pages, page_size, max_pages;   /* page_size: a multiple of 16; max_pages: entries of a row of the table */
+    int64_t q_token, q_head, o_token, o_head, k_token, k_head, v_token, v_head;   /* multiples of 8, as all strides of rows here */
+    int64_t kc_page, kc_head, kc_row, vc_page, vc_head, vc_row;
+    int64_t block_table_stride;
+    /* forward */
+    float *LSE;           /* fp32 [total_q, H], contiguous */
+    float *O_partial, *LSE_partial;   /* workspace of num_splits > 1: flash_forward_paged_workspace_bytes */
+    int max_seqlen_q;     /* the longest chunk of the call; 0: total_q.  Rows of a longer one may stay unwritten */
+    int max_seqlen_k;     /* the longest sequence; 0: what the table can name.  Decides speed alone */
+    float softmax_scale;  /* positive */
+    int is_causal, window_left, window_right;   /* as in flash_params: row i of n sees key j with j <= i + seqlens_k - n, ... */
+    int num_splits;       /* <= 0: chosen by the library */
+    /* append */
+    const float *inv_freq;     /* [rot / 2], or NULL: K is stored as it is, Q and O are not looked at */
+    int rot, interleaved;
+    float factor;
+    const void *positions;     /* NULL: the places in the sequence; otherwise [total_q], for the angles alone */
+    int positions_64;
+} flash_paged_params;
+
+/* New rows of K, turned as by flash_rotary, and of V into their pages; Q, if it is given, turned into O by the same launch.  Two tokens whose
+ * rows are the same row of the cache (sequences that share a page that is still written) leave one of the two there. */
+int flash_append_paged(const flash_paged_params *p, void *stream);
+
+/* O = softmax(mask(Q K^T * scale)) V of every sequence's new tokens over its pages, down to one token per sequence, and LSE.  Rows that
+ * see no key get O = 0 and LSE = -inf.  A value that is not finite in a row of V that a query does not see, or behind a
+ * sequence's end, does not reach that query's O. */
+int flash_forward_paged(const flash_paged_params *p, void *stream);
+
+/* The split count that flash_forward_paged uses for p, and the bytes of its workspace (0 for one split).  They depend on the sizes (B, H, H_kv, d,
+ * total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k), the masks and num_splits. */
+int flash_forward_paged_resolve_splits(const flash_paged_params *p);
+int flash_forward_paged_workspace_bytes(const flash_paged_params *p, size_t *o_partial_bytes, size_t *lse_partial_bytes);
+
+/* Defaults: all pointers NULL, all sizes 0, factor 1, no window, num_splits 0 (paged).  And the sizes of the structs, as flash_params_size. */
+void flash_rotary_params_init(flash_rotary_params *p);
+void flash_paged_params_init(flash_paged_params *p);
+size_t flash_rotary_params_size(void);
+size_t flash_paged_params_size(void);
+
 /* Text of the last HIP error seen by this thread inside the library ("" if none). */
 const char *flash_last_hip_error(void);
 
