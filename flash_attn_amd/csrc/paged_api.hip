@@ -107,13 +107,9 @@ int group_of(const flash_paged_params* p) { return p->H / p->H_kv; }
 int longest_chunk(const flash_paged_params* p) { return p->max_seqlen_q > 0 && p->max_seqlen_q < p->total_q ? p->max_seqlen_q : p->total_q; }
 int capacity_of(const flash_paged_params* p) { return p->num_pages > 0 ? p->page_size * p->max_pages : 0; }
 
-// Up to 32 rows per K/V head and sequence: the waves of a work-group share out the tiles.
-bool few_rows(const flash_paged_params* p) { return (long long)longest_chunk(p) * group_of(p) <= fa::kPagedFewRows; }
-
-// row blocks of all sequences, at most
-long long row_blocks(const flash_paged_params* p)
+long long blocks_of(const flash_paged_params* p, int br)
 {
-    const int br = few_rows(p) ? fa::kPagedFewRows : fa::kPagedTallRows, G = group_of(p);
+    const int G = group_of(p);
     const long long each = ((long long)longest_chunk(p) * G + br - 1) / br;
     const long long all = (long long)p->total_q * G / br + p->B;
     return each * p->B < all ? each * p->B : all;
@@ -122,29 +118,58 @@ long long row_blocks(const flash_paged_params* p)
 int window_left_of(const flash_paged_params* p) { return p->window_left >= capacity_of(p) ? -1 : p->window_left; }
 int window_right_of(const flash_paged_params* p) { return p->window_right >= (long long)capacity_of(p) + p->total_q ? -1 : p->window_right; }
 
-// tiles of 64 keys that a row block sees, at most
-int most_tiles(const flash_paged_params* p)
+// tiles of 64 keys that the masks leave a block of br rows, at most
+int window_tiles(const flash_paged_params* p, int br)
 {
-    const int cap = capacity_of(p), br = few_rows(p) ? fa::kPagedFewRows : fa::kPagedTallRows;
-    long long keys = p->max_seqlen_k > 0 && p->max_seqlen_k < cap ? p->max_seqlen_k : cap;
     const int wl = window_left_of(p), wr = window_right_of(p);
-    if (wl >= 0 && (p->is_causal || wr >= 0)) {
-        const long long span = (long long)wl + 1 + (p->is_causal || wr < 0 ? 0 : wr) + (br + group_of(p) - 1) / group_of(p) + 63;
-        if (span < keys) keys = span;
-    }
-    return (int)((keys + 63) / 64);
+    if (wl < 0 || (!p->is_causal && wr < 0)) return 0x7fffffff;
+    return (int)(((long long)wl + 1 + (p->is_causal ? 0 : wr) + (br + group_of(p) - 1) / group_of(p) + 63 + 63) / 64);
+}
+// ... and that it sees
+int most_tiles(const flash_paged_params* p, int br)
+{
+    const int cap = capacity_of(p), keys = p->max_seqlen_k > 0 && p->max_seqlen_k < cap ? p->max_seqlen_k : cap, w = window_tiles(p, br);
+    return w < (keys + 63) / 64 ? w : (keys + 63) / 64;
 }
 
+// Which form.  Up to 64 rows per K/V head and sequence the work-groups of 32 rows are the faster ones at every length: their waves stream
+// tiles of their own (B64 H_kv8 500 keys, 40 rows 21.7 us against 31.4; B8 H_kv8 4000 keys, 64 rows 27.9 / 31.6).  Longer chunks
+// take them while the launch is short: a work-group of 256 rows walks its tiles at 2 us each, whether or not it is alone, where one of
+// 32 rows has four waves at 32 or 64 keys each.  In units of 32 rows x 64 keys they cost some 3 ns against 1 ns in a full GPU.  32 rows / 256
+// rows: 1000 causal rows H8 (4000 units) 17.7 / 25.7 us, 512 rows on 1000 keys H8 (2700) 20.0 / 26.2, 1000 on 1000 (6100) 29.3 / 29.4, 256 on
+// 4000 B8 H8 (12000) 72.7 / 46.4.
+constexpr int kShortRows = 64, kShortUnits = 5000;
+bool few_rows(const flash_paged_params* p)
+{
+    const long long chunk = longest_chunk(p);
+    if (chunk * group_of(p) <= kShortRows) return true;
+    long long tiles = most_tiles(p, fa::kPagedFewRows);
+    const int cap = capacity_of(p);
+    const long long keys = p->max_seqlen_k > 0 && p->max_seqlen_k < cap ? p->max_seqlen_k : cap;
+    if (p->is_causal && tiles > (keys - chunk / 2) / 64 + 1) tiles = (keys > chunk / 2 ? keys - chunk / 2 : 0) / 64 + 1;  // (the mean row's)
+    return blocks_of(p, fa::kPagedFewRows) * p->H_kv * tiles <= kShortUnits;
+}
+
+// Split count that the library chooses.  A work-group per CU at least, as long as each split has some tiles; and for single tokens of several
+// sequences, whose lengths nobody here knows, pieces of some kFewestTiles tiles, so that the long sequences of a batch do not outlast the
+// others.  The merge reads 8 B H d bytes per split and token more, which is little next to the keys of a piece.
+constexpr int kFewestTiles = 32, kMostGroups = 2048;
 int splits_of(const flash_paged_params* p)
 {
-    const int nt = most_tiles(p);
+    const bool few = few_rows(p);
+    const int br = few ? fa::kPagedFewRows : fa::kPagedTallRows, nt = most_tiles(p, br);
     if (nt <= 1 || (long long)p->total_q * p->H >= 1LL << 26) return 1;  // (the merge has a wave per row: 2^32 threads)
     long long s = p->num_splits;
     if (s <= 0) {
-        const long long groups = row_blocks(p) * p->H_kv;
+        const long long groups = blocks_of(p, br) * p->H_kv;
         s = groups >= kNumCU ? 1 : kNumCU / groups;
-        const int least = few_rows(p) ? 2 : 4;  // tiles per split
+        const int least = few ? 2 : 4;  // tiles per split
         if (s > nt / least) s = nt / least;
+        if (few && p->B > 1) {
+            long long more = kFewestTiles;
+            more = nt / more < kMostGroups / groups ? nt / more : kMostGroups / groups;
+            if (more > s) s = more;
+        }
     }
     if (s > nt) s = nt;
     if (s > FLASH_MAX_SPLITS) s = FLASH_MAX_SPLITS;
@@ -164,13 +189,13 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     if ((rc = rows_strides(p->q_token, p->q_head, p->Q)) != FLASH_OK || (rc = rows_strides(p->o_token, p->o_head, p->O)) != FLASH_OK) return rc;
     if (!p->LSE) return FLASH_EINVAL;
     if (misaligned(p->LSE, 4)) return FLASH_EALIGN;
-    const int splits = splits_of(p), nt = most_tiles(p);
+    const bool few = few_rows(p);
+    const int br = few ? fa::kPagedFewRows : fa::kPagedTallRows, splits = splits_of(p), nt = most_tiles(p, br);
     if (splits > 1) {
         if (!p->O_partial || !p->LSE_partial) return FLASH_EWORKSPACE;
         if (misaligned(p->O_partial, 16) || misaligned(p->LSE_partial, 4)) return FLASH_EALIGN;
     }
-    const bool few = few_rows(p);
-    const long long blocks = row_blocks(p) * p->H_kv * splits;
+    const long long blocks = blocks_of(p, br) * p->H_kv * splits;
     if (blocks * (few ? 256 : 512) >= 1LL << 32) return FLASH_EINVAL;
     if ((rc = device_usable()) != FLASH_OK) return rc;
     fa::PagedArgs a{};
@@ -185,9 +210,9 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     a.capacity = capacity_of(p);
     a.causal = p->is_causal != 0, a.wl = window_left_of(p), a.wr = window_right_of(p);
     a.scale_log2 = p->softmax_scale * fa::kLog2e;
-    a.num_splits = splits, a.tiles_per_split = (nt + splits - 1) / splits;
-    a.direct = (long long)longest_chunk(p) * a.G <= (few ? fa::kPagedFewRows : fa::kPagedTallRows);
-    a.by_unit = fa::fast_div((long long)a.Hk * splits), a.by_heads = fa::fast_div(a.Hk), a.by_group = fa::fast_div(a.G), a.by_page = fa::fast_div(a.page);
+    a.num_splits = splits, a.tiles_per_split = (nt + splits - 1) / splits, a.window_tiles = window_tiles(p, br);
+    a.direct = (long long)longest_chunk(p) * a.G <= br;
+    a.by_heads = fa::fast_div(a.Hk), a.by_group = fa::fast_div(a.G), a.by_page = fa::fast_div(a.page);
     a.by_splits = fa::fast_div(splits);
     const bool bf16 = p->dtype == FLASH_BF16;
     rc = record_hip(p->d <= 64 ? fa::launch_paged_d64(a, bf16, few, blocks, st) : fa::launch_paged_d128(a, bf16, few, blocks, st));

@@ -26,6 +26,7 @@
 #pragma once
 #include <type_traits>
 
+#include "combine.h"
 #include "common.h"
 
 namespace fa {
@@ -47,9 +48,9 @@ struct PagedArgs {
     int B, H, Hk, G, d, tokens, num_pages, page, capacity;  // capacity: keys that a row of the table can name
     int causal, wl, wr;                // wl / wr < 0: unbounded
     float scale_log2;
-    int num_splits, tiles_per_split;
-    int direct;                        // every sequence has one row block: work-group u is sequence u
-    FastDiv by_unit, by_heads, by_group, by_page, by_splits;
+    int num_splits, tiles_per_split, window_tiles;
+    int direct;                        // every sequence has one row block
+    FastDiv by_heads, by_group, by_page, by_splits;
 };
 
 // What the merge needs of them (short arguments launch faster: common.h)
@@ -107,52 +108,75 @@ struct PagedItem {
     int tok0, rows;   // first token of the chunk; query rows of the problem (tokens times heads per K/V head)
     int row0;         // first row of the work-group
     int len, shift;   // keys; position of query 0
+    int splits, per;  // of the sequence; tiles of a split
 };
 
 // Lengths come from device memory: whatever they hold, nothing outside the tensors is touched.
 __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-// Work-group -> (sequence, row block, split, K/V head); false where there is nothing to do.  K/V heads vary fastest, splits next, so
-// that with a multiple of 8 of them the row blocks of a K/V head find its keys in one XCD's L2; row blocks of a sequence come last
-// first, which under a causal mask is heaviest first.
+// inclusive sum over the lanes of a wave
+__device__ __forceinline__ int wave_prefix(int v, int lane)
+{
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const int other = __shfl_up(v, s);
+        if (lane >= s) v += other;
+    }
+    return v;
+}
+
+// Tiles of a split of a sequence of `len` keys (*per), and its splits: pieces of as many tiles as the launch was sized for, or more, should
+// the sequence be longer than the caller said.  a.window_tiles: tiles that the masks leave a row block at most.
+__device__ __forceinline__ int splits_of_sequence(const PagedArgs& a, int len, int* per)
+{
+    const int nt = min((len + 63) >> 6, a.window_tiles);
+    const int each = max(a.tiles_per_split, a.by_splits.quotient(nt + a.num_splits - 1));
+    *per = each;
+    if (a.num_splits == 1) return 1;
+    return nt <= each ? 1 : (int)((uint32_t)(nt + each - 1) / (uint32_t)each);
+}
+
+// Work-group -> (sequence, row block, split, K/V head); false where there is nothing to do.  K/V heads vary fastest, so that with a multiple
+// of 8 of them the work-groups that read the same keys share an XCD's L2.  Behind that all pieces that the launch has come first, and the
+// work-groups that there are too many of (lengths are known on the device alone) last: work-groups are started in order and dealt to the parts of an
+// XCD in turn, and a launch with idle ones in between waits for one part with others empty.  Row blocks of a sequence come last first, which
+// under a causal mask is heaviest first.
 template <int BR>
 __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedItem* it)
 {
-    const int block = blockIdx.x;
-    const int u = a.by_unit.quotient(block), rest = block - u * (a.Hk * a.num_splits);
-    it->split = a.by_heads.quotient(rest);
-    it->hk = rest - it->split * a.Hk;
-    int b = u, m = 0;
-    if (!a.direct) {
-        // row blocks of 64 sequences at a time, a lane each
+    const int block = blockIdx.x, w = a.by_heads.quotient(block);
+    it->hk = block - w * a.Hk;
+    int b = 0, m = 0;
+    if (a.direct && (a.num_splits == 1 || a.B == 1)) {  // one row block per sequence, and one split or sequence
+        if (a.num_splits == 1) b = w, it->split = 0;
+        else it->split = w;
+    } else {
+        // 64 sequences at a time, a lane each
         int before = 0;
         bool found = false;
         for (int b0 = 0; b0 < a.B; b0 += 64) {
             const int mine = b0 + lane;
-            int n = 0;
+            int blocks = 0, splits = 1, per;
             if (mine < a.B) {
                 const int c0 = clamp_int(a.cu[mine], 0, a.tokens), c1 = clamp_int(a.cu[mine + 1], c0, a.tokens);
-                n = ((c1 - c0) * a.G + BR - 1) / BR;
+                blocks = ((c1 - c0) * a.G + BR - 1) / BR;
+                splits = splits_of_sequence(a, clamp_int(a.lens[mine], 0, a.capacity), &per);
             }
-            int upto = n;
-#pragma unroll
-            for (int s = 1; s < 64; s <<= 1) {
-                const int other = __shfl_up(upto, s);
-                if (lane >= s) upto += other;
-            }
-            const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > u);
+            const int upto = wave_prefix(blocks * splits, lane);
+            const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > w);
             if (past != 0) {
                 const int at = __builtin_ctzll(past);
-                b = b0 + at;
-                m = before + __builtin_amdgcn_readlane(upto, at) - 1 - u;
-                found = true;
+                const int n = __builtin_amdgcn_readlane(blocks, at), each = __builtin_amdgcn_readlane(splits, at);
+                const int local = w - (before + __builtin_amdgcn_readlane(upto, at) - n * each), first = (int)((uint32_t)local / (uint32_t)each);
+                b = wave_uniform(b0 + at);
+                m = wave_uniform(n - 1 - first);
+                it->split = wave_uniform(local - first * each);
+                found = (uint32_t)first < (uint32_t)n;  // (sums of offsets that make no sense may overflow)
                 break;
             }
             before += __builtin_amdgcn_readlane(upto, 63);
         }
         if (!found) return false;
-        b = wave_uniform(b);
-        m = wave_uniform(m);
     }
     const int c0 = clamp_int(read_uniform_int(a.cu + b), 0, a.tokens), c1 = clamp_int(read_uniform_int(a.cu + b + 1), c0, a.tokens);
     it->b = b;
@@ -161,7 +185,8 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
     it->row0 = m * BR;
     it->len = clamp_int(read_uniform_int(a.lens + b), 0, a.capacity);
     it->shift = it->len - (c1 - c0);
-    return it->row0 < it->rows;
+    it->splits = splits_of_sequence(a, it->len, &it->per);
+    return it->row0 < it->rows && it->split < it->splits;
 }
 
 // keys [kmin, kmax) that some row of the work-group sees, of those its split's share: the range of the row block is cut, not the
@@ -175,16 +200,27 @@ __device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedItem&
     if (a.wl >= 0) lo = max(0, p0 - a.wl);
     if (a.causal) hi = min(hi, p1 + 1);
     if (a.wr >= 0) hi = min(hi, p1 + a.wr + 1);
-    if (a.num_splits > 1) {
-        // as many tiles per split as the launch was sized for, or more, should the range be longer than the caller said
-        const int t0 = lo >> 6, nt = hi > lo ? ((hi + 63) >> 6) - t0 : 0;
-        const int per = max(a.tiles_per_split, a.by_splits.quotient(nt + a.num_splits - 1));
-        const int64_t s0 = ((int64_t)t0 + (int64_t)it.split * per) * 64, s1 = s0 + (int64_t)per * 64;
-        lo = (int)max((int64_t)lo, min(s0, (int64_t)hi));
-        hi = (int)min((int64_t)hi, s1);
+    if (it.splits > 1) {
+        const int64_t s0 = ((int64_t)(lo >> 6) + (int64_t)it.split * it.per) * 64;
+        lo = (int)max((int64_t)lo, min(s0, (int64_t)max(hi, lo)));
+        if (it.split < it.splits - 1) hi = (int)min((int64_t)hi, s0 + (int64_t)it.per * 64);
     }
     *kmin = lo;
     *kmax = hi;
+}
+
+// The first split's work-group says of the splits that its sequence does not have that there is nothing in them.
+template <int BR, int kThreads>
+__device__ __forceinline__ void paged_mark_missing(const PagedArgs& a, const PagedItem& it, int tid)
+{
+    const int missing = a.num_splits - it.splits;
+    if (it.split != 0 || missing == 0) return;
+    const int n = min(BR, it.rows - it.row0);
+    for (int r = tid / 16; r < n; r += kThreads / 16) {
+        const int i = a.by_group.quotient(it.row0 + r), head = it.hk * a.G + (it.row0 + r - i * a.G);
+        float* const lse = a.LSE_partial + ((size_t)(it.tok0 + i) * a.H + head) * a.num_splits + it.splits;
+        for (int s = tid % 16; s < missing; s += 16) lse[s] = -INFINITY;
+    }
 }
 
 // first and last key that row r (of the problem) sees; [lo, hi] may be empty
@@ -235,13 +271,13 @@ __device__ __forceinline__ void paged_store_empty(const PagedArgs& a, const Page
 
 // ---------------------------------------------------------------------------------------------- tiles in LDS
 //
-// A stage holds 64 keys row-major, D * 2 bytes each, with the 16-byte chunks of a row permuted so that the fragment reads are free of
+// A stage holds BC keys row-major, D * 2 bytes each, with the 16-byte chunks of a row permuted so that the fragment reads are free of
 // bank conflicts:
 //   K: chunk c of key r in slot c ^ (r % 16) (256-byte rows) or c ^ (r / 2 % 8) (128-byte rows)
 //   V: 32-byte chunk c in slot c ^ (2 (r % 4) + r / 4 % 2), or the two halves of a 128-byte row exchanged in rows 2, 3 mod 4
-template <int D>
+template <int D, int kKeys = 64>
 struct PagedTile {
-    static constexpr int BC = 64, KS = D / 16, MB = D / 32, ROW = D * 2, BUF = BC * ROW;
+    static constexpr int BC = kKeys, KB = BC / 32, KS = D / 16, MB = D / 32, ROW = D * 2, BUF = BC * ROW;
     static constexpr int RPB = 1024 / ROW;   // rows of a request
     static constexpr int REQ = BUF / 1024;   // requests of a tile
     static constexpr int CPR = ROW / 16;     // chunks of a row
@@ -250,7 +286,7 @@ struct PagedTile {
     {
         return D == 128 ? ((((slot >> 1) ^ (2 * (r & 3) + ((r >> 2) & 1))) << 1) | (slot & 1)) : slot ^ (((r >> 1) & 1) << 2);
     }
-    // lane part of a K fragment's address: key l32, chunk 2 ks + g -> k_lane ^ (ks << 5), + BUF / 2 for the second 32 keys
+    // lane part of a K fragment's address: key l32, chunk 2 ks + g -> k_lane ^ (ks << 5), + 32 ROW for the second 32 keys
     static __device__ __forceinline__ int k_lane(int lane)
     {
         const int l32 = lane & 31, g = lane >> 5, z = D == 128 ? l32 & 15 : (l32 >> 1) & 7;
@@ -288,25 +324,38 @@ __device__ __forceinline__ v8h v_fragment(uint32_t vbase, int st, int mb)
 template <int D>
 __device__ __forceinline__ v8h k_fragment(uint32_t kbase, int ks, int kb)
 {
-    return *reinterpret_cast<FA_LDS const v8h*>(lds_at(kbase ^ (uint32_t)(ks << 5)) + kb * (PagedTile<D>::BUF / 2));
+    return *reinterpret_cast<FA_LDS const v8h*>(lds_at(kbase ^ (uint32_t)(ks << 5)) + kb * (32 * PagedTile<D>::ROW));
 }
 
 constexpr float kPagedTau = 8.0f;                       // powers of two by which a row may outgrow its running maximum
 constexpr float kPagedNothing = -3.402823466e38f;       // running maximum of a row that has seen no key
 
-// Online softmax of one tile: scores in s (unscaled), P^T packed into p as the B operand of the second product.
-template <bool kBf16, int MB>
+// Online softmax of one tile of KB * 32 keys: scores in s (unscaled), P^T packed into p as the B operand of the second product.
+// sides != 0: some row does not see all of the tile, but keys lo_rel ... hi_rel, counted from the tile's first plus the lane's 4 g
+template <bool kBf16, int MB, int KB>
 struct PagedSoftmax {
     float m_ref = kPagedNothing, m_thr = -INFINITY, l_run = 0.0f;
-    __device__ __forceinline__ void tile(v16f (&s)[2], v16f (&oacc)[MB], uint32_t (&p)[2][2][4], float c2, float inv_c2, int sides, int lo_rel, int hi_rel)
+    __device__ __forceinline__ void tile(v16f (&s)[KB], v16f (&oacc)[MB], uint32_t (&p)[KB][2][4], float c2, float inv_c2, int sides, int lo_rel, int hi_rel)
     {
-        if (__builtin_expect(sides != 0, 0)) mask_tile<false>(s[0], s[1], wave_uniform(mask_modes_general(sides)), lo_rel, hi_rel, -INFINITY);
-        float mk[2] = {-INFINITY, -INFINITY};
+        if (__builtin_expect(sides != 0, 0)) {
+            if constexpr (KB == 2) {
+                mask_tile<false>(s[0], s[1], wave_uniform(mask_modes_general(sides)), lo_rel, hi_rel, -INFINITY);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = 8 * (r >> 2) + (r & 3);
+                    s[0][r] = key < lo_rel || key > hi_rel ? -INFINITY : s[0][r];
+                }
+            }
+        }
+        float mk[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) mk[kb] = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) mk[kb] = fmaxf(mk[kb], s[kb][r]);
-        const float mx = fmaxf(mk[0], mk[1]);
+            for (int kb = 0; kb < KB; ++kb) mk[kb] = fmaxf(mk[kb], s[kb][r]);
+        const float mx = fmaxf(mk[0], mk[KB - 1]);
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m_thr) != 0ull, 0)) {
             const float m_new = fmaxf(m_ref, xhalf_max(mx) * c2);  // c2 > 0
             float alpha = fast_exp2(m_ref - m_new);
@@ -321,7 +370,7 @@ struct PagedSoftmax {
         }
         float rs = 0.0f;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
                 const float p0 = fast_exp2(__builtin_fmaf(s[kb][r], c2, -m_ref)), p1 = fast_exp2(__builtin_fmaf(s[kb][r + 1], c2, -m_ref));
@@ -359,7 +408,7 @@ __device__ __forceinline__ void load_q(const PagedArgs& a, const PagedItem& it, 
 // which the row sees a part, or none.  Called once per wave, behind its loop, where some sum is not finite: looks for such
 // values among the wave's partly masked tiles and, if there are any, works out the rows in question once more key by key, visible
 // keys alone.  (Tiles first, first + step, ... of the range from key kb_first on.)
-template <int D, int MB, bool kBf16>
+template <int BC, int MB, bool kBf16>
 __device__ __forceinline__ void paged_rescue(const PagedArgs& a, const PagedItem& it, int r, int kmin, int kmax, int tile0, int ntiles, int first,
                                                        int step, float m_ref, v16f (&oacc)[MB])
 {
@@ -374,7 +423,7 @@ __device__ __forceinline__ void paged_rescue(const PagedArgs& a, const PagedItem
     // lane j: key j of the tile; masked for some row of the wave, and not finite somewhere?
     bool spoilt = false;
     for (int t = first; t < ntiles; t += step) {
-        const int kb0 = (tile0 + t) * 64, j = kb0 + lane;
+        const int kb0 = (tile0 + t) * BC, j = kb0 + (lane & (BC - 1));
         bool some = false;  // of the lanes' rows does one not see key j?  (the key is told to all rows in turn)
         for (int q = 0; q < 32; ++q) {
             const int l = __builtin_amdgcn_readlane(lo, q), h = __builtin_amdgcn_readlane(hi, q);
@@ -394,8 +443,8 @@ __device__ __forceinline__ void paged_rescue(const PagedArgs& a, const PagedItem
     const int tok = row_token(a, it, r < it.rows ? r : it.rows - 1, &head);
     const char* const q = a.Q + (size_t)tok * a.q_token + (size_t)head * a.q_head;
     for (int t = first; t < ntiles; t += step) {
-        const int kb0 = (tile0 + t) * 64;
-        const int j0 = max(kb0, lo), j1 = min(kb0 + 63, hi);
+        const int kb0 = (tile0 + t) * BC;
+        const int j0 = max(kb0, lo), j1 = min(kb0 + BC - 1, hi);
         for (int j = j0; j <= j1; ++j) {
             const char* const k = row_of(a.K, a.k_page, a.k_head, a.k_row, j);
             const char* const v = row_of(a.V, a.v_page, a.v_head, a.v_row, j);
@@ -436,46 +485,53 @@ __device__ __forceinline__ bool any_not_finite(const v16f (&oacc)[MB])
 
 // ---------------------------------------------------------------------------------------------- few rows
 
+// A wave has one stage of 8 KiB for K and for V each: tiles of 32 keys (256-byte rows) or 64.  K of the next tile is requested as soon as the scores
+// of this one have read theirs, V behind the second product.  With 64 to 68 KiB per work-group two share a CU: one streams while the other begins,
+// merges or ends.
 template <int D>
 struct FewCfg {
-    static constexpr int kWaves = 4, NST = D == 128 ? 1 : 2;
-    static constexpr int WAVE = NST * 2 * PagedTile<D>::BUF;  // LDS of a wave's stages
+    static constexpr int kWaves = 4, BC = D == 128 ? 32 : 64;
+    static constexpr int WAVE = 2 * PagedTile<D, BC>::BUF;    // LDS of a wave's stages
     static constexpr int OROW = D + 4;                        // floats of a row of partial O
-    static constexpr int SMEM = kWaves * WAVE;
-    static_assert(kWaves * (32 * OROW + 64) * 4 <= SMEM, "the merge takes the stages' place");
+    static constexpr int MERGE = kWaves * (32 * OROW + 64) * 4;
+    static constexpr int SMEM = kWaves * WAVE > MERGE ? kWaves * WAVE : MERGE;
+    static_assert(2 * SMEM <= 160 * 1024, "two work-groups per CU");
 };
 
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(256, 1) paged_few_kernel(const PagedArgs a)
+__global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
 {
-    using T = PagedTile<D>;
     using C = FewCfg<D>;
-    constexpr int KS = T::KS, MB = T::MB, REQ = T::REQ, NST = C::NST;
+    constexpr int BC = C::BC;
+    using T = PagedTile<D, BC>;
+    constexpr int KS = T::KS, MB = T::MB, KB = T::KB, REQ = T::REQ, GROUPS = BC / 16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6), l32 = lane & 31, g = lane >> 5;
 
     PagedItem it;
     if (!paged_item<kPagedFewRows>(a, lane, &it)) return;
+    paged_mark_missing<kPagedFewRows, 256>(a, it, tid);
     int kmin, kmax;
     paged_range<kPagedFewRows>(a, it, &kmin, &kmax);
     if (kmax <= kmin) {
         paged_store_empty<kPagedFewRows, 256>(a, it, tid);
         return;
     }
-    const int tile0 = kmin >> 6, ntiles = ((kmax + 63) >> 6) - tile0;
+    const int tile0 = kmin / BC, ntiles = (kmax + BC - 1) / BC - tile0;
     const int len = it.len;
     const int32_t* const table_row = a.table + (size_t)it.b * a.table_stride;
 
-    FA_LDS char* const mine = (FA_LDS char*)smem + wave * C::WAVE;
+    FA_LDS char* const kst = (FA_LDS char*)smem + wave * C::WAVE;
+    FA_LDS char* const vst = kst + T::BUF;
     if (a.d != D) {  // columns that no request writes
         const v4u z = {0u, 0u, 0u, 0u};
-        for (int k = lane; k < C::WAVE / 16; k += 64) *reinterpret_cast<FA_LDS v4u*>(mine + 16 * k) = z;
+        for (int k = lane; k < C::WAVE / 16; k += 64) *reinterpret_cast<FA_LDS v4u*>(kst + 16 * k) = z;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 
-    // ---- requests: request x of a tile covers its rows RPB x ... ; four table entries per tile, one for each 16 keys
+    // ---- requests: request x of a tile covers its rows RPB x ... ; one table entry for each 16 keys
     const int lrow = lane / T::CPR, slot = lane % T::CPR;
-    constexpr int kPer = REQ / 4;  // requests per 16 keys
+    constexpr int kPer = REQ / GROUPS;  // requests per 16 keys
     uint32_t koff[kPer], voff[kPer];
     bool kok[kPer], vok[kPer];
 #pragma unroll
@@ -486,21 +542,21 @@ __global__ void __launch_bounds__(256, 1) paged_few_kernel(const PagedArgs a)
         kok[x] = ck * 8 < a.d;
         vok[x] = cv * 8 < a.d;
     }
-    int entry[4];
+    int entry[GROUPS];
     auto ask_entries = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) entry[s] = paged_entry(a, table_row, len, (tile0 + t) * 64 + 16 * s);
+        for (int s = 0; s < GROUPS; ++s) entry[s] = paged_entry(a, table_row, len, (tile0 + t) * BC + 16 * s);
     };
-    // the 64 rows of tile t (its entries given) of K or V
-    auto request = [&](int t, const int (&entries)[4], const char* base, int64_t page_bytes, int64_t head_bytes, uint32_t row_bytes,
-                       const uint32_t (&off)[kPer], const bool (&ok)[kPer], FA_LDS char* dst) __attribute__((always_inline)) {
-        const int kb0 = (tile0 + t) * 64;
-        const bool whole = kb0 + 64 <= len;
+    // the rows of tile t (its entries given) of K or V
+    auto request = [&](int t, const char* base, int64_t page_bytes, int64_t head_bytes, uint32_t row_bytes, const uint32_t (&off)[kPer], const bool (&ok)[kPer],
+                       FA_LDS char* dst) __attribute__((always_inline)) {
+        const int kb0 = (tile0 + t) * BC;
+        const bool whole = kb0 + BC <= len;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+        for (int s = 0; s < GROUPS; ++s) {
             const int j = kb0 + 16 * s, jj = j < len ? j : len - 1;
             const int in_page = jj - a.by_page.quotient(jj) * a.page;
-            const char* const at = base + inside(a, entries[s]) * page_bytes + it.hk * head_bytes + (int64_t)in_page * row_bytes;
+            const char* const at = base + inside(a, entry[s]) * page_bytes + it.hk * head_bytes + (int64_t)in_page * row_bytes;
 #pragma unroll
             for (int x = 0; x < kPer; ++x) {
                 uint32_t o = off[x];
@@ -512,15 +568,13 @@ __global__ void __launch_bounds__(256, 1) paged_few_kernel(const PagedArgs a)
             }
         }
     };
-    auto k_stage = [&](int n) { return mine + (n % NST) * T::BUF; };
-    auto v_stage = [&](int n) { return mine + NST * T::BUF + (n % NST) * T::BUF; };
-    auto request_k = [&](int t, const int (&e)[4], int n) { request(t, e, a.K, a.k_page, a.k_head, a.k_row, koff, kok, k_stage(n)); };
-    auto request_v = [&](int t, const int (&e)[4], int n) { request(t, e, a.V, a.v_page, a.v_head, a.v_row, voff, vok, v_stage(n)); };
+    auto request_k = [&](int t) { request(t, a.K, a.k_page, a.k_head, a.k_row, koff, kok, kst); };
+    auto request_v = [&](int t) { request(t, a.V, a.v_page, a.v_head, a.v_row, voff, vok, vst); };
 
     const int r = it.row0 + l32;
     v8h qf[KS];
     v16f oacc[MB];
-    PagedSoftmax<kBf16, MB> soft;
+    PagedSoftmax<kBf16, MB, KB> soft;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
@@ -532,69 +586,50 @@ __global__ void __launch_bounds__(256, 1) paged_few_kernel(const PagedArgs a)
     if (wave < ntiles) {
         ask_entries(wave);
         load_q<KS>(a, it, r, g, qf);
-        request_k(wave, entry, 0);
-        request_v(wave, entry, 0);
+        request_k(wave);
+        request_v(wave);
         lo_max = __builtin_amdgcn_readlane(lo, 31);  // (bounds do not fall from row to row)
         hi_min = __builtin_amdgcn_readlane(hi, 0);
     }
     const float c2 = a.scale_log2, inv_c2 = __builtin_amdgcn_rcpf(c2);
     const int k_rd = T::k_lane(lane), v_rd = T::v_lane(lane);
-    int n = 0;
-    for (int t = wave; t < ntiles; t += 4, ++n) {
-        const int kb0 = (tile0 + t) * 64;
+    for (int t = wave; t < ntiles; t += 4) {
+        const int kb0 = (tile0 + t) * BC;
         const bool more = t + 4 < ntiles;
         if (more) ask_entries(t + 4);
-        if constexpr (NST == 2) {
-            if (more) {
-                request_k(t + 4, entry, n + 1);
-                request_v(t + 4, entry, n + 1);
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * REQ) : "memory");  // K of this tile is there
-            } else {
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");
-            }
-        } else {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");
-        }
-        if (n == 0) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");  // K of this tile is there
+        if (t == wave) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
         }
-        v16f s[2];
+        v16f s[KB];
         {
-            const uint32_t kbase = fragment_base(k_stage(n), k_rd);
+            const uint32_t kbase = fragment_base(kst, k_rd);
             const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) s[kb] = Elem<kBf16>::mfma(k_fragment<D>(kbase, ks, kb), qf[ks], ks == 0 ? z : s[kb]);
+                for (int kb = 0; kb < KB; ++kb) s[kb] = Elem<kBf16>::mfma(k_fragment<D>(kbase, ks, kb), qf[ks], ks == 0 ? z : s[kb]);
         }
-        if constexpr (NST == 1) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the fragments have been read
-            if (more) request_k(t + 4, entry, n + 1);
-        }
-        uint32_t p[2][2][4];
-        soft.tile(s, oacc, p, c2, inv_c2, mask_sides(kb0, lo_max, hi_min), lo - kb0 - 4 * g, hi - kb0 - 4 * g);
-        if constexpr (NST == 2) {
-            if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * REQ) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        } else {
-            if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the fragments have been read
+        if (more) request_k(t + 4);
+        uint32_t p[KB][2][4];
+        const int sides = is_negative(kb0 - lo_max) | is_negative(hi_min - (BC - 1) - kb0) << 1;
+        soft.tile(s, oacc, p, c2, inv_c2, sides, lo - kb0 - 4 * g, hi - kb0 - 4 * g);
+        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         {
-            const uint32_t vbase = fragment_base(v_stage(n), v_rd);
+            const uint32_t vbase = fragment_base(vst, v_rd);
 #pragma unroll
-            for (int st = 0; st < 4; ++st)
+            for (int st = 0; st < 2 * KB; ++st)
 #pragma unroll
                 for (int mb = 0; mb < MB; ++mb) oacc[mb] = Elem<kBf16>::mfma(v_fragment<D>(vbase, st, mb), as_fragment(p[st >> 1][st & 1]), oacc[mb]);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if constexpr (NST == 1) {
-            if (more) request_v(t + 4, entry, n + 1);
-        }
+        if (more) request_v(t + 4);
     }
     if (wave < ntiles && __builtin_expect(any_not_finite<MB>(oacc), 0))
-        paged_rescue<D, MB, kBf16>(a, it, r, kmin, kmax, tile0, ntiles, wave, 4, soft.m_ref, oacc);
+        paged_rescue<BC, MB, kBf16>(a, it, r, kmin, kmax, tile0, ntiles, wave, 4, soft.m_ref, oacc);
 
     // ---- merge of the four waves: reference of a row = the largest of theirs
     const int nrows = min(kPagedFewRows, it.rows - it.row0);
@@ -683,13 +718,15 @@ __device__ __forceinline__ void paged_barrier_keep()
 // Waves 0-3 and 4-7 run half an iteration apart (the second group passes one more barrier in front of the loop): while one wave of a
 // SIMD is at its softmax, the other is at its MFMAs.  V(t + 2) is requested at the start of iteration t and waited for at its end, K(t + 3) at
 // its end and waited for at the next one's; their slots were last read two barriers before.
-template <int D, bool kBf16>
-__global__ void __launch_bounds__(512, 2) paged_tall_kernel(const PagedArgs a)
+// DU: columns that are worked on, a multiple of 32 from d on (rows in LDS have D): with DU = D the products of d = 80 meet zeroes in
+// every third MFMA.
+template <int D, int DU, bool kBf16>
+__global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const PagedArgs a)
 {
     using T = PagedTile<D>;
     using C = TallCfg<D>;
     using E = Elem<kBf16>;
-    constexpr int KS = T::KS, MB = T::MB, NST = C::NST, NL = C::NL, BC = T::BC;
+    constexpr int KS = DU / 16, MB = DU / 32, NST = C::NST, NL = C::NL, BC = T::BC;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     FA_LDS char* const Ks = (FA_LDS char*)smem;
     FA_LDS char* const Vs = Ks + NST * T::BUF;
@@ -697,6 +734,7 @@ __global__ void __launch_bounds__(512, 2) paged_tall_kernel(const PagedArgs a)
 
     PagedItem it;
     if (!paged_item<kPagedTallRows>(a, lane, &it)) return;
+    paged_mark_missing<kPagedTallRows, 512>(a, it, tid);
     int kmin, kmax;
     paged_range<kPagedTallRows>(a, it, &kmin, &kmax);
     if (kmax <= kmin) {
@@ -759,7 +797,7 @@ __global__ void __launch_bounds__(512, 2) paged_tall_kernel(const PagedArgs a)
     v8h qf[KS];
     v16f oacc[MB], s[2];
     uint32_t p[2][2][4];
-    PagedSoftmax<kBf16, MB> soft;
+    PagedSoftmax<kBf16, MB, 2> soft;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
@@ -769,7 +807,7 @@ __global__ void __launch_bounds__(512, 2) paged_tall_kernel(const PagedArgs a)
 
     // ---- fragments of the MFMA phase, one software-pipelined stream of LDS reads and MFMAs (fwd_pp_kernel.h)
     v8h vf[4][MB];
-    constexpr int KPD = KS < 3 ? KS : 3;  // K k-steps in flight
+    constexpr int VPD = 2, KPD = KS < 3 ? KS : 3;  // steps of V and K in flight
     v8h kf[KS][2];
     auto v_read = [&](uint32_t vbase, int st) {
 #pragma unroll
@@ -795,17 +833,18 @@ __global__ void __launch_bounds__(512, 2) paged_tall_kernel(const PagedArgs a)
     };
     auto mfma_phase = [&](auto last_c, uint32_t vbase, uint32_t kbase) __attribute__((always_inline)) {
         constexpr bool kLast = decltype(last_c)::value;
+        // step st: reads of V step st + VPD (behind the last ones: of K), MFMAs of step st
         pv_mfma(0);
         __builtin_amdgcn_sched_barrier(0);
-        v_read(vbase, 2);
-        pv_mfma(1);
-        v_read(vbase, 3);
-        pv_mfma(2);
-        if constexpr (!kLast) {
 #pragma unroll
-            for (int ks = 0; ks < KPD; ++ks) k_read(kbase, ks);
+        for (int st = 1; st < 4; ++st) {
+            if (st + VPD - 1 < 4) v_read(vbase, st + VPD - 1);
+            if (st == 3 && !kLast) {
+#pragma unroll
+                for (int ks = 0; ks < KPD; ++ks) k_read(kbase, ks);
+            }
+            pv_mfma(st);
         }
-        pv_mfma(3);
         if constexpr (!kLast) {
             s_clear();
 #pragma unroll
@@ -814,12 +853,12 @@ __global__ void __launch_bounds__(512, 2) paged_tall_kernel(const PagedArgs a)
                 qk_mfma(ks);
             }
         }
-        __builtin_amdgcn_sched_group_barrier(0x100, 2 * MB, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, MB, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2 * MB, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, MB, 0);
-        if constexpr (!kLast) __builtin_amdgcn_sched_group_barrier(0x100, 2 * KPD, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, MB, 0);
+#pragma unroll
+        for (int st = 1; st < 4; ++st) {
+            if (st + VPD - 1 < 4) __builtin_amdgcn_sched_group_barrier(0x100, 2 * MB, 0);
+            if (st == 3 && !kLast) __builtin_amdgcn_sched_group_barrier(0x100, 2 * KPD, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, MB, 0);
+        }
         if constexpr (!kLast) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -851,7 +890,7 @@ __global__ void __launch_bounds__(512, 2) paged_tall_kernel(const PagedArgs a)
         v_read(vbase, 0);
         __builtin_amdgcn_sched_barrier(0);
         v_read(vbase, 1);
-        paged_barrier_keep<4 * MB>();
+        paged_barrier_keep<2 * VPD * MB>();
         __builtin_amdgcn_s_setprio(1);
         mfma_phase(last_c, vbase, kbase);
         __builtin_amdgcn_s_setprio(0);
@@ -915,7 +954,7 @@ __global__ void __launch_bounds__(512, 2) paged_tall_kernel(const PagedArgs a)
     if (first_row >= it.rows) return;
 
     // ---- epilogue
-    if (__builtin_expect(any_not_finite<MB>(oacc), 0)) paged_rescue<D, MB, kBf16>(a, it, r, kmin, kmax, tile0, ntiles, 0, 1, soft.m_ref, oacc);
+    if (__builtin_expect(any_not_finite<MB>(oacc), 0)) paged_rescue<BC, MB, kBf16>(a, it, r, kmin, kmax, tile0, ntiles, 0, 1, soft.m_ref, oacc);
     const float l = xhalf_sum(soft.l_run);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const float lse = l == 0.0f ? -INFINITY : __builtin_fmaf(soft.m_ref, kLn2, fast_log2(l) * kLn2);
@@ -963,7 +1002,8 @@ __global__ void __launch_bounds__(512, 2) paged_tall_kernel(const PagedArgs a)
 // ---------------------------------------------------------------------------------------------- merge of splits
 
 // O = sum_s w_s O_s, LSE = log sum_s exp LSE_s with w_s = exp(LSE_s - LSE): one or (kWaves = 4, few rows with many splits) four waves per
-// row.  Half a wave reads one split's row, 16 bytes per lane.  Splits of weight 0 are not read, nor written by who found nothing there.
+// row.  Half a wave reads one split's row, 16 bytes per lane.  Bound by latency where there are few rows: the first rows are requested
+// before their weights are known.  (What a split that found nothing has in its place is not looked at: its weight is 0.)
 template <bool kBf16, int kWaves>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMergeArgs a)
 {
@@ -971,40 +1011,42 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMergeArgs a
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6), half = lane >> 5, l32 = lane & 31;
     const int64_t row = kWaves == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     const int tok = (int)(row / a.H);
-    // rows in front of the first sequence and behind the last one are nobody's
-    if (tok >= a.tokens || tok < read_uniform_int(a.cu) || tok >= read_uniform_int(a.cu + a.B)) return;
+    if (tok >= a.tokens) return;
     const int head = (int)(row - (int64_t)tok * a.H), S = a.num_splits, d = a.d;
-    const float* const lse = a.LSE_partial + (size_t)row * S;
-    const float l0 = lane < S ? lse[lane] : -INFINITY, l1 = lane + 64 < S ? lse[lane + 64] : -INFINITY;
-    float m = fmaxf(l0, l1);
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-    const float m0 = m == -INFINITY ? 0.0f : m;
-    const float w0 = fast_exp2((l0 - m0) * kLog2e), w1 = fast_exp2((l1 - m0) * kLog2e);
-    float sum = w0 + w1;
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
-    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
     const float* const op = a.O_partial + (size_t)row * S * d + 4 * l32;
     const int first = kWaves == 4 ? 2 * wave : 0, step = 2 * kWaves;
-    // four reads at a time, whose weights are known
-    for (int s0 = first; s0 < S; s0 += 4 * step) {
-        float w[4];
-        v4f x[4];
+    constexpr int U = 4;  // rows in flight per half wave
+    v4f x[U];
+    auto request = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < U; ++k) {
             const int s = s0 + k * step + half;
-            const float wk = s < 64 ? __shfl(w0, s & 63) : __shfl(w1, s & 63);
-            const bool there = s < S && !(wk == 0.0f) && 4 * l32 < d;
             const v4f z = {0.0f, 0.0f, 0.0f, 0.0f};
-            w[k] = there ? wk : 0.0f;
             x[k] = z;
-            if (there) x[k] = *reinterpret_cast<const v4f*>(op + (size_t)s * d);
+            if (s < S && 4 * l32 < d) x[k] = *reinterpret_cast<const v4f*>(op + (size_t)s * d);
         }
+    };
+    request(first);
+    const float* const lse = a.LSE_partial + (size_t)row * S;
+    const float l0 = lane < S ? lse[lane] : -INFINITY, l1 = lane + 64 < S ? lse[lane + 64] : -INFINITY;
+    // rows in front of the first sequence and behind the last one are nobody's
+    if (tok < read_uniform_int(a.cu) || tok >= read_uniform_int(a.cu + a.B)) return;
+    const float m = wave_max(fmaxf(l0, l1));
+    const float m0 = m == -INFINITY ? 0.0f : m;
+    const float w0 = fast_exp2((l0 - m0) * kLog2e), w1 = fast_exp2((l1 - m0) * kLog2e);
+    const float sum = wave_sum(w0 + w1);
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = first; s0 < S; s0 += U * step) {
+        if (s0 != first) request(s0);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < U; ++k) {
+            const int s = s0 + k * step + half;
+            const float w = s < 64 ? __shfl(w0, s & 63) : __shfl(w1, s & 63);
+            if (s < S && !(w == 0.0f)) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w[k], x[k][e], o[e]);
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, x[k][e], o[e]);
+            }
+        }
     }
     if constexpr (kWaves == 4) {
         float* const mine = xs + ((wave * 2 + half) * 32 + l32) * 5;  // (five words apart: no bank conflicts)
@@ -1031,21 +1073,30 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMergeArgs a
 
 // ---------------------------------------------------------------------------------------------- launches
 
-template <int D, bool kBf16, bool kFew>
+template <int D, int DU, bool kBf16, bool kFew>
 inline hipError_t launch_paged_instance(const PagedArgs& a, long long blocks, hipStream_t st)
 {
-    const auto kern = kFew ? paged_few_kernel<D, kBf16> : paged_tall_kernel<D, kBf16>;
+    const auto kern = [] {
+        if constexpr (kFew) return paged_few_kernel<D, kBf16>;
+        else return paged_tall_kernel<D, DU, kBf16>;
+    }();
     constexpr int smem = kFew ? FewCfg<D>::SMEM : TallCfg<D>::SMEM;
     static DeviceFlags attr_done;  // per instantiation and device
     if (hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), smem, attr_done); e != hipSuccess) return e;
     return launch_kernel(kern, dim3((unsigned)blocks), dim3(kFew ? 256 : 512), smem, st, a);
 }
 
+template <int D, bool kBf16>
+inline int launch_paged_type(const PagedArgs& a, bool few, long long blocks, hipStream_t st)
+{
+    if (few) return (int)launch_paged_instance<D, D, kBf16, true>(a, blocks, st);
+    if (a.d <= D - 32) return (int)launch_paged_instance<D, D - 32, kBf16, false>(a, blocks, st);
+    return (int)launch_paged_instance<D, D, kBf16, false>(a, blocks, st);
+}
 template <int D>
 inline int launch_paged_bucket(const PagedArgs& a, bool bf16, bool few, long long blocks, hipStream_t st)
 {
-    if (bf16) return (int)(few ? launch_paged_instance<D, true, true>(a, blocks, st) : launch_paged_instance<D, true, false>(a, blocks, st));
-    return (int)(few ? launch_paged_instance<D, false, true>(a, blocks, st) : launch_paged_instance<D, false, false>(a, blocks, st));
+    return bf16 ? launch_paged_type<D, true>(a, few, blocks, st) : launch_paged_type<D, false>(a, few, blocks, st);
 }
 
 int launch_paged_d64(const PagedArgs& a, bool bf16, bool few, long long blocks, hipStream_t st);

@@ -1,7 +1,8 @@
 // Native front end of the Python binding: flash_attn_amd._native.
 //
-// flash_forward / flash_forward_splitkv of binding.py hand their arguments to the two functions below, which fill
-// flash_params, allocate the results and call the C ABI (the launch path of the reference's main(), src/main.cu:109-192).
+// flash_forward / flash_forward_splitkv of binding.py hand their arguments to the functions forward and splitkv below, which fill
+// flash_params, allocate the results and call the C ABI (the launch path of the reference's main(), src/main.cu:109-192), and so do
+// flash_rotary, flash_append_paged and flash_forward_paged of paged.py.
 //
 // What bounds a small call is this code: filling the struct field by field through ctypes, five data_ptr() calls, two
 // torch.empty() and torch.cuda.current_stream() took 13-15 us of host time per flash_forward and 18-19 us per
@@ -9,11 +10,13 @@
 //
 // Anything out of the ordinary -- an argument of another type, shapes or dtypes that do not fit, a workspace that is too
 // small, a program that wants to see its allocations -- returns NotImplemented with nothing allocated or launched; binding.py then takes its own path, which raises the
-// errors (and serves the debug outputs).
+// errors (and serves the debug outputs).  Of the calls of paged.py it also leaves those on another stream or device than the current one
+// and those that need a gradient; the others took 15 us (rotary) to 29 us (paged forward in splits) each through ctypes.
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
 #include <ATen/Context.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPCachingAllocator.h>
@@ -273,6 +276,201 @@ PyObject* splitkv(PyObject*, PyObject* const* args, Py_ssize_t n)
     });
 }
 
+// ---- paged.py
+
+typedef int (*rotary_fn)(const flash_rotary_params*, void*);
+typedef int (*paged_fn)(const flash_paged_params*, void*);
+typedef int (*paged_resolve_fn)(const flash_paged_params*);
+rotary_fn g_rotary = nullptr;
+paged_fn g_append = nullptr, g_paged = nullptr;
+paged_resolve_fn g_paged_resolve = nullptr;
+
+int dtype_of(const at::Tensor& t)
+{
+    switch (t.scalar_type()) {
+        case at::kHalf: return FLASH_FP16;
+        case at::kBFloat16: return FLASH_BF16;
+        case at::kFloat: return FLASH_FP32;
+        default: return -1;
+    }
+}
+bool unit_stride(const at::Tensor& t) { return t.dim() > 0 && (t.size(-1) <= 1 || t.stride(-1) == 1); }
+bool fits_int(const at::Tensor& t)
+{
+    for (const auto n : t.sizes())
+        if (n > INT32_MAX) return false;
+    return true;
+}
+// on the GPU that is current, whose current stream the call goes to
+bool is_here(const at::Tensor& t) { return t.is_cuda() && t.device().index() == c10::hip::current_device(); }
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef size, at::ScalarType type) { return at::detail::empty_cuda(size, type, like.device(), std::nullopt); }
+bool positions_ok(const at::Tensor& t) { return (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && unit_stride(t) && is_here(t); }
+bool frequencies_ok(const at::Tensor& f, int64_t d)
+{
+    return f.scalar_type() == at::kFloat && f.dim() == 1 && f.is_contiguous() && f.numel() >= 1 && f.numel() <= d / 2 && is_here(f);
+}
+
+// rotary(x, positions, inv_freq, interleaved, factor, inverse, out)
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    return guarded([&]() -> PyObject* {
+        if (n != 7 || !g_rotary || !allocates_plainly()) return not_implemented();
+        const at::Tensor *x = tensor_of(args[0]), *pos = tensor_of(args[1]), *f = tensor_of(args[2]), *out;
+        if (!x || !pos || !f || !optional_tensor(args[6], &out)) return not_implemented();
+        flash_rotary_params p{};
+        if (!real(args[4], &p.factor) || !PyBool_Check(args[3]) || !PyBool_Check(args[5])) return not_implemented();
+        p.interleaved = args[3] == Py_True, p.inverse = args[5] == Py_True;
+        const int64_t dims = x->dim();
+        if ((dims != 3 && dims != 4) || (p.dtype = dtype_of(*x)) < 0 || !unit_stride(*x) || !fits_int(*x) || !is_here(*x)) return not_implemented();
+        if (at::GradMode::is_enabled() && x->requires_grad()) return not_implemented();
+        const bool tokens = dims == 3;
+        p.B = tokens ? 1 : (int)x->size(0), p.H = (int)x->size(1), p.N = (int)x->size(tokens ? 0 : 2), p.d = (int)x->size(-1);
+        if (!positions_ok(*pos) || !frequencies_ok(*f, p.d)) return not_implemented();
+        if (!(pos->dim() == 1 && pos->size(0) == p.N) && !(pos->dim() == 2 && !tokens && pos->size(0) == p.B && pos->size(1) == p.N)) return not_implemented();
+        at::Tensor y;
+        if (out) {
+            if (out->sizes() != x->sizes() || out->scalar_type() != x->scalar_type() || !unit_stride(*out) || !is_here(*out)) return not_implemented();
+            y = *out;
+        } else {  // (in x's order of dimensions, where x is dense; paged.py sees to the others)
+            if (!x->is_non_overlapping_and_dense()) return not_implemented();
+            y = at::detail::empty_strided_cuda(x->sizes(), x->strides(), x->scalar_type(), x->device());
+        }
+        auto strides = [&](const at::Tensor& t, int64_t& b, int64_t& h, int64_t& r) { b = tokens ? 0 : t.stride(0), h = t.stride(1), r = t.stride(tokens ? 0 : 2); };
+        strides(*x, p.x_batch, p.x_head, p.x_row);
+        strides(y, p.y_batch, p.y_head, p.y_row);
+        p.X = x->data_ptr(), p.Y = y.data_ptr(), p.rot = 2 * (int)f->numel();
+        p.positions = pos->data_ptr(), p.positions_64 = pos->scalar_type() == at::kLong, p.positions_batch = pos->dim() == 2 ? pos->stride(0) : 0;
+        p.inv_freq = static_cast<const float*>(f->data_ptr());
+        void* const stream = c10::hip::getCurrentHIPStream().stream();
+        const int rc = g_rotary(&p, stream);
+        return rc != FLASH_OK ? raise(rc, "flash_rotary") : THPVariable_Wrap(y);
+    });
+}
+
+// Caches and index tensors: args = (k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q)
+bool parse_cache(PyObject* const* args, flash_paged_params& p)
+{
+    const at::Tensor* t[5];
+    for (int i = 0; i < 5; ++i)
+        if (!(t[i] = tensor_of(args[i])) || !is_here(*t[i]) || !fits_int(*t[i])) return false;
+    const at::Tensor &k = *t[0], &v = *t[1], &table = *t[2], &lens = *t[3], &cu = *t[4];
+    p.dtype = dtype_of(k);
+    if ((p.dtype != FLASH_FP16 && p.dtype != FLASH_BF16) || v.scalar_type() != k.scalar_type() || k.dim() != 4 || v.sizes() != k.sizes()) return false;
+    if (k.stride(3) != 1 || v.stride(3) != 1) return false;
+    for (int i = 2; i < 5; ++i)
+        if (t[i]->scalar_type() != at::kInt || t[i]->dim() != (i == 2 ? 2 : 1) || !unit_stride(*t[i])) return false;
+    const int64_t B = lens.size(0);
+    if (table.size(0) != B || cu.size(0) != B + 1) return false;
+    p.K_cache = k.data_ptr(), p.V_cache = v.data_ptr();
+    p.block_table = static_cast<const int32_t*>(table.data_ptr()), p.seqlens_k = static_cast<const int32_t*>(lens.data_ptr());
+    p.cu_seqlens_q = static_cast<const int32_t*>(cu.data_ptr());
+    p.num_pages = (int)k.size(0), p.H_kv = (int)k.size(1), p.page_size = (int)k.size(2), p.d = (int)k.size(3), p.B = (int)B, p.max_pages = (int)table.size(1);
+    p.kc_page = k.stride(0), p.kc_head = k.stride(1), p.kc_row = k.stride(2);
+    p.vc_page = v.stride(0), p.vc_head = v.stride(1), p.vc_row = v.stride(2);
+    p.block_table_stride = table.stride(0);
+    p.window_left = p.window_right = -1;
+    return true;
+}
+// rows [T, heads, d] of the cache's type
+bool rows_ok(const at::Tensor& t, int64_t T, int64_t heads, const flash_paged_params& p)
+{
+    return is_here(t) && t.dim() == 3 && t.size(0) == T && t.size(1) == heads && t.size(2) == p.d && dtype_of(t) == p.dtype && t.stride(2) == 1;
+}
+
+// append(k, v, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, q, inv_freq, interleaved, factor, positions, out)
+PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    return guarded([&]() -> PyObject* {
+        if (n != 13 || !g_append || !allocates_plainly()) return not_implemented();
+        const at::Tensor *k = tensor_of(args[0]), *v = tensor_of(args[1]), *q, *f, *pos, *out;
+        flash_paged_params p{};
+        if (!k || !v || !parse_cache(args + 2, p) || !optional_tensor(args[7], &q) || !optional_tensor(args[8], &f) || !optional_tensor(args[11], &pos) ||
+            !optional_tensor(args[12], &out) || !PyBool_Check(args[9]) || !real(args[10], &p.factor))
+            return not_implemented();
+        if ((q && !f) || (out && !q) || (pos && !f) || k->dim() != 3 || (q && q->dim() != 3) || k->size(0) > INT32_MAX) return not_implemented();
+        const int64_t T = k->size(0), H = q ? q->size(1) : p.H_kv;
+        if (H > INT32_MAX || !rows_ok(*k, T, p.H_kv, p) || !rows_ok(*v, T, p.H_kv, p) || (q && !rows_ok(*q, T, H, p)) || (out && !rows_ok(*out, T, H, p))) return not_implemented();
+        if (f && !frequencies_ok(*f, p.d)) return not_implemented();
+        if (pos && (!positions_ok(*pos) || pos->dim() != 1 || pos->size(0) != T)) return not_implemented();
+        p.total_q = (int)T, p.H = (int)H;
+        p.K = k->data_ptr(), p.V = v->data_ptr(), p.k_token = k->stride(0), p.k_head = k->stride(1), p.v_token = v->stride(0), p.v_head = v->stride(1);
+        if (f) p.inv_freq = static_cast<const float*>(f->data_ptr()), p.rot = 2 * (int)f->numel(), p.interleaved = args[9] == Py_True;
+        if (pos) p.positions = pos->data_ptr(), p.positions_64 = pos->scalar_type() == at::kLong;
+        at::Tensor y;
+        if (q) {
+            y = out ? *out : empty_on(*q, q->sizes(), q->scalar_type());
+            p.Q = q->data_ptr(), p.O = y.data_ptr(), p.q_token = q->stride(0), p.q_head = q->stride(1), p.o_token = y.stride(0), p.o_head = y.stride(1);
+        }
+        const int rc = g_append(&p, c10::hip::getCurrentHIPStream().stream());
+        if (rc != FLASH_OK) return raise(rc, "flash_append_paged");
+        if (q) return THPVariable_Wrap(y);
+        Py_RETURN_NONE;
+    });
+}
+
+// paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, causal, window, num_splits, workspace, out, lse)
+PyObject* paged(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    return guarded([&]() -> PyObject* {
+        if (n != 15 || !g_paged || !allocates_plainly()) return not_implemented();
+        const at::Tensor *q = tensor_of(args[0]), *out, *lse;
+        flash_paged_params p{};
+        if (!q || !parse_cache(args + 1, p) || !optional_tensor(args[13], &out) || !optional_tensor(args[14], &lse)) return not_implemented();
+        if (!small_int(args[6], &p.max_seqlen_q) || !small_int(args[7], &p.max_seqlen_k) || !PyBool_Check(args[9]) || !small_int(args[11], &p.num_splits)) return not_implemented();
+        if (args[8] == Py_None) p.softmax_scale = (float)std::pow((double)p.d, -0.5);
+        else if (!real(args[8], &p.softmax_scale)) return not_implemented();
+        if (!PyTuple_CheckExact(args[10]) || PyTuple_GET_SIZE(args[10]) != 2 || !small_int(PyTuple_GET_ITEM(args[10], 0), &p.window_left) ||
+            !small_int(PyTuple_GET_ITEM(args[10], 1), &p.window_right))
+            return not_implemented();
+        p.is_causal = args[9] == Py_True;
+        if (q->dim() != 3 || !fits_int(*q)) return not_implemented();
+        const int64_t T = q->size(0), H = q->size(1), d = p.d;
+        if (p.H_kv < 1 || H < 1 || H % p.H_kv != 0 || !rows_ok(*q, T, H, p) || (out && !rows_ok(*out, T, H, p))) return not_implemented();
+        if (lse && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != T || lse->size(1) != H || !lse->is_contiguous() || !is_here(*lse)))
+            return not_implemented();
+        p.total_q = (int)T, p.H = (int)H;
+        const int S = g_paged_resolve(&p);
+        if (S < 0) return raise(S, "flash_forward_paged_resolve_splits");
+        const int64_t rows = S > 1 ? T * H * S : 0;
+        at::Tensor own;  // workspace of this call, both parts in one allocation
+        if (args[12] != Py_None) {
+            if (!PyTuple_CheckExact(args[12]) || PyTuple_GET_SIZE(args[12]) != 2) return not_implemented();
+            const at::Tensor *wo = tensor_of(PyTuple_GET_ITEM(args[12], 0)), *wl = tensor_of(PyTuple_GET_ITEM(args[12], 1));
+            for (const at::Tensor* t : {wo, wl})
+                if (!t || t->scalar_type() != at::kFloat || !is_here(*t) || !t->is_contiguous()) return not_implemented();
+            if (wo->numel() < rows * d || wl->numel() < rows) return not_implemented();
+            p.O_partial = static_cast<float*>(wo->data_ptr()), p.LSE_partial = static_cast<float*>(wl->data_ptr());
+        } else if (rows) {
+            const int64_t o_floats = (rows * d + 63) & ~(int64_t)63;
+            own = empty_on(*q, {o_floats + rows}, at::kFloat);
+            p.O_partial = static_cast<float*>(own.data_ptr()), p.LSE_partial = p.O_partial + o_floats;
+        }
+        const at::Tensor o = out ? *out : empty_on(*q, q->sizes(), q->scalar_type());
+        const at::Tensor l = lse ? *lse : empty_on(*q, {T, H}, at::kFloat);
+        p.Q = q->data_ptr(), p.O = o.data_ptr(), p.LSE = static_cast<float*>(l.data_ptr());
+        p.q_token = q->stride(0), p.q_head = q->stride(1), p.o_token = o.stride(0), p.o_head = o.stride(1);
+        const int rc = g_paged(&p, c10::hip::getCurrentHIPStream().stream());
+        if (rc != FLASH_OK) return raise(rc, "flash_forward_paged");
+        PyObject* res = PyTuple_New(2);
+        if (!res) return nullptr;
+        PyTuple_SET_ITEM(res, 0, THPVariable_Wrap(o));
+        PyTuple_SET_ITEM(res, 1, THPVariable_Wrap(l));
+        return res;
+    });
+}
+
+// bind_paged(addresses of flash_rotary, flash_append_paged, flash_forward_paged, flash_forward_paged_resolve_splits), behind bind()
+PyObject* bind_paged(PyObject*, PyObject* args)
+{
+    unsigned long long r, a, f, s;
+    if (!PyArg_ParseTuple(args, "KKKK", &r, &a, &f, &s)) return nullptr;
+    g_rotary = reinterpret_cast<rotary_fn>(r);
+    g_append = reinterpret_cast<paged_fn>(a);
+    g_paged = reinterpret_cast<paged_fn>(f);
+    g_paged_resolve = reinterpret_cast<paged_resolve_fn>(s);
+    Py_RETURN_NONE;
+}
+
 // bind(addresses of flash_forward, flash_forward_splitkv, flash_splitkv_resolve_splits, FlashError): the library that
 // binding.lib() has loaded
 PyObject* bind(PyObject*, PyObject* args)
@@ -292,6 +490,10 @@ PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(forward)), METH_FASTCALL, nullptr},
     {"splitkv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(splitkv)), METH_FASTCALL, nullptr},
+    {"bind_paged", bind_paged, METH_VARARGS, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
+    {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
+    {"paged", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -71,6 +71,32 @@ def _lib():
     return _bound
 
 
+class _NoFrontEnd:
+    """Leaves every call to this file's own path."""
+
+    @staticmethod
+    def rotary(*args):
+        return NotImplemented
+
+    append = paged = rotary
+
+
+_native = None
+
+
+def _front_end():
+    """The native front end (csrc/py_binding.cpp), as binding.py has it."""
+    global _native
+    L, n = _lib(), binding._native or binding._front_end()
+    if hasattr(n, "bind_paged"):
+        n.bind_paged(*(C.cast(f, C.c_void_p).value for f in (L.flash_rotary, L.flash_append_paged, L.flash_forward_paged,
+                                                             L.flash_forward_paged_resolve_splits)))
+        _native = n
+    else:
+        _native = _NoFrontEnd
+    return _native
+
+
 def _types():
     import torch
 
@@ -225,7 +251,7 @@ def _rotary_function():
         def forward(ctx, x, positions, inv_freq, interleaved, factor, inverse, stream):
             ctx.save_for_backward(positions, inv_freq)
             ctx.how = (interleaved, factor, inverse)
-            return _rotary(x, positions, inv_freq, interleaved, factor, inverse, None, stream)
+            return flash_rotary(x, positions, inv_freq, interleaved, factor, inverse, stream=stream)  # (no gradients in here)
 
         @staticmethod
         def backward(ctx, g):
@@ -248,6 +274,11 @@ def flash_rotary(x, positions, inv_freq, interleaved=False, factor=1.0, inverse=
     dimension.  Pairs are (i, i + rot / 2), or (2 i, 2 i + 1) if interleaved.  inverse turns the other way: the gradient of x from the
     gradient of the result, which is also what backward() takes for an x that requires one.  out: where to, x itself for in place."""
     global _function
+    if stream is None:
+        y = (_native or _front_end()).rotary(x, positions, inv_freq, interleaved, factor, inverse, out)
+        if y is not NotImplemented:
+            return y
+    # arguments that the native front end leaves alone (those that raise among them)
     import torch
 
     if torch.is_grad_enabled() and x.requires_grad:
@@ -300,6 +331,11 @@ def flash_append_paged(k, v, k_cache, v_cache, block_table, seqlens_k, cu_seqlen
 
     With inv_freq K is turned on its way in as by flash_rotary, by its place in the sequence or by positions [tokens] where they are given, and
     so is q [tokens,H,d], if it is given: returned, in `out` if that is given (q itself for in place).  Returns None without q."""
+    if stream is None:
+        res = (_native or _front_end()).append(k, v, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, q, inv_freq, interleaved, factor, positions, out)
+        if res is not NotImplemented:
+            return res
+    # arguments that the native front end leaves alone (those that raise among them)
     import torch
 
     _check(q is None or inv_freq is not None, "q is turned with inv_freq: without it there is nothing to do for q")
@@ -340,6 +376,12 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
     which decides into how many splits its keys are cut (0: what the table can name).  num_splits <= 0: the library's choice.
     workspace: (O_partial, LSE_partial) of at least the bytes that paged_workspace_bytes says, otherwise allocated here.
     Rows that belong to no sequence are left as they are (new memory where out and lse are not given)."""
+    if stream is None:
+        res = (_native or _front_end()).paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
+                                              window, num_splits, workspace, out, lse)
+        if res is not NotImplemented:
+            return res
+    # arguments that the native front end leaves alone (those that raise among them)
     import torch
 
     _check(q.dim() == 3 and k_cache.dim() == 4, "q must be [tokens,H,d], caches [pages,H_kv,page_size,d]")
