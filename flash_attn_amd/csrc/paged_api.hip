@@ -85,7 +85,8 @@ int validate_cache(const flash_paged_params* p)
 {
     for (int64_t s : {p->kc_page, p->kc_head, p->kc_row, p->vc_page, p->vc_head, p->vc_row})
         if (s < 0 || odd_stride(s)) return FLASH_EINVAL;
-    if (p->kc_row > (1 << 26) || p->vc_row > (1 << 26)) return FLASH_EINVAL;  // (the 16 rows of a request are addressed with 32 bits)
+    // (the kernels address the 16 rows of a request with 32 bits, and multiply a page's number by 32 bits)
+    if (p->kc_row > (1 << 26) || p->vc_row > (1 << 26) || p->kc_page > 0x7fffffffLL || p->vc_page > 0x7fffffffLL) return FLASH_EINVAL;
     if (!p->seqlens_k || !p->cu_seqlens_q) return FLASH_EINVAL;
     if (p->max_pages > 0 && !p->block_table) return FLASH_EINVAL;
     if (misaligned(p->seqlens_k, 4) || misaligned(p->cu_seqlens_q, 4) || misaligned(p->block_table, 4)) return FLASH_EALIGN;
@@ -115,8 +116,10 @@ long long blocks_of(const flash_paged_params* p, int br)
     return each * p->B < all ? each * p->B : all;
 }
 
+// bounds that can never cut are none: the kernels' position + right stays in an int
 int window_left_of(const flash_paged_params* p) { return p->window_left >= capacity_of(p) ? -1 : p->window_left; }
-int window_right_of(const flash_paged_params* p) { return p->window_right >= (long long)capacity_of(p) + p->total_q ? -1 : p->window_right; }
+// (the last row stands at the last key, and no row more than a chunk in front of it)
+int window_right_of(const flash_paged_params* p) { return p->window_right >= p->total_q ? -1 : p->window_right; }
 
 // tiles of 64 keys that the masks leave a block of br rows, at most
 int window_tiles(const flash_paged_params* p, int br)
@@ -132,22 +135,25 @@ int most_tiles(const flash_paged_params* p, int br)
     return w < (keys + 63) / 64 ? w : (keys + 63) / 64;
 }
 
-// Which form.  Up to 64 rows per K/V head and sequence the work-groups of 32 rows are the faster ones at every length: their waves stream
-// tiles of their own (B64 H_kv8 500 keys, 40 rows 21.7 us against 31.4; B8 H_kv8 4000 keys, 64 rows 27.9 / 31.6).  Longer chunks
-// take them while the launch is short: a work-group of 256 rows walks its tiles at 2 us each, whether or not it is alone, where one of
-// 32 rows has four waves at 32 or 64 keys each.  In units of 32 rows x 64 keys they cost some 3 ns against 1 ns in a full GPU.  32 rows / 256
-// rows: 1000 causal rows H8 (4000 units) 17.7 / 25.7 us, 512 rows on 1000 keys H8 (2700) 20.0 / 26.2, 1000 on 1000 (6100) 29.3 / 29.4, 256 on
-// 4000 B8 H8 (12000) 72.7 / 46.4.
-constexpr int kShortRows = 64, kShortUnits = 5000;
-bool few_rows(const flash_paged_params* p)
+// Rows of a work-group, which says which form: 32 or 256.  Up to 64 rows per K/V head and sequence 32 are the faster ones at every length: their
+// waves stream tiles of their own (B64 H_kv8 500 keys, 40 rows 21.7 us against 31.4; B8 H_kv8 4000 keys, 64 rows 27.9 / 31.6).  Longer
+// chunks take them while the launch is short and its work-groups are on the GPU together: a work-group of 256 rows walks its tiles at up to 2 us
+// each whether or not it is alone, where one of 32 rows has four waves at it.  In units of 32 rows x 64 keys the small ones, each of which
+// asks the L2 for its tiles, cost 2 ns at d = 128 and 1 ns at d = 64 once the GPU is full, the large ones 1 and 0.7 ns.
+// 32 rows / 256 rows, one MI355X: d128 H8 1000 causal rows (2000 units) 16.0 / 26.1 us, 512 rows on 1000 keys (2600) 19.2 / 26.0, 1000 on 1000
+// (6100) 26.0 / 28.8, 100 on 16000 (8000) 30.9 / 26.1, 256 on 16000 (16000) 49.9 / 36.5; d64 H16 2000 (16000) 26.9 / 37.2, 4096 (68000)
+// 77 / 68; more than 1024 work-groups: d128 B8 H32 H_kv8 up to 256 (3400 units, 1136 work-groups) 22.3 / 14.5.  (128 rows, four waves that share
+// tiles, two work-groups per CU, were the fastest by more than 5 % on 3 of 94 such launches, 13.6 us against 14.5 at best.)
+constexpr int kShortRows = 64, kShortUnits = 7000, kShortUnits64 = 30000, kShortGroups = 1024;
+int rows_per_group(const flash_paged_params* p)
 {
-    const long long chunk = longest_chunk(p);
-    if (chunk * group_of(p) <= kShortRows) return true;
+    const long long chunk = longest_chunk(p), groups = blocks_of(p, fa::kPagedFewRows) * p->H_kv;
+    if (chunk * group_of(p) <= kShortRows) return fa::kPagedFewRows;
     long long tiles = most_tiles(p, fa::kPagedFewRows);
     const int cap = capacity_of(p);
     const long long keys = p->max_seqlen_k > 0 && p->max_seqlen_k < cap ? p->max_seqlen_k : cap;
     if (p->is_causal && tiles > (keys - chunk / 2) / 64 + 1) tiles = (keys > chunk / 2 ? keys - chunk / 2 : 0) / 64 + 1;  // (the mean row's)
-    return blocks_of(p, fa::kPagedFewRows) * p->H_kv * tiles <= kShortUnits;
+    return groups <= kShortGroups && groups * tiles <= (p->d <= 64 ? kShortUnits64 : kShortUnits) ? fa::kPagedFewRows : fa::kPagedTallRows;
 }
 
 // Split count that the library chooses.  A work-group per CU at least, as long as each split has some tiles; and for single tokens of several
@@ -156,16 +162,15 @@ bool few_rows(const flash_paged_params* p)
 constexpr int kFewestTiles = 32, kMostGroups = 2048;
 int splits_of(const flash_paged_params* p)
 {
-    const bool few = few_rows(p);
-    const int br = few ? fa::kPagedFewRows : fa::kPagedTallRows, nt = most_tiles(p, br);
+    const int br = rows_per_group(p), nt = most_tiles(p, br);
     if (nt <= 1 || (long long)p->total_q * p->H >= 1LL << 26) return 1;  // (the merge has a wave per row: 2^32 threads)
     long long s = p->num_splits;
     if (s <= 0) {
         const long long groups = blocks_of(p, br) * p->H_kv;
         s = groups >= kNumCU ? 1 : kNumCU / groups;
-        const int least = few ? 2 : 4;  // tiles per split
+        const int least = br == fa::kPagedFewRows ? 2 : 4;  // tiles per split
         if (s > nt / least) s = nt / least;
-        if (few && p->B > 1) {
+        if (br == fa::kPagedFewRows && p->B > 1) {
             long long more = kFewestTiles;
             more = nt / more < kMostGroups / groups ? nt / more : kMostGroups / groups;
             if (more > s) s = more;
@@ -189,21 +194,20 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     if ((rc = rows_strides(p->q_token, p->q_head, p->Q)) != FLASH_OK || (rc = rows_strides(p->o_token, p->o_head, p->O)) != FLASH_OK) return rc;
     if (!p->LSE) return FLASH_EINVAL;
     if (misaligned(p->LSE, 4)) return FLASH_EALIGN;
-    const bool few = few_rows(p);
-    const int br = few ? fa::kPagedFewRows : fa::kPagedTallRows, splits = splits_of(p), nt = most_tiles(p, br);
+    const int br = rows_per_group(p), splits = splits_of(p), nt = most_tiles(p, br);
     if (splits > 1) {
         if (!p->O_partial || !p->LSE_partial) return FLASH_EWORKSPACE;
         if (misaligned(p->O_partial, 16) || misaligned(p->LSE_partial, 4)) return FLASH_EALIGN;
     }
     const long long blocks = blocks_of(p, br) * p->H_kv * splits;
-    if (blocks * (few ? 256 : 512) >= 1LL << 32) return FLASH_EINVAL;
+    if (blocks * fa::paged_threads(br) >= 1LL << 32) return FLASH_EINVAL;
     if ((rc = device_usable()) != FLASH_OK) return rc;
     fa::PagedArgs a{};
     a.Q = static_cast<const char*>(p->Q), a.K = static_cast<const char*>(p->K_cache), a.V = static_cast<const char*>(p->V_cache);
     a.O = static_cast<char*>(p->O), a.LSE = p->LSE, a.O_partial = p->O_partial, a.LSE_partial = p->LSE_partial;
     a.table = p->block_table, a.lens = p->seqlens_k, a.cu = p->cu_seqlens_q;
     a.q_token = 2 * p->q_token, a.q_head = 2 * p->q_head, a.o_token = 2 * p->o_token, a.o_head = 2 * p->o_head;
-    a.k_page = 2 * p->kc_page, a.k_head = 2 * p->kc_head, a.v_page = 2 * p->vc_page, a.v_head = 2 * p->vc_head;
+    a.k_page = (uint32_t)(2 * p->kc_page), a.k_head = 2 * p->kc_head, a.v_page = (uint32_t)(2 * p->vc_page), a.v_head = 2 * p->vc_head;
     a.k_row = (uint32_t)(2 * p->kc_row), a.v_row = (uint32_t)(2 * p->vc_row);
     a.table_stride = p->block_table_stride;
     a.B = p->B, a.H = p->H, a.Hk = p->H_kv, a.G = group_of(p), a.d = p->d, a.tokens = p->total_q, a.num_pages = p->num_pages, a.page = p->page_size;
@@ -215,7 +219,7 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     a.by_heads = fa::fast_div(a.Hk), a.by_group = fa::fast_div(a.G), a.by_page = fa::fast_div(a.page);
     a.by_splits = fa::fast_div(splits);
     const bool bf16 = p->dtype == FLASH_BF16;
-    rc = record_hip(p->d <= 64 ? fa::launch_paged_d64(a, bf16, few, blocks, st) : fa::launch_paged_d128(a, bf16, few, blocks, st));
+    rc = record_hip(p->d <= 64 ? fa::launch_paged_d64(a, bf16, br, blocks, st) : fa::launch_paged_d128(a, bf16, br, blocks, st));
     if (rc != FLASH_OK || splits == 1) return rc;
     return record_hip(fa::launch_paged_merge(a, bf16, st));
 }

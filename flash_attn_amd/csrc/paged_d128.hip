@@ -2,7 +2,7 @@
 #include "paged_kernel.h"
 
 namespace fa {
-int launch_paged_d128(const PagedArgs& a, bool bf16, bool few, long long blocks, hipStream_t st) { return launch_paged_bucket<128>(a, bf16, few, blocks, st); }
+int launch_paged_d128(const PagedArgs& a, bool bf16, int rows, long long blocks, hipStream_t st) { return launch_paged_bucket<128>(a, bf16, rows, blocks, st); }
 
 // Four waves per row where rows are few and splits many: a wave alone would walk them one pair after the other.
 int launch_paged_merge(const PagedArgs& p, bool bf16, hipStream_t st)

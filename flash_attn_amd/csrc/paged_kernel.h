@@ -35,22 +35,25 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
-constexpr int kPagedTallRows = 256, kPagedFewRows = 32;
+constexpr int kPagedTallRows = 256, kPagedFewRows = 32;  // rows of a work-group
+constexpr int paged_threads(int rows) { return rows == kPagedTallRows ? 512 : 256; }
 
 struct PagedArgs {
+    // what a work-group needs to find its place comes first
+    const int32_t *table, *lens, *cu;
+    FastDiv by_heads;
+    int Hk, num_splits, B, direct;     // direct: every sequence has one row block
+    int tiles_per_split, window_tiles; // window_tiles: tiles of 64 keys that the masks leave a row block at most
+    FastDiv by_splits, by_group, by_page;
+    int H, G, d, tokens, num_pages, page, capacity;  // capacity: keys that a row of the table can name
+    int causal, wl, wr;                // wl / wr < 0: unbounded
     const char *Q, *K, *V;
     char* O;
     float* LSE;                        // [tokens, H]
     float *O_partial, *LSE_partial;    // [tokens, H, S, d] and [tokens, H, S]
-    const int32_t *table, *lens, *cu;
-    int64_t q_token, q_head, o_token, o_head, k_page, k_head, v_page, v_head, table_stride;  // bytes (table_stride: entries)
-    uint32_t k_row, v_row;             // bytes
-    int B, H, Hk, G, d, tokens, num_pages, page, capacity;  // capacity: keys that a row of the table can name
-    int causal, wl, wr;                // wl / wr < 0: unbounded
+    int64_t q_token, q_head, o_token, o_head, k_head, v_head, table_stride;  // bytes (table_stride: entries)
+    uint32_t k_page, v_page, k_row, v_row;                                   // bytes
     float scale_log2;
-    int num_splits, tiles_per_split, window_tiles;
-    int direct;                        // every sequence has one row block
-    FastDiv by_heads, by_group, by_page, by_splits;
 };
 
 // What the merge needs of them (short arguments launch faster: common.h)
@@ -242,12 +245,23 @@ __device__ __forceinline__ int row_token(const PagedArgs& a, const PagedItem& it
     return it.tok0 + i;
 }
 
-// Entry of the page that key j of the sequence lies in, kept inside the cache whatever the table holds.
-__device__ __forceinline__ int paged_entry(const PagedArgs& a, const int32_t* table_row, int len, int j)
-{
-    return read_uniform_int(table_row + a.by_page.quotient(j < len ? j : len - 1));
-}
-__device__ __forceinline__ int64_t inside(const PagedArgs& a, int entry) { return (uint32_t)entry < (uint32_t)a.num_pages ? entry : 0; }
+// Where rows of the sequence lie: entry of the table and row within the page, asked for a tile ahead of their use.  Keys from len on
+// stand for the last one.  The entry is kept inside the cache whatever the table holds.
+struct PagedPlace {
+    int entry, row;
+    __device__ __forceinline__ void ask(const PagedArgs& a, const int32_t* table_row, int len, int j)
+    {
+        const int jj = j < len ? j : len - 1, pg = a.by_page.quotient(jj);
+        row = jj - pg * a.page;
+        entry = read_uniform_int(table_row + pg);
+    }
+    // 32 x 32 -> 64-bit products on the scalar unit (the host sees to it that strides fit)
+    __device__ __forceinline__ const char* in(const PagedArgs& a, const char* head, uint32_t page_bytes, uint32_t row_bytes) const
+    {
+        const uint32_t e = (uint32_t)entry < (uint32_t)a.num_pages ? (uint32_t)entry : 0u;
+        return head + (uint64_t)e * page_bytes + (uint64_t)(uint32_t)row * row_bytes;
+    }
+};
 
 // rows of the work-group that see no key: O = 0, LSE = -inf, or the same as partial results
 template <int BR, int kThreads>
@@ -416,9 +430,10 @@ __device__ __forceinline__ void paged_rescue(const PagedArgs& a, const PagedItem
     const int32_t* const table_row = a.table + (size_t)it.b * a.table_stride;
     int lo, hi;
     paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
-    auto row_of = [&](const char* base, int64_t page_bytes, int64_t head_bytes, uint32_t row_bytes, int j) {
+    auto row_of = [&](const char* base, uint32_t page_bytes, int64_t head_bytes, uint32_t row_bytes, int j) {
         const int pg = a.by_page.quotient(j);
-        return base + inside(a, table_row[pg]) * page_bytes + it.hk * head_bytes + (int64_t)(j - pg * a.page) * row_bytes;
+        const PagedPlace at = {table_row[pg], j - pg * a.page};
+        return at.in(a, base + it.hk * head_bytes, page_bytes, row_bytes);
     };
     // lane j: key j of the tile; masked for some row of the wave, and not finite somewhere?
     bool spoilt = false;
@@ -542,34 +557,34 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
         kok[x] = ck * 8 < a.d;
         vok[x] = cv * 8 < a.d;
     }
-    int entry[GROUPS];
-    auto ask_entries = [&](int t) __attribute__((always_inline)) {
+    const char* const Kh = a.K + it.hk * a.k_head;
+    const char* const Vh = a.V + it.hk * a.v_head;
+    PagedPlace place[GROUPS];  // of the tile to request next
+    auto ask = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < GROUPS; ++s) entry[s] = paged_entry(a, table_row, len, (tile0 + t) * BC + 16 * s);
+        for (int s = 0; s < GROUPS; ++s) place[s].ask(a, table_row, len, (tile0 + t) * BC + 16 * s);
     };
-    // the rows of tile t (its entries given) of K or V
-    auto request = [&](int t, const char* base, int64_t page_bytes, int64_t head_bytes, uint32_t row_bytes, const uint32_t (&off)[kPer], const bool (&ok)[kPer],
+    // the rows of tile t (its places asked for) of K or V
+    auto request = [&](int t, const char* head, uint32_t page_bytes, uint32_t row_bytes, const uint32_t (&off)[kPer], const bool (&ok)[kPer],
                        FA_LDS char* dst) __attribute__((always_inline)) {
         const int kb0 = (tile0 + t) * BC;
         const bool whole = kb0 + BC <= len;
 #pragma unroll
         for (int s = 0; s < GROUPS; ++s) {
-            const int j = kb0 + 16 * s, jj = j < len ? j : len - 1;
-            const int in_page = jj - a.by_page.quotient(jj) * a.page;
-            const char* const at = base + inside(a, entry[s]) * page_bytes + it.hk * head_bytes + (int64_t)in_page * row_bytes;
+            const char* const at = place[s].in(a, head, page_bytes, row_bytes);
 #pragma unroll
             for (int x = 0; x < kPer; ++x) {
                 uint32_t o = off[x];
                 if (!whole) {  // rows past the last key repeat it
-                    const int r = T::RPB * x + lrow, most = len - 1 - jj;
+                    const int r = T::RPB * x + lrow, most = max(len - 1 - (kb0 + 16 * s), 0);
                     if (r > most) o -= (uint32_t)(r - most) * row_bytes;
                 }
                 if (ok[x]) dma_kib_nt(at, o, dst + (s * kPer + x) * 1024);
             }
         }
     };
-    auto request_k = [&](int t) { request(t, a.K, a.k_page, a.k_head, a.k_row, koff, kok, kst); };
-    auto request_v = [&](int t) { request(t, a.V, a.v_page, a.v_head, a.v_row, voff, vok, vst); };
+    auto request_k = [&](int t) { request(t, Kh, a.k_page, a.k_row, koff, kok, kst); };
+    auto request_v = [&](int t) { request(t, Vh, a.v_page, a.v_row, voff, vok, vst); };
 
     const int r = it.row0 + l32;
     v8h qf[KS];
@@ -584,7 +599,7 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
     paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
     int lo_max = lo, hi_min = hi;
     if (wave < ntiles) {
-        ask_entries(wave);
+        ask(wave);
         load_q<KS>(a, it, r, g, qf);
         request_k(wave);
         request_v(wave);
@@ -596,7 +611,7 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
     for (int t = wave; t < ntiles; t += 4) {
         const int kb0 = (tile0 + t) * BC;
         const bool more = t + 4 < ntiles;
-        if (more) ask_entries(t + 4);
+        if (more) ask(t + 4);
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");  // K of this tile is there
         if (t == wave) {
 #pragma unroll
@@ -690,13 +705,64 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
     }
 }
 
-// ---------------------------------------------------------------------------------------------- many rows
+// ---------------------------------------------------------------------------------------------- tiles that waves share
 
-template <int D>
-struct TallCfg {
-    static constexpr int kWaves = 8, NST = 4;                 // LDS stages per tensor
-    static constexpr int SMEM = NST * 2 * PagedTile<D>::BUF;  // 128 or 64 KiB
-    static constexpr int NL = PagedTile<D>::REQ / kWaves;     // requests per wave and tile, K and V each
+// What one of kWaves waves requests of the work-group's tiles: KiB blocks wave, wave + kWaves, ... of each.
+template <int D, int kWaves>
+struct PagedRequests {
+    using T = PagedTile<D>;
+    static constexpr int NL = T::REQ / kWaves, STEP = T::RPB * kWaves;  // blocks, and rows from one to the next
+    static_assert(STEP % 16 == 0, "the permutations of the chunks repeat");
+    const int32_t* table_row;
+    const char *Kh, *Vh;
+    int len, tile0, wave, brow, lrow;
+    uint32_t koff, voff;
+    bool kok, vok;
+    PagedPlace place[NL];   // of the tile of K to request next
+    const char* vnext[NL];  // rows of the tile of V to request next: where K's were
+
+    __device__ __forceinline__ void set(const PagedArgs& a, const PagedItem& it, int first_tile, int wave_, int lane)
+    {
+        table_row = a.table + (size_t)it.b * a.table_stride;
+        Kh = a.K + it.hk * a.k_head;
+        Vh = a.V + it.hk * a.v_head;
+        len = it.len, tile0 = first_tile, wave = wave_;
+        lrow = lane / T::CPR;
+        brow = T::RPB * wave;
+        const int slot = lane % T::CPR, ck = T::k_chunk(slot, brow + lrow), cv = T::v_chunk(slot, brow + lrow);
+        koff = (uint32_t)lrow * a.k_row + ck * 16, voff = (uint32_t)lrow * a.v_row + cv * 16;
+        kok = ck * 8 < a.d, vok = cv * 8 < a.d;
+    }
+    __device__ __forceinline__ void ask(const PagedArgs& a, int t)
+    {
+#pragma unroll
+        for (int x = 0; x < NL; ++x) place[x].ask(a, table_row, len, (tile0 + t) * T::BC + brow + STEP * x);
+    }
+    __device__ __forceinline__ void request(int t, int x, const char* at, uint32_t row_bytes, uint32_t off, bool ok, FA_LDS char* stage) const
+    {
+        const int kb0 = (tile0 + t) * T::BC;
+        uint32_t o = off;
+        if (kb0 + T::BC > len) {  // rows past the last key repeat it
+            const int most = max(len - 1 - (kb0 + brow + STEP * x), 0);
+            if (lrow > most) o -= (uint32_t)(lrow - most) * row_bytes;
+        }
+        if (ok) dma_kib(at, o, stage + (wave + kWaves * x) * 1024);
+    }
+    __device__ __forceinline__ void load_k(const PagedArgs& a, int t, FA_LDS char* stage) const
+    {
+#pragma unroll
+        for (int x = 0; x < NL; ++x) request(t, x, place[x].in(a, Kh, a.k_page, a.k_row), a.k_row, koff, kok, stage);
+    }
+    __device__ __forceinline__ void find_v(const PagedArgs& a)
+    {
+#pragma unroll
+        for (int x = 0; x < NL; ++x) vnext[x] = place[x].in(a, Vh, a.v_page, a.v_row);
+    }
+    __device__ __forceinline__ void load_v(const PagedArgs& a, int t, FA_LDS char* stage) const
+    {
+#pragma unroll
+        for (int x = 0; x < NL; ++x) request(t, x, vnext[x], a.v_row, voff, vok, stage);
+    }
 };
 
 // LDS-only barrier: requests in flight are not waited for, and nothing moves across.
@@ -715,6 +781,65 @@ __device__ __forceinline__ void paged_barrier_keep()
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// Results of a wave's 32 rows from first_row on (r: the lane's).  `ost`: LDS of the wave's own, 32 rows of D columns.
+template <int D, int MB, bool kBf16>
+__device__ __forceinline__ void paged_store_rows(const PagedArgs& a, const PagedItem& it, int first_row, int r, int lane, int g, float m_ref, float l_run,
+                                                 const v16f (&oacc)[MB], FA_LDS char* ost)
+{
+    using T = PagedTile<D>;
+    using E = Elem<kBf16>;
+    const int l32 = lane & 31;
+    const float l = xhalf_sum(l_run);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float lse = l == 0.0f ? -INFINITY : __builtin_fmaf(m_ref, kLn2, fast_log2(l) * kLn2);
+    int head;
+    const int tok = row_token(a, it, r < it.rows ? r : it.rows - 1, &head);
+    const size_t at = (size_t)tok * a.H + head;
+    if (a.num_splits > 1) {
+        if (r < it.rows) {
+            const size_t part = at * a.num_splits + it.split;
+            if (g == 0) a.LSE_partial[part] = lse;
+            float* const op = a.O_partial + part * a.d;
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int rg = 0; rg < 4; ++rg) {
+                    const int c = 32 * mb + 8 * rg + 4 * g;
+                    const v4f o = {oacc[mb][4 * rg] * inv, oacc[mb][4 * rg + 1] * inv, oacc[mb][4 * rg + 2] * inv, oacc[mb][4 * rg + 3] * inv};
+                    if (c < a.d) *reinterpret_cast<v4f*>(op + c) = o;
+                }
+        }
+        return;
+    }
+    if (r < it.rows && g == 0) a.LSE[at] = lse;
+    // O^T is turned round in LDS and leaves as whole rows
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int rg = 0; rg < 4; ++rg) {
+            const v2u w = {E::pack(oacc[mb][4 * rg] * inv, oacc[mb][4 * rg + 1] * inv), E::pack(oacc[mb][4 * rg + 2] * inv, oacc[mb][4 * rg + 3] * inv)};
+            *reinterpret_cast<FA_LDS v2u*>(ost + l32 * T::ROW + T::k_chunk(4 * mb + rg, l32) * 16 + g * 8) = w;
+        }
+#pragma unroll
+    for (int x = 0; x < 32 / T::RPB; ++x) {
+        const int rl = T::RPB * x + lane / T::CPR, c = T::k_chunk(lane % T::CPR, rl);
+        const v4u val = *reinterpret_cast<FA_LDS const v4u*>(ost + x * 1024 + lane * 16);
+        if (first_row + rl < it.rows && c * 8 < a.d) {
+            int oh;
+            const int ot = row_token(a, it, first_row + rl, &oh);
+            __builtin_nontemporal_store(val, reinterpret_cast<v4u*>(a.O + (size_t)ot * a.o_token + (size_t)oh * a.o_head + c * 16));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- many rows
+
+template <int D>
+struct TallCfg {
+    static constexpr int kWaves = 8, NST = 4;                 // LDS stages per tensor
+    static constexpr int SMEM = NST * 2 * PagedTile<D>::BUF;  // 128 or 64 KiB
+};
+
 // Waves 0-3 and 4-7 run half an iteration apart (the second group passes one more barrier in front of the loop): while one wave of a
 // SIMD is at its softmax, the other is at its MFMAs.  V(t + 2) is requested at the start of iteration t and waited for at its end, K(t + 3) at
 // its end and waited for at the next one's; their slots were last read two barriers before.
@@ -726,7 +851,7 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
     using T = PagedTile<D>;
     using C = TallCfg<D>;
     using E = Elem<kBf16>;
-    constexpr int KS = DU / 16, MB = DU / 32, NST = C::NST, NL = C::NL, BC = T::BC;
+    constexpr int KS = DU / 16, MB = DU / 32, NST = C::NST, NL = PagedRequests<D, C::kWaves>::NL, BC = T::BC;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     FA_LDS char* const Ks = (FA_LDS char*)smem;
     FA_LDS char* const Vs = Ks + NST * T::BUF;
@@ -742,9 +867,6 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
         return;
     }
     const int tile0 = kmin >> 6, ntiles = ((kmax + 63) >> 6) - tile0;
-    const int len = it.len;
-    const int32_t* const table_row = a.table + (size_t)it.b * a.table_stride;
-
     if (a.d != D) {  // columns that no request writes
         const v4u z = {0u, 0u, 0u, 0u};
         for (int k = tid; k < C::SMEM / 16; k += 512) *reinterpret_cast<FA_LDS v4u*>(Ks + 16 * k) = z;
@@ -755,36 +877,8 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
     const int rblk = wave < 4 ? wave : 11 - wave;
     const int first_row = it.row0 + rblk * 32, r = first_row + l32;
 
-    // ---- requests of this wave: KiB blocks wave and (256-byte rows) wave + 8 of a tile
-    const int lrow = lane / T::CPR, slot = lane % T::CPR;
-    const int brow = T::RPB * wave;  // first row of block `wave`; the other one's is 32 further on
-    const int ck = T::k_chunk(slot, brow + lrow), cv = T::v_chunk(slot, brow + lrow);
-    const uint32_t koff = (uint32_t)lrow * a.k_row + ck * 16, voff = (uint32_t)lrow * a.v_row + cv * 16;
-    const bool kok = ck * 8 < a.d, vok = cv * 8 < a.d;
-    int kent[NL], vent[NL];  // table entries of the next tiles of K and V to request
-    auto ask_entries = [&](int t, int (&e)[NL]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int x = 0; x < NL; ++x) e[x] = paged_entry(a, table_row, len, (tile0 + t) * BC + brow + 32 * x);
-    };
-    auto request = [&](int t, const int (&e)[NL], const char* base, int64_t page_bytes, int64_t head_bytes, uint32_t row_bytes, uint32_t off, bool ok,
-                       FA_LDS char* stage) __attribute__((always_inline)) {
-        const int kb0 = (tile0 + t) * BC;
-        const bool whole = kb0 + BC <= len;
-#pragma unroll
-        for (int x = 0; x < NL; ++x) {
-            const int j = kb0 + brow + 32 * x, jj = j < len ? j : len - 1;
-            const int in_page = jj - a.by_page.quotient(jj) * a.page;
-            const char* const at = base + inside(a, e[x]) * page_bytes + it.hk * head_bytes + (int64_t)in_page * row_bytes;
-            uint32_t o = off;
-            if (!whole) {  // rows past the last key repeat it
-                const int most = j < len ? len - 1 - j : 0;
-                if (lrow > most) o -= (uint32_t)(lrow - most) * row_bytes;
-            }
-            if (ok) dma_kib(at, o, stage + (wave + 8 * x) * 1024);
-        }
-    };
-    auto load_k = [&](int t, const int (&e)[NL], FA_LDS char* stage) { request(t, e, a.K, a.k_page, a.k_head, a.k_row, koff, kok, stage); };
-    auto load_v = [&](int t, const int (&e)[NL], FA_LDS char* stage) { request(t, e, a.V, a.v_page, a.v_head, a.v_row, voff, vok, stage); };
+    PagedRequests<D, C::kWaves> req;
+    req.set(a, it, tile0, wave, lane);
 
     // ---- what the rows of this wave see
     int lo, hi, lo_max, hi_min, lo_min, hi_max;
@@ -869,11 +963,10 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
     };
     // what has to have landed at the end of iteration t, and the requests for what is to come
     auto tail_requests = [&](int t, FA_LDS char* wrk) __attribute__((always_inline)) {
-#pragma unroll
-        for (int x = 0; x < NL; ++x) vent[x] = kent[x];  // K(t + 3)'s entries are V(t + 3)'s
         if (t + 3 < ntiles) {
-            load_k(t + 3, kent, wrk);
-            ask_entries(t + 4, kent);
+            req.load_k(a, t + 3, wrk);
+            req.find_v(a);
+            req.ask(a, t + 4);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -882,7 +975,7 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
     auto iteration = [&](auto last_c, FA_LDS const char* __restrict__ rdv, FA_LDS const char* __restrict__ rdk, FA_LDS char* __restrict__ wrk,
                          FA_LDS char* __restrict__ wrv, int t) __attribute__((always_inline)) {
         const int kb0 = (tile0 + t) * BC;
-        if (t + 2 < ntiles) load_v(t + 2, vent, wrv);
+        if (t + 2 < ntiles) req.load_v(a, t + 2, wrv);
         soft.tile(s, oacc, p, c2, inv_c2, mask_sides(kb0, lo_max, hi_min), lo - kb0 - 4 * g, hi - kb0 - 4 * g);
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t vbase = fragment_base(rdv, v_rd);
@@ -903,14 +996,13 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
 #pragma unroll
     for (int t = 0; t < 3; ++t) {
         if (t < ntiles) {
-            ask_entries(t, kent);
-            load_k(t, kent, Ks + t * T::BUF);
-            if (t < 2) load_v(t, kent, Vs + t * T::BUF);
+            req.ask(a, t);
+            req.load_k(a, t, Ks + t * T::BUF);
+            req.find_v(a);
+            if (t < 2) req.load_v(a, t, Vs + t * T::BUF);
         }
     }
-#pragma unroll
-    for (int x = 0; x < NL; ++x) vent[x] = kent[x];  // of tile 2
-    ask_entries(3, kent);
+    req.ask(a, 3);  // (vnext: of tile 2)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
@@ -930,7 +1022,7 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
 
     // Tiles of which no row of this wave sees a key: only the wave's share of the requests and the barriers.
     auto idle_iteration = [&](int t) {
-        if (t + 2 < ntiles) load_v(t + 2, vent, Vs + ((t + 2) % NST) * T::BUF);
+        if (t + 2 < ntiles) req.load_v(a, t + 2, Vs + ((t + 2) % NST) * T::BUF);
         paged_barrier();
         tail_requests(t, Ks + ((t + 3) % NST) * T::BUF);
         paged_barrier();
@@ -955,48 +1047,7 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
 
     // ---- epilogue
     if (__builtin_expect(any_not_finite<MB>(oacc), 0)) paged_rescue<BC, MB, kBf16>(a, it, r, kmin, kmax, tile0, ntiles, 0, 1, soft.m_ref, oacc);
-    const float l = xhalf_sum(soft.l_run);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const float lse = l == 0.0f ? -INFINITY : __builtin_fmaf(soft.m_ref, kLn2, fast_log2(l) * kLn2);
-    int head;
-    const int tok = row_token(a, it, r < it.rows ? r : it.rows - 1, &head);
-    const size_t at = (size_t)tok * a.H + head;
-    if (a.num_splits > 1) {
-        if (r < it.rows) {
-            const size_t part = at * a.num_splits + it.split;
-            if (g == 0) a.LSE_partial[part] = lse;
-            float* const op = a.O_partial + part * a.d;
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-                for (int rg = 0; rg < 4; ++rg) {
-                    const int c = 32 * mb + 8 * rg + 4 * g;
-                    const v4f o = {oacc[mb][4 * rg] * inv, oacc[mb][4 * rg + 1] * inv, oacc[mb][4 * rg + 2] * inv, oacc[mb][4 * rg + 3] * inv};
-                    if (c < a.d) *reinterpret_cast<v4f*>(op + c) = o;
-                }
-        }
-        return;
-    }
-    if (r < it.rows && g == 0) a.LSE[at] = lse;
-    // O^T is turned round in LDS of the wave's own (every read of the tiles is behind the last barrier) and leaves as whole rows
-    FA_LDS char* const ost = Ks + wave * (32 * T::ROW);
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int rg = 0; rg < 4; ++rg) {
-            const v2u w = {E::pack(oacc[mb][4 * rg] * inv, oacc[mb][4 * rg + 1] * inv), E::pack(oacc[mb][4 * rg + 2] * inv, oacc[mb][4 * rg + 3] * inv)};
-            *reinterpret_cast<FA_LDS v2u*>(ost + l32 * T::ROW + T::k_chunk(4 * mb + rg, l32) * 16 + g * 8) = w;
-        }
-#pragma unroll
-    for (int x = 0; x < 32 / T::RPB; ++x) {
-        const int rl = T::RPB * x + lrow, c = T::k_chunk(slot, rl);
-        const v4u val = *reinterpret_cast<FA_LDS const v4u*>(ost + x * 1024 + lane * 16);
-        if (first_row + rl < it.rows && c * 8 < a.d) {
-            int oh;
-            const int ot = row_token(a, it, first_row + rl, &oh);
-            __builtin_nontemporal_store(val, reinterpret_cast<v4u*>(a.O + (size_t)ot * a.o_token + (size_t)oh * a.o_head + c * 16));
-        }
-    }
+    paged_store_rows<D, MB, kBf16>(a, it, first_row, r, lane, g, soft.m_ref, soft.l_run, oacc, Ks + wave * (32 * T::ROW));
 }
 
 // ---------------------------------------------------------------------------------------------- merge of splits
@@ -1073,34 +1124,35 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMergeArgs a
 
 // ---------------------------------------------------------------------------------------------- launches
 
-template <int D, int DU, bool kBf16, bool kFew>
+template <int D, int DU, bool kBf16, int kRows>
 inline hipError_t launch_paged_instance(const PagedArgs& a, long long blocks, hipStream_t st)
 {
     const auto kern = [] {
-        if constexpr (kFew) return paged_few_kernel<D, kBf16>;
+        if constexpr (kRows == kPagedFewRows) return paged_few_kernel<D, kBf16>;
         else return paged_tall_kernel<D, DU, kBf16>;
     }();
-    constexpr int smem = kFew ? FewCfg<D>::SMEM : TallCfg<D>::SMEM;
+    constexpr int smem = kRows == kPagedFewRows ? FewCfg<D>::SMEM : TallCfg<D>::SMEM;
     static DeviceFlags attr_done;  // per instantiation and device
     if (hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), smem, attr_done); e != hipSuccess) return e;
-    return launch_kernel(kern, dim3((unsigned)blocks), dim3(kFew ? 256 : 512), smem, st, a);
+    return launch_kernel(kern, dim3((unsigned)blocks), dim3(paged_threads(kRows)), smem, st, a);
 }
 
+// rows: of a work-group, which says which form
 template <int D, bool kBf16>
-inline int launch_paged_type(const PagedArgs& a, bool few, long long blocks, hipStream_t st)
+inline int launch_paged_type(const PagedArgs& a, int rows, long long blocks, hipStream_t st)
 {
-    if (few) return (int)launch_paged_instance<D, D, kBf16, true>(a, blocks, st);
-    if (a.d <= D - 32) return (int)launch_paged_instance<D, D - 32, kBf16, false>(a, blocks, st);
-    return (int)launch_paged_instance<D, D, kBf16, false>(a, blocks, st);
+    if (rows == kPagedFewRows) return (int)launch_paged_instance<D, D, kBf16, kPagedFewRows>(a, blocks, st);
+    if (a.d <= D - 32) return (int)launch_paged_instance<D, D - 32, kBf16, kPagedTallRows>(a, blocks, st);
+    return (int)launch_paged_instance<D, D, kBf16, kPagedTallRows>(a, blocks, st);
 }
 template <int D>
-inline int launch_paged_bucket(const PagedArgs& a, bool bf16, bool few, long long blocks, hipStream_t st)
+inline int launch_paged_bucket(const PagedArgs& a, bool bf16, int rows, long long blocks, hipStream_t st)
 {
-    return bf16 ? launch_paged_type<D, true>(a, few, blocks, st) : launch_paged_type<D, false>(a, few, blocks, st);
+    return bf16 ? launch_paged_type<D, true>(a, rows, blocks, st) : launch_paged_type<D, false>(a, rows, blocks, st);
 }
 
-int launch_paged_d64(const PagedArgs& a, bool bf16, bool few, long long blocks, hipStream_t st);
-int launch_paged_d128(const PagedArgs& a, bool bf16, bool few, long long blocks, hipStream_t st);
+int launch_paged_d64(const PagedArgs& a, bool bf16, int rows, long long blocks, hipStream_t st);
+int launch_paged_d128(const PagedArgs& a, bool bf16, int rows, long long blocks, hipStream_t st);
 int launch_paged_merge(const PagedArgs& a, bool bf16, hipStream_t st);
 
 }  // namespace fa

@@ -89,7 +89,7 @@ BOTH = [
     (E_INVAL, {"page_size": 2 ** 16, "max_pages": 2 ** 16}), (E_INVAL, {"total_q": 2 ** 30, "H": 1024, "H_kv": 1024}), (E_INVAL, {"B": 2 ** 25}),
     (E_INVAL, {"block_table": None}), (E_INVAL, {"seqlens_k": None}), (E_INVAL, {"cu_seqlens_q": None}), (E_INVAL, {"K_cache": None}),
     (E_INVAL, {"V_cache": None}), (E_INVAL, {"block_table_stride": -1}), (E_INVAL, {"kc_row": 68}), (E_INVAL, {"vc_page": 2052}), (E_INVAL, {"vc_head": -64}),
-    (E_INVAL, {"kc_row": 2 ** 27}), (E_INVAL, {"q_token": 516}), (E_INVAL, {"q_head": 4}), (E_INVAL, {"o_head": -64}), (E_INVAL, {"Q": None, "O": None, "K": None}),
+    (E_INVAL, {"kc_row": 2 ** 27}), (E_INVAL, {"kc_page": 2 ** 31}), (E_INVAL, {"vc_page": 2 ** 33}), (E_INVAL, {"q_token": 516}), (E_INVAL, {"q_head": 4}), (E_INVAL, {"o_head": -64}), (E_INVAL, {"Q": None, "O": None, "K": None}),
     (E_INVAL, {"O": None}), (E_ALIGN, {"Q": 0x10008}), (E_ALIGN, {"O": 0x20002}), (E_ALIGN, {"K_cache": 0x50008}), (E_ALIGN, {"V_cache": 0x60004}),
     (E_ALIGN, {"block_table": 0x80002}), (E_ALIGN, {"seqlens_k": 0x90001}), (E_ALIGN, {"cu_seqlens_q": 0xa0002}), (0, {"B": 0}), (0, {"total_q": 0, "Q": None})]
 
