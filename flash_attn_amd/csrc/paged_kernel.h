@@ -117,15 +117,15 @@ struct PagedItem {
 // Lengths come from device memory: whatever they hold, nothing outside the tensors is touched.
 __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-// inclusive sum over the lanes of a wave
+// inclusive sum over the lanes of a wave: inside rows of 16 lanes by DPP shifts, then the rows' last lanes
 __device__ __forceinline__ int wave_prefix(int v, int lane)
 {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const int other = __shfl_up(v, s);
-        if (lane >= s) v += other;
-    }
-    return v;
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr by 1, 2, 4, 8, nothing shifted in
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31), r2 = r1 + __builtin_amdgcn_readlane(v, 47);
+    return v + (lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
 }
 
 // Tiles of a split of a sequence of `len` keys (*per), and its splits: pieces of as many tiles as the launch was sized for, or more, should
@@ -149,46 +149,50 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
 {
     const int block = blockIdx.x, w = a.by_heads.quotient(block);
     it->hk = block - w * a.Hk;
-    int b = 0, m = 0;
+    int b = 0, m = 0, c0, c1, len;
     if (a.direct && (a.num_splits == 1 || a.B == 1)) {  // one row block per sequence, and one split or sequence
         if (a.num_splits == 1) b = w, it->split = 0;
         else it->split = w;
+        c0 = clamp_int(read_uniform_int(a.cu + b), 0, a.tokens), c1 = clamp_int(read_uniform_int(a.cu + b + 1), c0, a.tokens);
+        len = clamp_int(read_uniform_int(a.lens + b), 0, a.capacity);
     } else {
         // 64 sequences at a time, a lane each
         int before = 0;
         bool found = false;
         for (int b0 = 0; b0 < a.B; b0 += 64) {
             const int mine = b0 + lane;
-            int blocks = 0, splits = 1, per;
+            int blocks = 0, splits = 1, per, first = 0, end = 0, keys = 0;
             if (mine < a.B) {
-                const int c0 = clamp_int(a.cu[mine], 0, a.tokens), c1 = clamp_int(a.cu[mine + 1], c0, a.tokens);
-                blocks = ((c1 - c0) * a.G + BR - 1) / BR;
-                splits = splits_of_sequence(a, clamp_int(a.lens[mine], 0, a.capacity), &per);
+                first = a.cu[mine], end = a.cu[mine + 1], keys = a.lens[mine];
+                first = clamp_int(first, 0, a.tokens), end = clamp_int(end, first, a.tokens), keys = clamp_int(keys, 0, a.capacity);
+                blocks = ((end - first) * a.G + BR - 1) / BR;
+                splits = splits_of_sequence(a, keys, &per);
             }
             const int upto = wave_prefix(blocks * splits, lane);
             const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > w);
             if (past != 0) {
                 const int at = __builtin_ctzll(past);
                 const int n = __builtin_amdgcn_readlane(blocks, at), each = __builtin_amdgcn_readlane(splits, at);
-                const int local = w - (before + __builtin_amdgcn_readlane(upto, at) - n * each), first = (int)((uint32_t)local / (uint32_t)each);
+                const int local = w - (before + __builtin_amdgcn_readlane(upto, at) - n * each);
+                const int block_of = each == 1 ? local : (int)((uint32_t)local / (uint32_t)each);
                 b = wave_uniform(b0 + at);
-                m = wave_uniform(n - 1 - first);
-                it->split = wave_uniform(local - first * each);
-                found = (uint32_t)first < (uint32_t)n;  // (sums of offsets that make no sense may overflow)
+                m = wave_uniform(n - 1 - block_of);
+                it->split = wave_uniform(local - block_of * each);
+                c0 = __builtin_amdgcn_readlane(first, at), c1 = __builtin_amdgcn_readlane(end, at), len = __builtin_amdgcn_readlane(keys, at);
+                found = (uint32_t)block_of < (uint32_t)n;  // (sums of offsets that make no sense may overflow)
                 break;
             }
             before += __builtin_amdgcn_readlane(upto, 63);
         }
         if (!found) return false;
     }
-    const int c0 = clamp_int(read_uniform_int(a.cu + b), 0, a.tokens), c1 = clamp_int(read_uniform_int(a.cu + b + 1), c0, a.tokens);
     it->b = b;
     it->tok0 = c0;
     it->rows = (c1 - c0) * a.G;
     it->row0 = m * BR;
-    it->len = clamp_int(read_uniform_int(a.lens + b), 0, a.capacity);
-    it->shift = it->len - (c1 - c0);
-    it->splits = splits_of_sequence(a, it->len, &it->per);
+    it->len = len;
+    it->shift = len - (c1 - c0);
+    it->splits = splits_of_sequence(a, len, &it->per);
     return it->row0 < it->rows && it->split < it->splits;
 }
 
@@ -992,11 +996,12 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
     };
 
     // ---- prologue
+    req.ask(a, 0);
     load_q<KS>(a, it, r, g, qf);
 #pragma unroll
     for (int t = 0; t < 3; ++t) {
         if (t < ntiles) {
-            req.ask(a, t);
+            if (t > 0) req.ask(a, t);
             req.load_k(a, t, Ks + t * T::BUF);
             req.find_v(a);
             if (t < 2) req.load_v(a, t, Vs + t * T::BUF);

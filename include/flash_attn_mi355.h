@@ -215,7 +215,7 @@ typedef struct flash_rotary_params {
     const void *X;
     void *Y;
     int dtype;            /* FLASH_FP16, FLASH_BF16 or FLASH_FP32 */
-    int B, H, N, d;       /* rows of d elements, [B,H,N,d] */
+    int B, H, N, d;       /* rows of d elements, [B,H,N,d]; B * N at most 2^25 */
     int rot;              /* even, 2 ... min(d, 512) */
     int64_t x_batch, x_head, x_row, y_batch, y_head, y_row;
     const void *positions;     /* of row n of batch b: positions[b * positions_batch + n] */
@@ -242,7 +242,7 @@ typedef struct flash_paged_params {
     const int32_t *block_table, *seqlens_k, *cu_seqlens_q;
     int dtype;            /* FLASH_FP16 or FLASH_BF16 */
     int B, H, H_kv, d;    /* H a multiple of H_kv; d a multiple of 8 up to FLASH_MAX_HEAD_DIM */
-    int total_q, num_pages, page_size, max_pages;   /* page_size: a multiple of 16; max_pages: entries of a row of the table */
+    int total_q, num_pages, page_size, max_pages;   /* total_q: at most 2^25; page_size: a multiple of 16; max_pages: entries of a row of the table */
     int64_t q_token, q_head, o_token, o_head, k_token, k_head, v_token, v_head;   /* multiples of 8, as all strides of rows here */
     int64_t kc_page, kc_head, kc_row, vc_page, vc_head, vc_row;
     int64_t block_table_stride;

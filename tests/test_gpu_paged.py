@@ -97,6 +97,59 @@ def test_many_sequences(fa):
     check(fa, Batch([1] * 150, [1 + (31 * b) % 500 for b in range(150)], 2, 1, 64, 16, F16, seed=6), causal=True, max_seqlen_q=1)
 
 
+@pytest.mark.parametrize("H", [33, 64, 96, 128])
+def test_one_head_for_many(fa, H):
+    """More query heads per K/V head than a work-group of few rows has rows."""
+    for news, lens in (([1, 1], [300, 90]), ([3, 2], [200, 65])):
+        for splits in (0, 2):
+            check(fa, Batch(news, lens, H, 1, 64, 16, BF16, seed=H), causal=True, max_seqlen_q=max(news), num_splits=splits)
+
+
+def test_long_chunks_of_short_launches(fa):
+    """Chunks of more than 64 rows that work-groups of 32 rows take, and the same sequences in a launch that they do not."""
+    for d, dtype in ((64, F16), (128, BF16)):
+        few = Batch([90, 500, 1], [200, 700, 64], 2, 2, d, 16, dtype, seed=21)
+        check(fa, few, causal=True)
+        check(fa, few, causal=True, window=(33, -1))
+        check(fa, few)
+        many = Batch([90] * 40, [200] * 40, 32, 32, d, 16, dtype, seed=22)
+        o, lse = run(fa, many, causal=True)
+        for b in (0, 17, 39):
+            one = Batch([90], [200], 32, 32, d, 16, dtype)
+            one.q, one.k_cache, one.v_cache, one.table = many.q[90 * b:90 * b + 90], many.k_cache, many.v_cache, many.table[b:b + 1]
+            ref.check_attention(o[90 * b:90 * b + 90], lse[90 * b:90 * b + 90], one.reference(causal=True), f"{d} {b}")
+
+
+def test_no_pages(fa):
+    """An empty pool, and a table without columns: rows see nothing, tokens go nowhere."""
+    q, k = torch.randn((3, 4, 64), device="cuda").half(), torch.randn((3, 2, 64), device="cuda").half()
+    lens, cu = torch.tensor([7, 2], dtype=torch.int32, device="cuda"), torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
+    for pages, width in ((0, 4), (5, 0), (0, 0)):
+        kc, vc = (torch.full((pages, 2, 16, 64), 3.0, dtype=F16, device="cuda") for _ in range(2))
+        table = torch.zeros((2, width), dtype=torch.int32, device="cuda")
+        for splits in (0, 4):
+            o, lse = fa.flash_forward_paged(q, kc, vc, table, lens, cu, causal=True, num_splits=splits)
+            assert (o == 0).all() and torch.isneginf(lse).all()
+        f = fa.rotary_frequencies(64, device="cuda")[0]
+        turned = fa.flash_append_paged(k, k, kc, vc, table, lens, cu, q=q, inv_freq=f)
+        assert torch.isfinite(turned).all() and (kc == 3).all() and (vc == 3).all()
+    assert fa.flash_forward_paged(q[:0], kc, vc, table[:0], lens[:0], cu[:1])[0].shape == (0, 4, 64)
+    assert fa.flash_append_paged(k[:0], k[:0], kc, vc, table, lens, cu) is None
+
+
+def test_shared_pages(fa):
+    """Two sequences whose tables begin with the same pages, and one table for all."""
+    batch = Batch([1, 40], [200, 300], 4, 2, 64, 16, F16, seed=23)
+    batch.table[1, :10] = batch.table[0, :10]
+    check(fa, batch, causal=True)
+    q, k, v, table, lens, cu = batch.cuda()
+    lens[:] = 200
+    o, lse = fa.flash_forward_paged(q, k, v, table[:1].expand(2, -1), lens, cu, causal=True)
+    batch.table[1] = batch.table[0]
+    batch.lens[:] = 200
+    ref.check_attention(o, lse, batch.reference(causal=True))
+
+
 def test_promises_of_lengths_are_about_speed(fa):
     """max_seqlen_k below the truth, max_seqlen_q above it."""
     batch = Batch([1, 1], [3000, 2000], 8, 2, 128, 16, F16)
