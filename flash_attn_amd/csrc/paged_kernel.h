@@ -8,17 +8,21 @@
 // are read once per K/V head, whatever G is.
 //
 // Pages.  A request of the tile loads (global_load_lds_dwordx4, one KiB) covers 4 rows of 256 bytes or 8 of 128.  Tiles begin at multiples of
-// 64 keys and pages hold multiples of 16, so the rows of a request lie in one page: its place is worked out on the scalar unit (an
-// entry of the table by s_load, one tile ahead of its use) and the lanes' own offsets never change.  No vector instruction goes
-// into paging, and with it no page size costs more than another.
+// 32 keys and pages hold multiples of 16, so the rows of a request lie in one page: its place is worked out on the scalar unit (an
+// entry of the table by s_load, one tile ahead of its use, and two 32 x 32 -> 64-bit products) and the lanes' own offsets never change.
+// No vector instruction goes into paging, and with it no page size costs more than another: 119 scalar instructions per tile and
+// wave of the tall form beside 194 vector instructions and 32 MFMAs (185 with every address worked out where it is used).
 //
 // Two forms share the mathematics of fwd_kernel.h (S^T = K Q^T and O^T += V^T P^T on 32x32x16 MFMA, one query row per lane, scores
 // scaled inside the exponent, a running maximum that is raised only when some row outgrows it by 2^8):
 //   paged_tall_kernel  256 rows per work-group, eight waves that share the tiles, the schedule of fwd_pp_kernel.h: on every SIMD one
-//                      wave is at its MFMAs while the other is at its softmax.  Bound by MFMA and softmax.
-//   paged_few_kernel   up to 32 rows, four waves that share out the tiles, each with LDS stages of its own and no barrier in the loop;
-//                      the four results are merged through LDS.  Bound by HBM.
-// Either form may split the key range (num_splits): partial results in fp32, merged by paged_merge_kernel.
+//                      wave is at its MFMAs while the other is at its softmax.  Bound by MFMA and softmax (and by the clock that the
+//                      power management leaves them): 8192 causal rows H32 H_kv8 d128 bf16 505-537 us, 1.02-1.09 PFLOP/s.
+//   paged_few_kernel   32 rows, four waves that share out the tiles, each with LDS stages of its own and no barrier in the loop;
+//                      the four results are merged through LDS.  Bound by HBM: single tokens B16 H32 H_kv32 on 4096 keys d128 163 us,
+//                      6.6 TB/s.
+// Either form may split the key range (num_splits): partial results in fp32, merged by paged_merge_kernel.  Which one a call gets:
+// rows_per_group in paged_api.hip.
 //
 // What is not in the sequence must not reach the result: keys past its end are not read (their rows repeat the last key's), columns
 // d ... D - 1 of the tiles in LDS are zeroed once and never requested, and a product of a masked probability, 0, with a V that is
@@ -505,8 +509,10 @@ __device__ __forceinline__ bool any_not_finite(const v16f (&oacc)[MB])
 // ---------------------------------------------------------------------------------------------- few rows
 
 // A wave has one stage of 8 KiB for K and for V each: tiles of 32 keys (256-byte rows) or 64.  K of the next tile is requested as soon as the scores
-// of this one have read theirs, V behind the second product.  With 64 to 68 KiB per work-group two share a CU: one streams while the other begins,
-// merges or ends.
+// of this one have read theirs, V behind the second product; requests are non-temporal, since nobody else asks for the keys.  With 64 to
+// 68 KiB per work-group two share a CU: one streams while the other begins, merges or ends.  Tiles of 64 keys at d = 128, two stages at
+// d = 64, one work-group per CU -> so: single tokens B64 H32 H_kv8 up to 500 keys 24.2 -> 15.0 us, up to 16384 391 -> 375 (unsplit), B64 H16 d64
+// 2000 keys 89.8 -> 79.7 (6.6 TB/s), B1 H32 H_kv8 32000 in 32 splits 27.9 -> 26.7.
 template <int D>
 struct FewCfg {
     static constexpr int kWaves = 4, BC = D == 128 ? 32 : 64;
@@ -845,10 +851,11 @@ struct TallCfg {
 };
 
 // Waves 0-3 and 4-7 run half an iteration apart (the second group passes one more barrier in front of the loop): while one wave of a
-// SIMD is at its softmax, the other is at its MFMAs.  V(t + 2) is requested at the start of iteration t and waited for at its end, K(t + 3) at
+// SIMD is at its softmax, the other is at its MFMAs.  A tile of 256 rows x 64 keys at d = 128 takes a CU 1.97 us, as in fwd_pp_kernel, 90 % of
+// what that mix of MFMAs and softmax reaches without any waits; ragged prompts up to 4096 H32 H_kv4 fp16 372 us, 0.92 PFLOP/s.  V(t + 2) is requested at the start of iteration t and waited for at its end, K(t + 3) at
 // its end and waited for at the next one's; their slots were last read two barriers before.
 // DU: columns that are worked on, a multiple of 32 from d on (rows in LDS have D): with DU = D the products of d = 80 meet zeroes in
-// every third MFMA.
+// every third MFMA (a window of 512 keys B3 H12 N1777 32.1 -> 29.8 us).
 template <int D, int DU, bool kBf16>
 __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const PagedArgs a)
 {
@@ -1058,8 +1065,9 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
 // ---------------------------------------------------------------------------------------------- merge of splits
 
 // O = sum_s w_s O_s, LSE = log sum_s exp LSE_s with w_s = exp(LSE_s - LSE): one or (kWaves = 4, few rows with many splits) four waves per
-// row.  Half a wave reads one split's row, 16 bytes per lane.  Bound by latency where there are few rows: the first rows are requested
-// before their weights are known.  (What a split that found nothing has in its place is not looked at: its weight is 0.)
+// row.  Half a wave reads one split's row, 16 bytes per lane.  Bound by latency where there are few rows (32 rows x 27 splits of 128 columns
+// 3.3 us): the first rows are requested before their weights are known; by HBM where there are many (16384 x 4: 9.8 us, 38 MB).  (What a
+// split that found nothing has in its place is not looked at: its weight is 0.)
 template <bool kBf16, int kWaves>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMergeArgs a)
 {

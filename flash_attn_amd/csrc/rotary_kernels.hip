@@ -10,7 +10,9 @@
 // Bound by memory: every element is read once and written once.  A wave has one token: its lanes work out the token's sines
 // and cosines, a pair each, into LDS of the wave's own, and then walk the rows (heads) of the token in pieces of a pair of 16-byte chunks, whose
 // angles they read back from there.  So an angle costs its 64-bit products and its sine once per token, not once per head.  Tokens of
-// short launches are shared out among `parts` waves.
+// short launches are shared out among `parts` waves.  Measured on one MI355X: rotary B4 H32 N4096 d128 bf16 43-52 us (5.2-6.2 TB/s read and
+// written, a copy of that size 4.7-4.9), append of 16384 tokens H32 H_kv8 d128 with Q 79 us (5.1 TB/s), one token H32 2.2 us and 64 of them into
+// their pages 4 us of GPU time (a launch).  (The rows' first pieces requested in front of the angles: d80 6.3 -> 6.1 us, but N4096 43.1 -> 47.4.)
 #include "rotary_kernels.h"
 
 namespace fa {
@@ -176,7 +178,9 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
     }
 }
 
-constexpr int kBusyWaves = 4096;  // waves that keep the memory busy: 16 per CU
+// Waves that keep the memory busy: 8 per CU.  (2048 / 4096 / 8192: append of 2620 tokens H16 H_kv4 d64 7.9 / 8.0 / 9.8 us, 512 tokens H32 H_kv8 d128
+// 5.5 / 5.8 / 5.7, rotary B3 H12 N1777 d80 6.3 / 6.3 / 7.1.)
+constexpr int kBusyWaves = 2048;
 
 // waves per token: as many as there are pieces of 64 chunks, as long as the launch is short of waves
 inline int parts_for(int64_t tokens, int64_t pieces)
