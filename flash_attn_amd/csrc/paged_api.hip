@@ -38,6 +38,8 @@ int run_rotary(const flash_rotary_params* p, hipStream_t st)
     // (in place: the same rows, not others of the same memory)
     if (p->X == p->Y && ((p->B > 1 && p->x_batch != p->y_batch) || (p->H > 1 && p->x_head != p->y_head) || (p->N > 1 && p->x_row != p->y_row)))
         return FLASH_EINVAL;
+    // (rows that are one and the same cannot be written)
+    if ((p->B > 1 && p->y_batch == 0) || (p->H > 1 && p->y_head == 0) || (p->N > 1 && p->y_row == 0)) return FLASH_EINVAL;
     const size_t size = p->dtype == FLASH_FP32 ? 4 : 2;
     if (misaligned(p->X, size) || misaligned(p->Y, size) || misaligned(p->positions, p->positions_64 ? 8 : 4) || misaligned(p->inv_freq, 4))
         return FLASH_EALIGN;
@@ -98,6 +100,9 @@ int validate_cache(const flash_paged_params* p)
     }
     return FLASH_OK;
 }
+
+// rows [tokens, heads, d] that are written: no two of them the same
+bool apart(int64_t token, int64_t head, int tokens, int heads) { return (tokens <= 1 || token != 0) && (heads <= 1 || head != 0); }
 
 int rows_strides(int64_t token, int64_t head, const void* base)
 {
@@ -194,7 +199,7 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     if (empty) return FLASH_OK;
     if ((rc = validate_cache(p)) != FLASH_OK) return rc;
     if ((rc = rows_strides(p->q_token, p->q_head, p->Q)) != FLASH_OK || (rc = rows_strides(p->o_token, p->o_head, p->O)) != FLASH_OK) return rc;
-    if (!p->LSE) return FLASH_EINVAL;
+    if (!p->LSE || !apart(p->o_token, p->o_head, p->total_q, p->H)) return FLASH_EINVAL;
     if (misaligned(p->LSE, 4)) return FLASH_EALIGN;
     const int br = rows_per_group(p), splits = splits_of(p), nt = most_tiles(p, br);
     if (splits > 1) {
@@ -240,8 +245,12 @@ int run_append(const flash_paged_params* p, hipStream_t st)
     if (empty) return FLASH_OK;
     if ((rc = validate_cache(p)) != FLASH_OK) return rc;
     if ((rc = rows_strides(p->k_token, p->k_head, p->K)) != FLASH_OK || (rc = rows_strides(p->v_token, p->v_head, p->V)) != FLASH_OK) return rc;
+    if (p->num_pages > 0 && (!apart(p->kc_page, p->kc_head, p->num_pages, p->H_kv) || p->kc_row == 0 || !apart(p->vc_page, p->vc_head, p->num_pages, p->H_kv) ||
+                             p->vc_row == 0))
+        return FLASH_EINVAL;
     if (queries) {
         if ((rc = rows_strides(p->q_token, p->q_head, p->Q)) != FLASH_OK || (rc = rows_strides(p->o_token, p->o_head, p->O)) != FLASH_OK) return rc;
+        if (!apart(p->o_token, p->o_head, p->total_q, p->H)) return FLASH_EINVAL;
         if (p->Q == p->O && ((p->total_q > 1 && p->q_token != p->o_token) || (p->H > 1 && p->q_head != p->o_head))) return FLASH_EINVAL;
     }
     if ((rc = device_usable()) != FLASH_OK) return rc;

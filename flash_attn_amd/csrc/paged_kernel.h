@@ -14,7 +14,9 @@
 // wave of the tall form beside 194 vector instructions and 32 MFMAs (185 with every address worked out where it is used).
 //
 // Two forms share the mathematics of fwd_kernel.h (S^T = K Q^T and O^T += V^T P^T on 32x32x16 MFMA, one query row per lane, scores
-// scaled inside the exponent, a running maximum that is raised only when some row outgrows it by 2^8):
+// scaled inside the exponent, a running maximum that is raised only when some row outgrows it by 2^8).  Scores, maxima, sums and O are held in
+// 32 bits, partial results of splits and waves too; the probabilities are rounded once, to nearest, to the type of V, whose matrix product takes
+// no other, behind the sum of the denominator, which has them as they are:
 //   paged_tall_kernel  256 rows per work-group, eight waves that share the tiles, the schedule of fwd_pp_kernel.h: on every SIMD one
 //                      wave is at its MFMAs while the other is at its softmax.  Bound by MFMA and softmax (and by the clock that the
 //                      power management leaves them): 8192 causal rows H32 H_kv8 d128 bf16 505-537 us, 1.02-1.09 PFLOP/s.

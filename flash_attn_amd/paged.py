@@ -108,6 +108,11 @@ def _check(cond, text):
         raise ValueError(text)
 
 
+def _int(v):
+    """v as a C int; what lies outside is as good as the nearest one."""
+    return max(-_INT_MAX, min(int(v), _INT_MAX))
+
+
 def _same_device(*tensors):
     """The device of all tensors that are given."""
     device = None
@@ -391,11 +396,11 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
     p = _paged_params(k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, H, T)
     p.q_token, p.q_head = _rows(q, "q", H, k_cache.shape[3], k_cache.dtype)
     p.Q = q.data_ptr()
-    p.max_seqlen_q, p.max_seqlen_k = min(int(max_seqlen_q), _INT_MAX), min(int(max_seqlen_k), _INT_MAX)
+    p.max_seqlen_q, p.max_seqlen_k = _int(max_seqlen_q), _int(max_seqlen_k)
     p.softmax_scale = float(softmax_scale) if softmax_scale is not None else d ** -0.5
     p.is_causal = int(bool(causal))
-    p.window_left, p.window_right = int(window[0]), int(window[1])
-    p.num_splits = int(num_splits)
+    p.window_left, p.window_right = _int(window[0]), _int(window[1])
+    p.num_splits = _int(num_splits)
     given = workspace if workspace is not None else ()
     device = _same_device(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, out, lse, *given)
     L = _lib()
@@ -426,8 +431,8 @@ def _paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max
     _lib().flash_paged_params_init(C.byref(p))
     p.B, p.H, p.H_kv, p.d, p.total_q, p.page_size, p.max_pages = B, H, H_kv, d, total_q, page_size, max_pages
     p.num_pages = 1
-    p.max_seqlen_q, p.max_seqlen_k = max_seqlen_q, max_seqlen_k
-    p.is_causal, p.window_left, p.window_right, p.num_splits = int(bool(causal)), int(window[0]), int(window[1]), num_splits
+    p.max_seqlen_q, p.max_seqlen_k = _int(max_seqlen_q), _int(max_seqlen_k)
+    p.is_causal, p.window_left, p.window_right, p.num_splits = int(bool(causal)), _int(window[0]), _int(window[1]), _int(num_splits)
     return p
 
 

@@ -80,6 +80,14 @@ def test_splits_of_chunks(fa, splits, dtype, d):
     check(fa, Batch([100, 3, 290], [1500, 100, 290], 4, 2, d, 16, dtype, seed=splits), causal=True, num_splits=splits)
 
 
+def test_bounds_past_a_c_int(fa):
+    batch = Batch([40], [300], 2, 1, 64, 16, F16, seed=24)
+    want = run(fa, batch, causal=True, window=(-1, -1))
+    for kw in (dict(window=(2 ** 32 + 5, -1)), dict(window=(-2 ** 32 + 5, 2 ** 40)), dict(max_seqlen_q=2 ** 40, max_seqlen_k=2 ** 33)):
+        got = run(fa, batch, causal=True, **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_lengths_of_nothing(fa):
     """Sequences without keys, without new tokens, with more new tokens than keys: rows in front of key 0 see nothing."""
     for news, lens in (([1, 1, 1], [0, 5, 0]), ([40, 0, 3, 290], [10, 9, 0, 280]), ([2, 3], [1, 0])):

@@ -56,7 +56,8 @@ def rotary_params(paged, **kw):
     (E_INVAL, {"rot": 0}), (E_INVAL, {"rot": 3}), (E_INVAL, {"rot": 66}), (E_INVAL, {"d": 1000, "rot": 514}), (E_INVAL, {"factor": math.nan}),
     (E_INVAL, {"factor": math.inf}), (E_INVAL, {"X": None}), (E_INVAL, {"Y": None}), (E_INVAL, {"positions": None}), (E_INVAL, {"inv_freq": None}),
     (E_INVAL, {"x_row": -64}), (E_INVAL, {"y_head": -1}), (E_INVAL, {"positions_batch": -1}), (E_INVAL, {"B": 2 ** 30, "N": 2 ** 30}), (E_INVAL, {"B": 2, "N": 2 ** 24 + 1}),
-    (E_INVAL, {"Y": 0x10000, "y_row": 128}), (E_INVAL, {"Y": 0x10000, "y_head": 64}),
+    (E_INVAL, {"Y": 0x10000, "y_row": 128}), (E_INVAL, {"y_row": 0}), (E_INVAL, {"y_head": 0}), (E_INVAL, {"B": 2, "y_batch": 0}),
+    (E_INVAL, {"Y": 0x10000, "x_row": 0, "y_row": 0}), (E_INVAL, {"Y": 0x10000, "y_head": 64}),
     (E_ALIGN, {"X": 0x10001}), (E_ALIGN, {"Y": 0x20001}), (E_ALIGN, {"dtype": 2, "X": 0x10002}), (E_ALIGN, {"positions": 0x30002}),
     (E_ALIGN, {"positions": 0x30004, "positions_64": 1}), (E_ALIGN, {"inv_freq": 0x40002}), (0, {"B": 0}), (0, {"H": 0}), (0, {"N": 0, "X": None})])
 def test_rotary_refuses(paged, code, kw):
@@ -103,7 +104,7 @@ def test_paged_calls_refuse(paged, code, kw):
 
 @pytest.mark.parametrize("code,kw", [
     (E_INVAL, {"softmax_scale": 0.0}), (E_INVAL, {"softmax_scale": -1.0}), (E_INVAL, {"softmax_scale": math.nan}), (E_INVAL, {"softmax_scale": math.inf}),
-    (E_INVAL, {"LSE": None}), (E_ALIGN, {"LSE": 0x70002}), (E_SPLITS, {"num_splits": 129}), (E_WORKSPACE, {"num_splits": 4}),
+    (E_INVAL, {"LSE": None}), (E_INVAL, {"o_token": 0}), (E_INVAL, {"o_head": 0}), (E_ALIGN, {"LSE": 0x70002}), (E_SPLITS, {"num_splits": 129}), (E_WORKSPACE, {"num_splits": 4}),
     (E_WORKSPACE, {"num_splits": 4, "O_partial": 0x100000}), (E_ALIGN, {"num_splits": 4, "O_partial": 0x100008, "LSE_partial": 0x200000}),
     (E_ALIGN, {"num_splits": 4, "O_partial": 0x100000, "LSE_partial": 0x200002}), (E_INVAL, {"max_seqlen_q": -1}), (E_INVAL, {"max_seqlen_k": -1}),
     (E_INVAL, {"B": 2 ** 24, "total_q": 2 ** 24, "H": 100, "H_kv": 100})])
@@ -115,7 +116,7 @@ def test_forward_refuses(paged, code, kw):
 @pytest.mark.parametrize("code,kw", [
     (E_INVAL, {"rot": 0}), (E_INVAL, {"rot": 66}), (E_INVAL, {"rot": 7}), (E_INVAL, {"factor": math.nan}), (E_ALIGN, {"inv_freq": 0xb0002}),
     (E_ALIGN, {"positions": 0x11002}), (E_ALIGN, {"positions": 0x11004, "positions_64": 1}), (E_INVAL, {"K": None}), (E_INVAL, {"V": None}),
-    (E_INVAL, {"k_token": 132}), (E_INVAL, {"v_head": 4}), (E_ALIGN, {"K": 0x30008}), (E_ALIGN, {"V": 0x40008}), (E_INVAL, {"O": 0x10000, "o_token": 1024})])
+    (E_INVAL, {"k_token": 132}), (E_INVAL, {"kc_page": 0}), (E_INVAL, {"kc_row": 0}), (E_INVAL, {"vc_head": 0}), (E_INVAL, {"o_token": 0}), (E_INVAL, {"v_head": 4}), (E_ALIGN, {"K": 0x30008}), (E_ALIGN, {"V": 0x40008}), (E_INVAL, {"O": 0x10000, "o_token": 1024})])
 def test_append_refuses(paged, code, kw):
     assert paged._lib().flash_append_paged(C.byref(paged_params(paged, **kw)), None) == code
     assert paged._lib().flash_append_paged(None, None) == E_INVAL
@@ -148,6 +149,11 @@ def test_split_counts_and_workspace(fa):
         fa.paged_resolve_splits(1, 8, 3, 64, 1, 16, 4)
     with pytest.raises(fa.FlashError):
         fa.paged_workspace_bytes(1, 8, 2, 64, 1, 16, 4, num_splits=129)
+    # what does not fit a C int is as good as what does
+    huge = dict(max_seqlen_q=2 ** 40, max_seqlen_k=2 ** 40, window=(2 ** 32 + 5, -2 ** 32 + 5))
+    assert fa.paged_resolve_splits(1, 8, 1, 64, 1, 16, 100, num_splits=7, **huge) == fa.paged_resolve_splits(1, 8, 1, 64, 1, 16, 100, num_splits=7)
+    with pytest.raises(fa.FlashError):
+        fa.paged_resolve_splits(1, 8, 1, 64, 1, 16, 100, num_splits=2 ** 32 + 1)
     # a window bounds the keys that there are to cut
     assert fa.paged_resolve_splits(1, 8, 1, 64, 1, 16, 10000, max_seqlen_q=1, causal=True, window=(63, -1), num_splits=128) <= 3
 
