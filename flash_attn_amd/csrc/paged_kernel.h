@@ -777,6 +777,13 @@ struct PagedRequests {
     }
 };
 
+// One KiB into LDS from an address of each lane's own (dma_kib in common.h).
+__device__ __forceinline__ void dma_kib_lanes(const char* at, FA_LDS char* lds_dst)
+{
+    const uint32_t m0v = (uint32_t)(uintptr_t)lds_dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0v), "v"(at) : "memory", "m0");
+}
+
 // LDS-only barrier: requests in flight are not waited for, and nothing moves across.
 __device__ __forceinline__ void paged_barrier()
 {
@@ -849,7 +856,9 @@ __device__ __forceinline__ void paged_store_rows(const PagedArgs& a, const Paged
 template <int D>
 struct TallCfg {
     static constexpr int kWaves = 8, NST = 4;                 // LDS stages per tensor
-    static constexpr int SMEM = NST * 2 * PagedTile<D>::BUF;  // 128 or 64 KiB
+    // 128 or 64 KiB of stages, and room for the Q rows of two waves; those of the others lie in stages that are empty at the start
+    static constexpr int QBUF = 32 * PagedTile<D>::ROW, SMEM = NST * 2 * PagedTile<D>::BUF + 2 * QBUF;
+    static_assert(2 * QBUF == PagedTile<D>::BUF, "Q rows of two waves per stage");
 };
 
 // Waves 0-3 and 4-7 run half an iteration apart (the second group passes one more barrier in front of the loop): while one wave of a
@@ -1004,9 +1013,24 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
         paged_barrier();
     };
 
-    // ---- prologue
+    // ---- prologue: Q, K(0), V(0), K(1), V(1), K(2) are requested in this order, and the first scores wait for Q and K(0) alone: 80 KiB
+    // per CU (D = 128), against 144 KiB for all.  Q takes the way of the tiles, whole rows per request, through LDS of the
+    // wave's own.  Before (Q by lanes into registers, one wait for everything) -> so: 1024 causal rows, B 8, H 32, d = 64 71.6 -> 67.8 us,
+    // 256 rows on 512 keys, B 128, H 8, d = 128 106.2 -> 103.0 us, 2048 rows, B 2, H 16, d = 80 51.8 -> 50.6 us.  What is
+    // left before the first scores, about 3 us, is these bytes' way from L2 into the CU: the page numbers of all three tiles asked
+    // for at once changed nothing.
     req.ask(a, 0);
-    load_q<KS>(a, it, r, g, qf);
+    FA_LDS char* const qst = wave < 2   ? Ks + 2 * NST * T::BUF + wave * C::QBUF
+                             : wave < 4 ? Vs + 2 * T::BUF + (wave - 2) * C::QBUF
+                             : wave < 6 ? Ks + 3 * T::BUF + (wave - 4) * C::QBUF
+                                        : Vs + 3 * T::BUF + (wave - 6) * C::QBUF;
+#pragma unroll
+    for (int x = 0; x < 32 / T::RPB; ++x) {
+        const int rl = T::RPB * x + lane / T::CPR, c = T::k_chunk(lane % T::CPR, rl), row = first_row + rl;
+        int head;
+        const int tok = row_token(a, it, row < it.rows ? row : it.rows - 1, &head);
+        if (c * 8 < a.d) dma_kib_lanes(a.Q + (size_t)tok * a.q_token + (size_t)head * a.q_head + c * 16, qst + x * 1024);
+    }
 #pragma unroll
     for (int t = 0; t < 3; ++t) {
         if (t < ntiles) {
@@ -1017,10 +1041,17 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
         }
     }
     req.ask(a, 3);  // (vnext: of tile 2)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (ntiles > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * NL) : "memory");
+    else if (ntiles == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NL) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+    {
+        const uint32_t qbase = fragment_base(qst, k_rd);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
-    paged_barrier();
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = k_fragment<D>(qbase, ks, 0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));  // in registers before the loop
+    }
+    paged_barrier();  // K(0) is there for all, and every wave has read its Q
     {
         const uint32_t kbase = fragment_base(Ks, k_rd);
 #pragma unroll
@@ -1032,6 +1063,10 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
             qk_mfma(ks);
         }
     }
+    if (ntiles > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+    else if (ntiles == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    paged_barrier();  // V(0) and K(1) too
     if (grp == 1) paged_barrier();
 
     // Tiles of which no row of this wave sees a key: only the wave's share of the requests and the barriers.
