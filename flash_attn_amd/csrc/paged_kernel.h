@@ -49,6 +49,7 @@ struct PagedArgs {
     const int32_t *table, *lens, *cu;
     FastDiv by_heads;
     int Hk, num_splits, B, direct;     // direct: every sequence has one row block
+    int ordered;                       // > 0: row blocks of all sequences by the end of their keys, in pieces of so many
     int tiles_per_split, window_tiles; // window_tiles: tiles of 64 keys that the masks leave a row block at most
     FastDiv by_splits, by_group, by_page;
     int H, G, d, tokens, num_pages, page, capacity;  // capacity: keys that a row of the table can name
@@ -149,7 +150,8 @@ __device__ __forceinline__ int splits_of_sequence(const PagedArgs& a, int len, i
 // of 8 of them the work-groups that read the same keys share an XCD's L2.  Behind that all pieces that the launch has come first, and the
 // work-groups that there are too many of (lengths are known on the device alone) last: work-groups are started in order and dealt to the parts of an
 // XCD in turn, and a launch with idle ones in between waits for one part with others empty.  Row blocks of a sequence come last first, which
-// under a causal mask is heaviest first.
+// under a causal mask is heaviest first; a.ordered: those of all sequences, by the piece of nine of the longest length in which their keys end,
+// the last piece first, a piece's sequences in turn.
 template <int BR>
 __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedItem* it)
 {
@@ -161,6 +163,40 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
         else it->split = w;
         c0 = clamp_int(read_uniform_int(a.cu + b), 0, a.tokens), c1 = clamp_int(read_uniform_int(a.cu + b + 1), c0, a.tokens);
         len = clamp_int(read_uniform_int(a.lens + b), 0, a.capacity);
+    } else if (a.ordered) {
+        // A lane per sequence, B <= 64.  Two looks at two ends each find the piece of the work-group's row block.
+        int first = 0, end = 0, keys = 0;
+        if (lane < a.B) {
+            first = a.cu[lane], end = a.cu[lane + 1], keys = a.lens[lane];
+            first = clamp_int(first, 0, a.tokens), end = clamp_int(end, first, a.tokens), keys = clamp_int(keys, 0, a.capacity);
+        }
+        const int n = ((end - first) * a.G + BR - 1) / BR, reach = a.causal ? 0 : a.wr;
+        auto ends_behind = [&](int t) {  // the lane's blocks that see a key behind the first t pieces: its last ones, as ends do not fall
+            const int c = a.ordered * t;
+            int x = max(c - (keys - (end - first)), -(1 << 30)) - reach;  // the first token that sees key c
+            x = reach < 0 ? 0 : max(x, 0);
+            return keys <= c || x >= end - first ? 0 : n - x * a.G / BR;
+        };
+        int t0 = 0, f0 = n, f1 = 0, before = 0;  // blocks behind the piece's begin (0: all) and behind its end (none behind the last); f1 of all lanes
+#pragma unroll
+        for (int step = 3; step > 0; step -= 2) {
+            const int near = ends_behind(t0 + step), far = ends_behind(t0 + 2 * step);
+            const uint32_t all = (uint32_t)__builtin_amdgcn_readlane(wave_prefix(near + (far << 16), lane), 63);  // (kOrderedGroups: 16 bits hold each)
+            const int all_near = (int)(all & 0xffffu), all_far = (int)(all >> 16);
+            if (all_far > w) t0 += 2 * step, f0 = far;
+            else if (all_near > w) t0 += step, f0 = near, f1 = far, before = all_far;
+            else f1 = near, before = all_near;
+        }
+        const int upto = wave_prefix(f0 - f1, lane), local = w - before;
+        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > local);
+        if (past == 0) return false;
+        b = wave_uniform(__builtin_ctzll(past));
+        const int block_of = __builtin_amdgcn_readlane(f1, b) + local - (__builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(f0 - f1, b));
+        const int blocks = __builtin_amdgcn_readlane(n, b);
+        if ((uint32_t)block_of >= (uint32_t)blocks) return false;  // (sums of offsets that make no sense may overflow)
+        m = wave_uniform(blocks - 1 - block_of);
+        it->split = 0;
+        c0 = __builtin_amdgcn_readlane(first, b), c1 = __builtin_amdgcn_readlane(end, b), len = __builtin_amdgcn_readlane(keys, b);
     } else {
         // 64 sequences at a time, a lane each
         int before = 0;

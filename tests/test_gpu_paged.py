@@ -128,6 +128,21 @@ def test_long_chunks_of_short_launches(fa):
             ref.check_attention(o[90 * b:90 * b + 90], lse[90 * b:90 * b + 90], one.reference(causal=True), f"{d} {b}")
 
 
+@pytest.mark.parametrize("B,G,most", [(2, 4, 700), (3, 8, 400), (17, 2, 300), (64, 2, 80), (65, 2, 80)])
+def test_row_blocks_of_all_sequences_by_length(fa, B, G, most):
+    """Launches whose row blocks are ordered across sequences, and one of too many sequences for that: each block has its place, also where
+    sequences are empty, rows stand in front of key 0, or the promised lengths are too short."""
+    news = [most] + [(37 * b * most // 64 + b) % most for b in range(1, B)]
+    lens = [max(0, n + (29 * b) % 150 - 40) for b, n in enumerate(news)]
+    if B > 2:
+        news[2], lens[2] = 0, 0
+    batch = Batch(news, lens, 8 * G, 8, 64, 16, BF16, seed=B)
+    for kw in (dict(causal=True), dict(causal=True, window=(50, -1)), dict(), dict(window=(-1, 33)), dict(window=(70, 0))):
+        check(fa, batch, what=f"{kw}", num_splits=1, max_seqlen_q=max(news), **kw)
+    want, got = run(fa, batch, causal=True, num_splits=1), run(fa, batch, causal=True, num_splits=1, max_seqlen_k=20)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_no_pages(fa):
     """An empty pool, and a table without columns: rows see nothing, tokens go nowhere."""
     q, k = torch.randn((3, 4, 64), device="cuda").half(), torch.randn((3, 2, 64), device="cuda").half()
