@@ -171,8 +171,10 @@ int rows_per_group(const flash_paged_params* p)
 
 // Split count that the library chooses.  A work-group per CU at least, as long as each split has some tiles; and for single tokens of several
 // sequences, whose lengths nobody here knows, pieces of some kFewestTiles tiles, so that the long sequences of a batch do not outlast the
-// others.  The merge reads 8 B H d bytes per split and token more, which is little next to the keys of a piece.
-constexpr int kFewestTiles = 32, kMostGroups = 2048;
+// others.  The merge reads 8 B H d bytes per split and token more, which is little next to the keys of a piece.  Its launch costs 3 us, in
+// which a work-group of 32 rows walks some tiles: shorter ranges stay whole.  Whole / in splits, single tokens, H 8, H_kv 2, one MI355X: d = 128
+// 256 keys 6.3 / 9.3 us, 512 keys 8.6 / 9.3, 1024 keys 13.6 / 9.2; d = 64, G = 1: 512 keys 6.3 / 9.5, 1024 keys 8.9 / 9.5, 2048 keys 14.7 / 9.1.
+constexpr int kFewestTiles = 32, kMostGroups = 2048, kWholeTiles = 8, kWholeTiles64 = 16;
 int splits_of(const flash_paged_params* p)
 {
     const int br = rows_per_group(p), nt = most_tiles(p, br);
@@ -188,6 +190,7 @@ int splits_of(const flash_paged_params* p)
             more = nt / more < kMostGroups / groups ? nt / more : kMostGroups / groups;
             if (more > s) s = more;
         }
+        if (br == fa::kPagedFewRows && nt <= (p->d <= 64 ? kWholeTiles64 : kWholeTiles)) s = 1;
     }
     if (s > nt) s = nt;
     if (s > FLASH_MAX_SPLITS) s = FLASH_MAX_SPLITS;
