@@ -16,6 +16,7 @@ using fa::record_hip;
 
 constexpr int kNumCU = 256;  // MI355X
 constexpr int kMostTokens = 1 << 25;
+constexpr long long kMostOfToken = 1LL << 30;  // elements of a token's heads: the kernels count them in an int, with a launch's step on top
 
 // strides of rows that are moved 16 bytes at a time
 inline bool odd_stride(int64_t s) { return (s & 7) != 0; }
@@ -29,7 +30,7 @@ int run_rotary(const flash_rotary_params* p, hipStream_t st)
     if (p->B < 0 || p->H < 0 || p->N < 0 || p->d <= 0) return FLASH_EINVAL;
     if (p->rot < 2 || (p->rot & 1) || p->rot > p->d || p->rot > 512) return FLASH_EINVAL;
     // (a wave per row of a batch: a launch is limited to 2^32 threads)
-    if ((long long)p->B * p->N > kMostTokens || (long long)p->H * p->d > 0x7fffffffLL) return FLASH_EINVAL;
+    if ((long long)p->B * p->N > kMostTokens || (long long)p->H * p->d > kMostOfToken) return FLASH_EINVAL;
     if (!std::isfinite(p->factor)) return FLASH_EINVAL;
     for (int64_t s : {p->x_batch, p->x_head, p->x_row, p->y_batch, p->y_head, p->y_row, p->positions_batch})
         if (s < 0) return FLASH_EINVAL;
@@ -78,7 +79,7 @@ int validate_paged(const flash_paged_params* p, bool* empty)
     if (p->max_seqlen_q < 0 || p->max_seqlen_k < 0 || p->block_table_stride < 0) return FLASH_EINVAL;
     // (positions and keys stay far below 2^31 in the kernels' int arithmetic)
     if ((long long)p->page_size * p->max_pages > (1LL << 30) || p->total_q > kMostTokens || p->B > (1 << 24)) return FLASH_EINVAL;
-    if ((long long)p->total_q * p->H > 0x7fffffffLL - 0x1000000) return FLASH_EINVAL;
+    if ((long long)p->total_q * p->H > 0x7fffffffLL - 0x1000000 || (long long)p->H * p->d > kMostOfToken) return FLASH_EINVAL;
     if (p->num_splits > FLASH_MAX_SPLITS) return FLASH_ESPLITS;
     if (p->B == 0 || p->total_q == 0) *empty = true;
     return FLASH_OK;

@@ -181,7 +181,7 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
 #pragma unroll
         for (int step = 3; step > 0; step -= 2) {
             const int near = ends_behind(t0 + step), far = ends_behind(t0 + 2 * step);
-            const uint32_t all = (uint32_t)__builtin_amdgcn_readlane(wave_prefix(near + (far << 16), lane), 63);  // (kOrderedGroups: 16 bits hold each)
+            const uint32_t all = (uint32_t)__builtin_amdgcn_readlane(wave_prefix((int)((uint32_t)near + ((uint32_t)far << 16)), lane), 63);  // (kOrderedGroups: 16 bits hold each)
             const int all_near = (int)(all & 0xffffu), all_far = (int)(all >> 16);
             if (all_far > w) t0 += 2 * step, f0 = far;
             else if (all_near > w) t0 += step, f0 = near, f1 = far, before = all_far;

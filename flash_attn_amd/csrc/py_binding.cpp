@@ -322,7 +322,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n)
         p.interleaved = args[3] == Py_True, p.inverse = args[5] == Py_True;
         const int64_t dims = x->dim();
         if ((dims != 3 && dims != 4) || (p.dtype = dtype_of(*x)) < 0 || !unit_stride(*x) || !fits_int(*x) || !is_here(*x)) return not_implemented();
-        if (at::GradMode::is_enabled() && x->requires_grad()) return not_implemented();
+        if (at::GradMode::is_enabled() && (x->requires_grad() || f->requires_grad() || (out && out->requires_grad()))) return not_implemented();
         const bool tokens = dims == 3;
         p.B = tokens ? 1 : (int)x->size(0), p.H = (int)x->size(1), p.N = (int)x->size(tokens ? 0 : 2), p.d = (int)x->size(-1);
         if (!positions_ok(*pos) || !frequencies_ok(*f, p.d)) return not_implemented();

@@ -223,6 +223,8 @@ def _rotary(x, positions, inv_freq, interleaved, factor, inverse, out, stream):
     _check(tuple(positions.shape) == (N,) or (x.dim() == 4 and tuple(positions.shape) == (B, N)), "positions must be [N] or, for [B,H,N,d], [B,N]")
     _check(inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous(), "inv_freq must be contiguous fp32 [rot / 2]")
     _check(1 <= inv_freq.numel() <= x.shape[-1] // 2, "inv_freq must have 1 ... d / 2 elements")
+    _check(not torch.is_grad_enabled() or not inv_freq.requires_grad, "inv_freq gets no gradient: detach it")
+    _check(not torch.is_grad_enabled() or out is None or not out.requires_grad, "out must not require a gradient")
     device = _same_device(x, positions, inv_freq, out)
     with _on(device, stream) as handle:
         y = out
@@ -288,6 +290,7 @@ def flash_rotary(x, positions, inv_freq, interleaved=False, factor=1.0, inverse=
 
     if torch.is_grad_enabled() and x.requires_grad:
         _check(out is None, "out cannot be given for an x that requires a gradient")
+        _check(not inv_freq.requires_grad, "inv_freq gets no gradient: detach it")
         if _function is None:
             _function = _rotary_function()
         return _function.apply(x, positions, inv_freq, interleaved, factor, inverse, stream)
@@ -377,8 +380,9 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
     """Attention of the new tokens q [tokens,H,d] over their sequences' pages: (O [tokens,H,d], LSE fp32 [tokens,H]).
 
     Query head h reads K/V head h / (H / H_kv).  Token i of n stands at position seqlens_k - n + i; causal and window (left, right) are as in
-    flash_forward, from there.  max_seqlen_q: at least the longest chunk of the call (0: the number of tokens); max_seqlen_k: the longest sequence,
-    which decides into how many splits its keys are cut (0: what the table can name).  num_splits <= 0: the library's choice.
+    flash_forward, from there.  max_seqlen_q: at least the longest chunk of the call (0: the number of tokens), otherwise rows may stay
+    unwritten; max_seqlen_k: the longest sequence, which decides into how many splits its keys are cut (0: what the table can name).
+    num_splits <= 0: the library's choice.
     workspace: (O_partial, LSE_partial) of at least the bytes that paged_workspace_bytes says, otherwise allocated here.
     Rows that belong to no sequence are left as they are (new memory where out and lse are not given)."""
     if stream is None:
@@ -427,6 +431,7 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
 
 
 def _paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k, causal, window, num_splits):
+    _check(max(B, H, H_kv, d, total_q, page_size, max_pages) <= _INT_MAX, "sizes are too large")
     p = PagedParams()
     _lib().flash_paged_params_init(C.byref(p))
     p.B, p.H, p.H_kv, p.d, p.total_q, p.page_size, p.max_pages = B, H, H_kv, d, total_q, page_size, max_pages

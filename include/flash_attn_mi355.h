@@ -215,7 +215,7 @@ typedef struct flash_rotary_params {
     const void *X;
     void *Y;
     int dtype;            /* FLASH_FP16, FLASH_BF16 or FLASH_FP32 */
-    int B, H, N, d;       /* rows of d elements, [B,H,N,d]; B * N at most 2^25 */
+    int B, H, N, d;       /* rows of d elements, [B,H,N,d]; B * N at most 2^25, H * d at most 2^30 */
     int rot;              /* even, 2 ... min(d, 512) */
     int64_t x_batch, x_head, x_row, y_batch, y_head, y_row;
     const void *positions;     /* of row n of batch b: positions[b * positions_batch + n] */
@@ -241,7 +241,7 @@ typedef struct flash_paged_params {
     void *K_cache, *V_cache;   /* [num_pages, H_kv, page_size, d], any strides */
     const int32_t *block_table, *seqlens_k, *cu_seqlens_q;
     int dtype;            /* FLASH_FP16 or FLASH_BF16 */
-    int B, H, H_kv, d;    /* H a multiple of H_kv; d a multiple of 8 up to FLASH_MAX_HEAD_DIM */
+    int B, H, H_kv, d;    /* H a multiple of H_kv; d a multiple of 8 up to FLASH_MAX_HEAD_DIM; H * d at most 2^30 */
     int total_q, num_pages, page_size, max_pages;   /* total_q: at most 2^25; page_size: a multiple of 16; max_pages: entries of a row of the table */
     int64_t q_token, q_head, o_token, o_head, k_token, k_head, v_token, v_head;   /* multiples of 8, as all strides of rows here */
     int64_t kc_page, kc_head, kc_row, vc_page, vc_head, vc_row;
@@ -249,7 +249,7 @@ typedef struct flash_paged_params {
     /* forward */
     float *LSE;           /* fp32 [total_q, H], contiguous */
     float *O_partial, *LSE_partial;   /* workspace of num_splits > 1: flash_forward_paged_workspace_bytes */
-    int max_seqlen_q;     /* the longest chunk of the call; 0: total_q.  Rows of a longer one may stay unwritten */
+    int max_seqlen_q;     /* at least the longest chunk of the call, otherwise rows of O may stay unwritten; 0: total_q */
     int max_seqlen_k;     /* the longest sequence; 0: what the table can name.  Decides speed alone */
     float softmax_scale;  /* positive */
     int is_causal, window_left, window_right;   /* as in flash_params: row i of n sees key j with j <= i + seqlens_k - n, ... */

@@ -204,3 +204,15 @@ def test_offsets_past_32_bits(fa):
     check(fa.flash_rotary(x, positions.cuda(), f.cuda(), out=torch.empty((1, 2, 3, 64), dtype=torch.float16, device="cuda")), host, positions, f)
     fa.flash_rotary(x, positions.cuda(), f.cuda(), out=x)
     check(x, host, positions, f)
+
+
+def test_frequencies_that_need_a_gradient(fa):
+    """A learned inv_freq would get none: refused while gradients are recorded, taken where they are not."""
+    x, n, f = torch.randn((1, 2, 3, 16), device="cuda"), torch.arange(3, device="cuda"), torch.rand(8, device="cuda", requires_grad=True)
+    for y in (x, x.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="inv_freq gets no gradient"):
+            fa.flash_rotary(y, n, f)
+    with pytest.raises(ValueError, match="out must not"):
+        fa.flash_rotary(x, n, f.detach(), out=torch.zeros_like(x).requires_grad_())
+    with torch.no_grad():
+        assert torch.equal(fa.flash_rotary(x, n, f), fa.flash_rotary(x, n, f.detach()))

@@ -55,7 +55,7 @@ def rotary_params(paged, **kw):
     (E_INVAL, {"dtype": 3}), (E_INVAL, {"dtype": -1}), (E_INVAL, {"B": -1}), (E_INVAL, {"H": -1}), (E_INVAL, {"N": -1}), (E_INVAL, {"d": 0}),
     (E_INVAL, {"rot": 0}), (E_INVAL, {"rot": 3}), (E_INVAL, {"rot": 66}), (E_INVAL, {"d": 1000, "rot": 514}), (E_INVAL, {"factor": math.nan}),
     (E_INVAL, {"factor": math.inf}), (E_INVAL, {"X": None}), (E_INVAL, {"Y": None}), (E_INVAL, {"positions": None}), (E_INVAL, {"inv_freq": None}),
-    (E_INVAL, {"x_row": -64}), (E_INVAL, {"y_head": -1}), (E_INVAL, {"positions_batch": -1}), (E_INVAL, {"B": 2 ** 30, "N": 2 ** 30}), (E_INVAL, {"B": 2, "N": 2 ** 24 + 1}),
+    (E_INVAL, {"x_row": -64}), (E_INVAL, {"y_head": -1}), (E_INVAL, {"positions_batch": -1}), (E_INVAL, {"B": 2 ** 30, "N": 2 ** 30}), (E_INVAL, {"B": 2, "N": 2 ** 24 + 1}), (E_INVAL, {"H": 2 ** 24 + 1}), (E_INVAL, {"H": 2 ** 30, "d": 2, "rot": 2}),
     (E_INVAL, {"Y": 0x10000, "y_row": 128}), (E_INVAL, {"y_row": 0}), (E_INVAL, {"y_head": 0}), (E_INVAL, {"B": 2, "y_batch": 0}),
     (E_INVAL, {"Y": 0x10000, "x_row": 0, "y_row": 0}), (E_INVAL, {"Y": 0x10000, "y_head": 64}),
     (E_ALIGN, {"X": 0x10001}), (E_ALIGN, {"Y": 0x20001}), (E_ALIGN, {"dtype": 2, "X": 0x10002}), (E_ALIGN, {"positions": 0x30002}),
@@ -87,7 +87,7 @@ BOTH = [
     (E_INVAL, {"dtype": 2}), (E_INVAL, {"dtype": -1}), (E_INVAL, {"B": -1}), (E_INVAL, {"H": 0}), (E_INVAL, {"H_kv": 0}), (E_INVAL, {"H": 7}),
     (E_INVAL, {"d": 0}), (E_INVAL, {"d": 60, "rot": 4}), (E_HEADDIM, {"d": 136}), (E_INVAL, {"total_q": -1}), (E_INVAL, {"num_pages": -1}),
     (E_INVAL, {"page_size": 0}), (E_INVAL, {"page_size": 24}), (E_INVAL, {"page_size": -16}), (E_INVAL, {"max_pages": -1}),
-    (E_INVAL, {"page_size": 2 ** 16, "max_pages": 2 ** 16}), (E_INVAL, {"total_q": 2 ** 25, "H": 1024, "H_kv": 1024}), (E_INVAL, {"total_q": 2 ** 25 + 1}), (E_INVAL, {"B": 2 ** 25}),
+    (E_INVAL, {"page_size": 2 ** 16, "max_pages": 2 ** 16}), (E_INVAL, {"total_q": 2 ** 25, "H": 1024, "H_kv": 1024}), (E_INVAL, {"total_q": 2 ** 25 + 1}), (E_INVAL, {"B": 2 ** 25}), (E_INVAL, {"total_q": 1, "H": 2 ** 24 + 2}),
     (E_INVAL, {"block_table": None}), (E_INVAL, {"seqlens_k": None}), (E_INVAL, {"cu_seqlens_q": None}), (E_INVAL, {"K_cache": None}),
     (E_INVAL, {"V_cache": None}), (E_INVAL, {"block_table_stride": -1}), (E_INVAL, {"kc_row": 68}), (E_INVAL, {"vc_page": 2052}), (E_INVAL, {"vc_head": -64}),
     (E_INVAL, {"kc_row": 2 ** 27}), (E_INVAL, {"kc_page": 2 ** 31}), (E_INVAL, {"vc_page": 2 ** 33}), (E_INVAL, {"q_token": 516}), (E_INVAL, {"q_head": 4}), (E_INVAL, {"o_head": -64}), (E_INVAL, {"Q": None, "O": None, "K": None}),
@@ -198,6 +198,25 @@ def test_python_rotary_refuses(fa):
             fa.flash_rotary(*args)
     with pytest.raises(ValueError):
         fa.flash_rotary(x.requires_grad_(), n, f, out=torch.zeros((1, 2, 3, 16)))
+
+
+def test_gradients_that_nobody_works_out(fa):
+    x, n, f = torch.zeros((1, 2, 3, 16)), torch.arange(3), torch.ones(8, requires_grad=True)
+    for y in (x, x.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="inv_freq gets no gradient"):
+            fa.flash_rotary(y, n, f)
+    with pytest.raises(ValueError, match="out must not"):
+        fa.flash_rotary(x, n, f.detach(), out=torch.zeros((1, 2, 3, 16), requires_grad=True))
+
+
+def test_sizes_past_a_c_int(fa):
+    good = [1, 8, 8, 64, 1, 16, 100]
+    fa.paged_resolve_splits(*good)
+    for i in range(len(good)):
+        with pytest.raises(ValueError, match="too large"):
+            fa.paged_resolve_splits(*[2 ** 32 + v if k == i else v for k, v in enumerate(good)])
+        with pytest.raises(ValueError, match="too large"):
+            fa.paged_workspace_bytes(*[2 ** 32 + v if k == i else v for k, v in enumerate(good)])
 
 
 def test_frequencies(fa):
