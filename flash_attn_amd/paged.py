@@ -380,8 +380,8 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
     """Attention of the new tokens q [tokens,H,d] over their sequences' pages: (O [tokens,H,d], LSE fp32 [tokens,H]).
 
     Query head h reads K/V head h / (H / H_kv).  Token i of n stands at position seqlens_k - n + i; causal and window (left, right) are as in
-    flash_forward, from there.  max_seqlen_q: at least the longest chunk of the call (0: the number of tokens), otherwise rows may stay
-    unwritten; max_seqlen_k: the longest sequence, which decides into how many splits its keys are cut (0: what the table can name).
+    flash_forward, from there.  max_seqlen_q: at least the longest chunk of the call (0: the number of tokens), otherwise rows may be
+    missing or meaningless; max_seqlen_k: the longest sequence, which decides into how many splits its keys are cut (0: what the table can name).
     num_splits <= 0: the library's choice.
     workspace: (O_partial, LSE_partial) of at least the bytes that paged_workspace_bytes says, otherwise allocated here.
     Rows that belong to no sequence are left as they are (new memory where out and lse are not given)."""

@@ -249,7 +249,7 @@ typedef struct flash_paged_params {
     /* forward */
     float *LSE;           /* fp32 [total_q, H], contiguous */
     float *O_partial, *LSE_partial;   /* workspace of num_splits > 1: flash_forward_paged_workspace_bytes */
-    int max_seqlen_q;     /* at least the longest chunk of the call, otherwise rows of O may stay unwritten; 0: total_q */
+    int max_seqlen_q;     /* at least the longest chunk of the call, otherwise rows of O and LSE may be missing or meaningless; 0: total_q */
     int max_seqlen_k;     /* the longest sequence; 0: what the table can name.  Decides speed alone */
     float softmax_scale;  /* positive */
     int is_causal, window_left, window_right;   /* as in flash_params: row i of n sees key j with j <= i + seqlens_k - n, ... */
