@@ -170,9 +170,67 @@ int rows_per_group(const flash_paged_params* p)
     return groups <= kShortGroups && groups * tiles <= (p->d <= 64 ? kShortUnits64 : kShortUnits) ? fa::kPagedFewRows : fa::kPagedTallRows;
 }
 
-// Split count that the library chooses.  A work-group per CU at least, as long as each split has some tiles; and for single tokens of several
-// sequences, whose lengths nobody here knows, pieces of some kFewestTiles tiles, so that the long sequences of a batch do not outlast the
-// others.  The merge reads 8 B H d bytes per split and token more, which is little next to the keys of a piece.  Its launch costs 3 us, in
+// Whether the work-groups of a launch in splits are the pieces that its row blocks have, one after the other (PagedArgs::pieces): where the mask cuts
+// the ends of the ranges alone, and a wave has a lane for each split of each sequence.  (32 rows in long caches, where nearly all pieces are
+// there, stay in the order that leaves row blocks of the same keys to the same XCD.)
+bool real_pieces(const flash_paged_params* p, int br, int splits)
+{
+    if (splits < 2 || (long long)p->B * splits > 64 || window_left_of(p) >= 0 || (!p->is_causal && window_right_of(p) < 0)) return false;
+    return br == fa::kPagedTallRows || ((long long)longest_chunk(p) * group_of(p) > br && keys_of(p) / 2 <= longest_chunk(p));
+}
+
+// Splits by an estimate, for launches with several row blocks per sequence:
+//     begin + tiles of a piece * t + [splits > 1] (merge + partial results written and read at 7 TB/s)
+// as long as the pieces have a CU each, or half of one (32 rows, d <= 64: t grows by half then; at d = 128 two on a CU take twice as long).  Under
+// a causal mask the first row blocks have fewer pieces than the last, so there may be more splits than places per row block.  One MI355X, splits that a
+// CU for every row block and split would allow / by this rule, us: 4096 causal rows H4 d128 4: 47.7, 7: 40.7; H8 2: 72.4, 3: 63.0; 2 x 3000 rows
+// H4 2: 57.4, 4: 44.0; 1500 rows H16 H_kv2 2: 41.4, 4: 34.8; 8192 rows H4 d64 2: 80.0, 3: 63.5; where nothing is gained: 2048 rows in a window of 600, H16
+// H_kv8, 26.5 whole, 36.6 in 2.  32 rows: 2839 causal rows H1 d128 2: 24.1, 5: 19.3; 2 x up to 2359 rows H1 d96 1: 29.4, 2: 23.2; 875 rows on 4989 keys
+// H4 d64 2: 25.4, 4: 20.8; the worst of 130 random launches 367 rows on 8324 keys H2 d96 11: 19.3, 8: 21.0.
+constexpr double kPartialBytesPerUs = 7e6;
+int splits_by_estimate(const flash_paged_params* p, int br, int nt)
+{
+    // row blocks of a chunk of mean length behind the longest sequence's keys
+    const bool tall = br == fa::kPagedTallRows, narrow = p->d <= 64;
+    const int G = group_of(p), keys = keys_of(p), reach = p->is_causal ? 0 : window_right_of(p);
+    const int mean = (p->total_q + p->B - 1) / p->B, chunk = mean < longest_chunk(p) ? mean : longest_chunk(p);
+    const long long n = ((long long)chunk * G + br - 1) / br, parts = (long long)p->B * p->H_kv;
+    const double begin_us = tall ? 7.0 : 4.5, merge_us = tall ? 8.0 : 3.0, tile_us = tall ? (narrow ? 0.95 : p->d <= 96 ? 1.35 : 1.53) : narrow ? 0.365 : 0.6;
+    const double split_us = 8.0 * p->d * p->total_q * p->H / kPartialBytesPerUs;
+    const long long places = !tall && narrow ? 2 * kNumCU : kNumCU + kNumCU / 32;  // (a few more find a CU that short pieces have left)
+    double best = begin_us + nt * tile_us;
+    int chosen = 1;
+    for (int s = 2; s <= nt && s <= FLASH_MAX_SPLITS; ++s) {
+        const int per = (nt + s - 1) / s;
+        if ((nt + per - 1) / per != s) continue;  // (a smaller count says the same)
+        long long pieces = n * s;
+        if (real_pieces(p, br, s)) {
+            pieces = n;
+            if (s <= n) {
+                for (int k = 1; k < s; ++k) {
+                    const long long key = 64LL * per * k, x = key - (keys - chunk) - reach;
+                    pieces += keys <= key || x >= chunk ? 0 : n - (x > 0 ? x * G / br : 0);
+                }
+            } else {
+                for (long long m = 0; m < n; ++m) {
+                    const long long last = ((m + 1) * br < (long long)chunk * G ? (m + 1) * br : (long long)chunk * G) - 1, hi = keys - chunk + last / G + 1 + reach;
+                    const long long tiles = ((hi < keys ? hi : keys) + 63) / 64;
+                    pieces += tiles > per ? (tiles + per - 1) / per - 1 : 0;
+                }
+            }
+        } else if (!tall && (long long)s * p->H_kv > 8 && (long long)s * p->H_kv % 8 != 0) {
+            continue;  // (row blocks that read the same keys would lie on different XCDs: 80 rows on 13400 keys, B 8, H 1, 10 splits 34.7 us, 8 27.1)
+        }
+        if (pieces * parts > places) break;
+        const double us = begin_us + per * tile_us * (!tall && pieces * parts > kNumCU ? 1.5 : 1.0) + merge_us + split_us * pieces / n;
+        if (us < best) best = us, chosen = s;
+    }
+    return chosen;
+}
+
+// Split count that the library chooses.  One row block of 32 rows per sequence: a work-group per CU at least, as long as each split has two tiles; and
+// where there are several sequences, whose lengths nobody here knows, pieces of some kFewestTiles tiles, so that the long sequences of a batch do not
+// outlast the others.  The merge reads 8 B H d bytes per split and token more, which is little next to the keys of a piece.  Its launch costs 3 us, in
 // which a work-group of 32 rows walks some tiles: shorter ranges stay whole.  Whole / in splits, single tokens, H 8, H_kv 2, one MI355X: d = 128
 // 256 keys 6.3 / 9.3 us, 512 keys 8.6 / 9.3, 1024 keys 13.6 / 9.2; d = 64, G = 1: 512 keys 6.3 / 9.5, 1024 keys 8.9 / 9.5, 2048 keys 14.7 / 9.1.
 constexpr int kFewestTiles = 32, kMostGroups = 2048, kWholeTiles = 8, kWholeTiles64 = 16;
@@ -183,15 +241,19 @@ int splits_of(const flash_paged_params* p)
     long long s = p->num_splits;
     if (s <= 0) {
         const long long groups = blocks_of(p, br) * p->H_kv;
-        s = groups >= kNumCU ? 1 : kNumCU / groups;
-        const int least = br == fa::kPagedFewRows ? 2 : 4;  // tiles per split
-        if (s > nt / least) s = nt / least;
-        if (br == fa::kPagedFewRows && p->B > 1) {
+        if (br == fa::kPagedTallRows) return groups >= kNumCU ? 1 : splits_by_estimate(p, br, nt);
+        if (nt <= (p->d <= 64 ? kWholeTiles64 : kWholeTiles)) return 1;
+        if ((long long)longest_chunk(p) * group_of(p) > br) {
+            s = splits_by_estimate(p, br, nt);
+        } else {
+            s = groups >= kNumCU ? 1 : kNumCU / groups;
+            if (s > nt / 2) s = nt / 2;
+        }
+        if (p->B > 1) {
             long long more = kFewestTiles;
             more = nt / more < kMostGroups / groups ? nt / more : kMostGroups / groups;
             if (more > s) s = more;
         }
-        if (br == fa::kPagedFewRows && nt <= (p->d <= 64 ? kWholeTiles64 : kWholeTiles)) s = 1;
     }
     if (s > nt) s = nt;
     if (s > FLASH_MAX_SPLITS) s = FLASH_MAX_SPLITS;
@@ -250,6 +312,7 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     a.num_splits = splits, a.tiles_per_split = (nt + splits - 1) / splits, a.window_tiles = window_tiles(p, br);
     a.direct = (long long)longest_chunk(p) * a.G <= br;
     a.ordered = splits == 1 && ordered(p, br) ? (keys_of(p) + 8) / 9 : 0;
+    a.pieces = real_pieces(p, br, splits);
     a.by_heads = fa::fast_div(a.Hk), a.by_group = fa::fast_div(a.G), a.by_page = fa::fast_div(a.page);
     a.by_splits = fa::fast_div(splits);
     const bool bf16 = p->dtype == FLASH_BF16;

@@ -49,6 +49,7 @@ struct PagedArgs {
     const int32_t *table, *lens, *cu;
     FastDiv by_heads;
     int Hk, num_splits, B, direct;     // direct: every sequence has one row block
+    int pieces;                        // != 0: of the splits only those that a row block has
     int ordered;                       // > 0: row blocks of all sequences by the end of their keys, in pieces of so many
     int tiles_per_split, window_tiles; // window_tiles: tiles of 64 keys that the masks leave a row block at most
     FastDiv by_splits, by_group, by_page;
@@ -118,7 +119,7 @@ struct PagedItem {
     int tok0, rows;   // first token of the chunk; query rows of the problem (tokens times heads per K/V head)
     int row0;         // first row of the work-group
     int len, shift;   // keys; position of query 0
-    int splits, per;  // of the sequence; tiles of a split
+    int splits, per;  // of the sequence (a.pieces: of the row block); tiles of a split
 };
 
 // Lengths come from device memory: whatever they hold, nothing outside the tensors is touched.
@@ -146,12 +147,23 @@ __device__ __forceinline__ int splits_of_sequence(const PagedArgs& a, int len, i
     return nt <= each ? 1 : (int)((uint32_t)(nt + each - 1) / (uint32_t)each);
 }
 
+// Of a sequence's n row blocks those that see key c or one behind it: its last ones, as ends do not fall.
+template <int BR>
+__device__ __forceinline__ int blocks_behind(const PagedArgs& a, int tokens, int keys, int n, int c)
+{
+    const int reach = a.causal ? 0 : a.wr;
+    int x = max(c - (keys - tokens), -(1 << 30)) - reach;  // the first token that sees key c
+    x = reach < 0 ? 0 : max(x, 0);
+    return keys <= c || x >= tokens ? 0 : n - x * a.G / BR;
+}
+
 // Work-group -> (sequence, row block, split, K/V head); false where there is nothing to do.  K/V heads vary fastest, so that with a multiple
 // of 8 of them the work-groups that read the same keys share an XCD's L2.  Behind that all pieces that the launch has come first, and the
 // work-groups that there are too many of (lengths are known on the device alone) last: work-groups are started in order and dealt to the parts of an
 // XCD in turn, and a launch with idle ones in between waits for one part with others empty.  Row blocks of a sequence come last first, which
 // under a causal mask is heaviest first; a.ordered: those of all sequences, by the piece of nine of the longest length in which their keys end,
-// the last piece first, a piece's sequences in turn.
+// the last piece first, a piece's sequences in turn.  a.pieces: first splits of a sequence's row blocks, second splits of those that have one, ...: under a
+// causal mask the others would stand between them with nothing to do, and what comes behind the places of the GPU waits for a round.
 template <int BR>
 __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedItem* it)
 {
@@ -170,13 +182,8 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
             first = a.cu[lane], end = a.cu[lane + 1], keys = a.lens[lane];
             first = clamp_int(first, 0, a.tokens), end = clamp_int(end, first, a.tokens), keys = clamp_int(keys, 0, a.capacity);
         }
-        const int n = ((end - first) * a.G + BR - 1) / BR, reach = a.causal ? 0 : a.wr;
-        auto ends_behind = [&](int t) {  // the lane's blocks that see a key behind the first t pieces: its last ones, as ends do not fall
-            const int c = a.ordered * t;
-            int x = max(c - (keys - (end - first)), -(1 << 30)) - reach;  // the first token that sees key c
-            x = reach < 0 ? 0 : max(x, 0);
-            return keys <= c || x >= end - first ? 0 : n - x * a.G / BR;
-        };
+        const int n = ((end - first) * a.G + BR - 1) / BR;
+        auto ends_behind = [&](int t) { return blocks_behind<BR>(a, end - first, keys, n, a.ordered * t); };
         int t0 = 0, f0 = n, f1 = 0, before = 0;  // blocks behind the piece's begin (0: all) and behind its end (none behind the last); f1 of all lanes
 #pragma unroll
         for (int step = 3; step > 0; step -= 2) {
@@ -197,6 +204,27 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
         m = wave_uniform(blocks - 1 - block_of);
         it->split = 0;
         c0 = __builtin_amdgcn_readlane(first, b), c1 = __builtin_amdgcn_readlane(end, b), len = __builtin_amdgcn_readlane(keys, b);
+    } else if (a.pieces) {
+        // a lane per sequence and split, B * num_splits <= 64, windows without a left end: what is there of a split is the last row blocks
+        const int bl = a.by_splits.quotient(lane), s = lane - bl * a.num_splits;
+        int first = 0, end = 0, keys = 0, each = 1;
+        if (bl < a.B) {
+            first = a.cu[bl], end = a.cu[bl + 1], keys = a.lens[bl];
+            first = clamp_int(first, 0, a.tokens), end = clamp_int(end, first, a.tokens), keys = clamp_int(keys, 0, a.capacity);
+            splits_of_sequence(a, keys, &each);
+        }
+        const int n = ((end - first) * a.G + BR - 1) / BR;
+        const int there = s == 0 ? n : blocks_behind<BR>(a, end - first, keys, n, (int)min((int64_t)s * each * 64, (int64_t)keys));
+        const int upto = wave_prefix(there, lane);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > w);
+        if (past == 0) return false;
+        const int at = wave_uniform(__builtin_ctzll(past));
+        const int block_of = w - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(there, at)), blocks = __builtin_amdgcn_readlane(n, at);
+        if ((uint32_t)block_of >= (uint32_t)blocks) return false;
+        b = wave_uniform(a.by_splits.quotient(at));
+        it->split = at - b * a.num_splits;
+        m = wave_uniform(blocks - 1 - block_of);
+        c0 = __builtin_amdgcn_readlane(first, at), c1 = __builtin_amdgcn_readlane(end, at), len = __builtin_amdgcn_readlane(keys, at);
     } else {
         // 64 sequences at a time, a lane each
         int before = 0;
@@ -235,6 +263,11 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
     it->len = len;
     it->shift = len - (c1 - c0);
     it->splits = splits_of_sequence(a, len, &it->per);
+    if (a.pieces) {  // of the row block
+        const int last = min(it->row0 + BR, it->rows) - 1, reach = a.causal ? 0 : a.wr;
+        const int hi = reach < 0 ? len : min(len, a.by_group.quotient(last) + it->shift + reach + 1);
+        it->splits = hi <= it->per * 64 ? 1 : (int)((uint32_t)((hi + 63) / 64 + it->per - 1) / (uint32_t)it->per);
+    }
     return it->row0 < it->rows && it->split < it->splits;
 }
 

@@ -143,6 +143,23 @@ def test_row_blocks_of_all_sequences_by_length(fa, B, G, most):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("B,G,most,splits", [(1, 4, 1500, 7), (1, 4, 1500, 24), (2, 4, 700, 5), (3, 8, 400, 2), (17, 2, 300, 3), (17, 2, 300, 4), (16, 2, 300, 4), (3, 1, 300, 4),
+                                             (1, 1, 333, 6), (32, 1, 70, 2)])
+def test_pieces_that_row_blocks_have(fa, B, G, most, splits):
+    """Splits of chunks whose first row blocks have fewer pieces than the last, in work-groups of 256 and of 32 rows, also where sequences are
+    empty, rows stand in front of key 0, or the promised lengths are too short; two of too many sequences and splits for that order."""
+    news = [most] + [(37 * b * most // 64 + b) % most for b in range(1, B)]
+    lens = [max(0, n + (29 * b) % 250 - 60 * (b > 0)) for b, n in enumerate(news)]
+    if B > 2:
+        news[2], lens[2] = 0, 0
+    Hk = 8 if B * G > 3 else 2
+    batch = Batch(news, lens, Hk * G, Hk, 128, 16, F16, seed=B + splits)
+    for kw in (dict(causal=True), dict(causal=True, window=(50, -1)), dict(), dict(window=(-1, 33)), dict(causal=True, max_seqlen_k=max(lens)),
+               dict(causal=True, max_seqlen_k=40)):
+        check(fa, batch, what=f"{kw}", num_splits=splits, max_seqlen_q=max(news), **kw)
+    check(fa, batch, causal=True)
+
+
 def test_no_pages(fa):
     """An empty pool, and a table without columns: rows see nothing, tokens go nowhere."""
     q, k = torch.randn((3, 4, 64), device="cuda").half(), torch.randn((3, 2, 64), device="cuda").half()
