@@ -342,6 +342,25 @@ def test_tables_with_pages_that_are_not_there(fa):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("G,splits", [(8, 1), (8, 3), (1, 1), (1, 4)])
+def test_offsets_that_make_no_sense(fa, G, splits):
+    """In launches whose row blocks are ordered across sequences or come in pieces: rows in front of O and behind it stay as they are."""
+    batch = Batch([300, 20, 80], [400, 20, 200], 8 * G, 8, 64, 16, F16, seed=G)
+    q, k, v, table, lens, cu = batch.cuda()
+    T, H = q.shape[0], q.shape[1]
+    for bad in ([0, 300, 20, 400], [-4, 100, 200, 400], [0, 1, 399, 10 ** 9], [500, 500, 500, 500], [400, 300, 20, 0], [0, 2 ** 31 - 1, -2 ** 31, 400], [0, 400, 0, 400]):
+        cu.copy_(torch.tensor(bad, dtype=torch.int32))
+        for length in (None, -3, 2 ** 31 - 1):
+            own = lens.clone()
+            if length is not None:
+                own[1] = length
+            out, lse = torch.full((T + 64, H, 64), 7.0, dtype=F16, device="cuda"), torch.full((T + 64, H), 7.0, device="cuda")
+            for most in (300, 0):
+                fa.flash_forward_paged(q, k, v, table, own, cu, causal=True, max_seqlen_q=most, max_seqlen_k=400, num_splits=splits, out=out[32:32 + T], lse=lse[32:32 + T])
+            for x in (out, lse):
+                assert (x[:32] == 7).all() and (x[32 + T:] == 7).all()
+
+
 # ---- calls
 
 
