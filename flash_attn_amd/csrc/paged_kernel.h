@@ -932,17 +932,19 @@ struct TallCfg {
 
 // Waves 0-3 and 4-7 run half an iteration apart (the second group passes one more barrier in front of the loop): while one wave of a
 // SIMD is at its softmax, the other is at its MFMAs.  A tile of 256 rows x 64 keys at d = 128 takes a CU 1.97 us, as in fwd_pp_kernel, 90 % of
-// what that mix of MFMAs and softmax reaches without any waits; ragged prompts up to 4096 H32 H_kv4 fp16 372 us, 0.92 PFLOP/s.  V(t + 2) is requested at the start of iteration t and waited for at its end, K(t + 3) at
-// its end and waited for at the next one's; their slots were last read two barriers before.
-// DU: columns that are worked on, a multiple of 32 from d on (rows in LDS have D): with DU = D the products of d = 80 meet zeroes in
-// every third MFMA (a window of 512 keys B3 H12 N1777 32.1 -> 29.8 us).
+// what that mix of MFMAs and softmax reaches without any waits; ragged prompts up to 4096 H32 H_kv4 fp16 372 us, 0.92 PFLOP/s.  V(t + 2) is
+// requested at the start of iteration t and waited for at its end, K(t + 3) at its end and waited for at the next one's; their slots were last
+// read two barriers before.
+// DU: columns that are worked on, a multiple of 16 from d on, the scores in steps of 16, O in blocks of 32 (rows in LDS have D): with DU = D the
+// products of d = 80 meet zeroes in every third MFMA (a window of 512 keys B3 H12 N1777, DU 128, 96, 80: 32.1, 29.8, 29.3 us; 8 x up to 2000 rows H16
+// 69.9 -> 67.0 with 80; d = 40 on 8000 keys 89.7 -> 86.6 with 48; d = 112 138.0 -> 136.2 with 112).
 template <int D, int DU, bool kBf16>
 __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const PagedArgs a)
 {
     using T = PagedTile<D>;
     using C = TallCfg<D>;
     using E = Elem<kBf16>;
-    constexpr int KS = DU / 16, MB = DU / 32, NST = C::NST, NL = PagedRequests<D, C::kWaves>::NL, BC = T::BC;
+    constexpr int KS = DU / 16, MB = (DU + 31) / 32, NST = C::NST, NL = PagedRequests<D, C::kWaves>::NL, BC = T::BC;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     FA_LDS char* const Ks = (FA_LDS char*)smem;
     FA_LDS char* const Vs = Ks + NST * T::BUF;
@@ -1267,7 +1269,10 @@ template <int D, bool kBf16>
 inline int launch_paged_type(const PagedArgs& a, int rows, long long blocks, hipStream_t st)
 {
     if (rows == kPagedFewRows) return (int)launch_paged_instance<D, D, kBf16, kPagedFewRows>(a, blocks, st);
+    if constexpr (D == 128)
+        if (a.d <= 80) return (int)launch_paged_instance<D, 80, kBf16, kPagedTallRows>(a, blocks, st);
     if (a.d <= D - 32) return (int)launch_paged_instance<D, D - 32, kBf16, kPagedTallRows>(a, blocks, st);
+    if (a.d <= D - 16) return (int)launch_paged_instance<D, D - 16, kBf16, kPagedTallRows>(a, blocks, st);
     return (int)launch_paged_instance<D, D, kBf16, kPagedTallRows>(a, blocks, st);
 }
 template <int D>
