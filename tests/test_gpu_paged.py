@@ -434,6 +434,29 @@ def test_captured_steps_follow_lengths_and_pages(fa):
         assert torch.equal(k, mine[0]) and torch.equal(v, mine[1])
 
 
+@pytest.mark.parametrize("G,splits", [(8, 1), (8, 3), (1, 4)])
+def test_captured_chunks_follow_lengths_and_offsets(fa, G, splits):
+    """A captured call of ragged chunks, in order of lengths or in pieces, replayed with other chunks of the same tokens."""
+    Hk, d, T = 4, 64, 600
+    batch = Batch([300, 100, 200], [700, 700, 700], Hk * G, Hk, d, 16, BF16, seed=31)
+    q, k, v, table, lens, cu = batch.cuda()
+    kw = dict(causal=True, num_splits=splits, max_seqlen_q=600, max_seqlen_k=700)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, lse = fa.flash_forward_paged(q, k, v, table, lens, cu, **kw)
+    for news, keys in (([300, 100, 200], [700, 100, 333]), ([600, 0, 0], [600, 20, 0]), ([0, 1, 599], [5, 700, 650]), ([200, 200, 200], [200, 100, 700]), ([7, 590, 3], [7, 700, 3])):
+        cu.copy_(torch.tensor([0, news[0], news[0] + news[1], T], dtype=torch.int32))
+        lens.copy_(torch.tensor(keys, dtype=torch.int32))
+        want = fa.flash_forward_paged(q, k, v, table, lens, cu, **kw)
+        torch.cuda.synchronize()
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o, want[0]) and torch.equal(lse, want[1]), (news, keys)
+        batch.cu, batch.lens = cu.cpu(), lens.cpu()
+        ref.check_attention(o, lse, batch.reference(causal=True), f"{news} {keys}")
+
+
 # ---- append
 
 
