@@ -1138,7 +1138,13 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
     else if (ntiles == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     paged_barrier();  // V(0) and K(1) too
-    if (grp == 1) paged_barrier();
+    if (grp == 1) {
+        // V(1): the first group reads it before the barrier that ends this group's first iteration, behind which alone the second group's part of it
+        // would be sure to have landed
+        if (ntiles > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        paged_barrier();
+    }
 
     // Tiles of which no row of this wave sees a key: only the wave's share of the requests and the barriers.
     auto idle_iteration = [&](int t) {
