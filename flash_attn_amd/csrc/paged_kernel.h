@@ -26,9 +26,10 @@
 // Either form may split the key range (num_splits): partial results in fp32, merged by paged_merge_kernel.  Which one a call gets:
 // rows_per_group in paged_api.hip.
 //
-// What is not in the sequence must not reach the result: keys past its end are not read (their rows repeat the last key's), columns
-// d ... D - 1 of the tiles in LDS are zeroed once and never requested, and a product of a masked probability, 0, with a V that is
-// not finite is taken back out at the end (rescue).
+// What is not in the sequence must not reach the result: keys past its end are not read, columns d ... D - 1 of the tiles in LDS are zeroed once and
+// never requested, and a product of a masked probability, 0, with a V that is not finite is taken back out at the end (rescue).  Rows of a tile past the
+// sequence's end repeat the last key's in K, whose scores are masked.  In V they have to be finite whatever the last key holds, which its row may
+// see: in the 32-row form they come from a row of zeroes (kPagedZeroes), in the 256-row form they are cleared if need be (paged_clear_past).
 #pragma once
 #include <type_traits>
 
@@ -577,7 +578,20 @@ __device__ __forceinline__ bool any_not_finite(const v16f (&oacc)[MB])
     return __builtin_amdgcn_ballot_w64(!(z == 0.0f)) != 0ull;
 }
 
+// One KiB into LDS from an address of each lane's own (dma_kib and dma_kib_nt in common.h).
+template <bool kNt>
+__device__ __forceinline__ void dma_kib_lanes(const char* at, FA_LDS char* lds_dst)
+{
+    const uint32_t m0v = (uint32_t)(uintptr_t)lds_dst;
+    if constexpr (kNt) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" : : "s"(m0v), "v"(at) : "memory", "m0");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0v), "v"(at) : "memory", "m0");
+}
+
 // ---------------------------------------------------------------------------------------------- few rows
+
+// Where rows of V past a sequence's end come from.  (Rows that repeat the last key's and are looked over in LDS, as in the 256-row form, cost 0.3-1 us more at
+// the end of these short work-groups: 58 single tokens H64 H_kv16 d80 11.4 us with rows that nobody clears, 11.5 so, 12.5 looked over.)
+static __device__ const v4u kPagedZeroes = {0u, 0u, 0u, 0u};
 
 // A wave has one stage of 8 KiB for K and for V each: tiles of 32 keys (256-byte rows) or 64.  K of the next tile is requested as soon as the scores
 // of this one have read theirs, V behind the second product; requests are non-temporal, since nobody else asks for the keys.  With 64 to
@@ -646,8 +660,9 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
         for (int s = 0; s < GROUPS; ++s) place[s].ask(a, table_row, len, (tile0 + t) * BC + 16 * s);
     };
     // the rows of tile t (its places asked for) of K or V
-    auto request = [&](int t, const char* head, uint32_t page_bytes, uint32_t row_bytes, const uint32_t (&off)[kPer], const bool (&ok)[kPer],
+    auto request = [&](auto is_v_c, int t, const char* head, uint32_t page_bytes, uint32_t row_bytes, const uint32_t (&off)[kPer], const bool (&ok)[kPer],
                        FA_LDS char* dst) __attribute__((always_inline)) {
+        constexpr bool kIsV = decltype(is_v_c)::value;
         const int kb0 = (tile0 + t) * BC;
         const bool whole = kb0 + BC <= len;
 #pragma unroll
@@ -656,16 +671,21 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
 #pragma unroll
             for (int x = 0; x < kPer; ++x) {
                 uint32_t o = off[x];
-                if (!whole) {  // rows past the last key repeat it
+                if (!whole) {  // rows past the last key: of K they repeat it, of V they are zeroes
                     const int r = T::RPB * x + lrow, most = max(len - 1 - (kb0 + 16 * s), 0);
+                    if constexpr (kIsV) {
+                        const char* const from = kb0 + 16 * s + r < len ? at + o : reinterpret_cast<const char*>(&kPagedZeroes);
+                        if (ok[x]) dma_kib_lanes<true>(from, dst + (s * kPer + x) * 1024);
+                        continue;
+                    }
                     if (r > most) o -= (uint32_t)(r - most) * row_bytes;
                 }
                 if (ok[x]) dma_kib_nt(at, o, dst + (s * kPer + x) * 1024);
             }
         }
     };
-    auto request_k = [&](int t) { request(t, Kh, a.k_page, a.k_row, koff, kok, kst); };
-    auto request_v = [&](int t) { request(t, Vh, a.v_page, a.v_row, voff, vok, vst); };
+    auto request_k = [&](int t) { request(std::false_type{}, t, Kh, a.k_page, a.k_row, koff, kok, kst); };
+    auto request_v = [&](int t) { request(std::true_type{}, t, Vh, a.v_page, a.v_row, voff, vok, vst); };
 
     const int r = it.row0 + l32;
     v8h qf[KS];
@@ -846,13 +866,6 @@ struct PagedRequests {
     }
 };
 
-// One KiB into LDS from an address of each lane's own (dma_kib in common.h).
-__device__ __forceinline__ void dma_kib_lanes(const char* at, FA_LDS char* lds_dst)
-{
-    const uint32_t m0v = (uint32_t)(uintptr_t)lds_dst;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0v), "v"(at) : "memory", "m0");
-}
-
 // LDS-only barrier: requests in flight are not waited for, and nothing moves across.
 __device__ __forceinline__ void paged_barrier()
 {
@@ -929,6 +942,24 @@ struct TallCfg {
     static constexpr int QBUF = 32 * PagedTile<D>::ROW, SMEM = NST * 2 * PagedTile<D>::BUF + 2 * QBUF;
     static_assert(2 * QBUF == PagedTile<D>::BUF, "Q rows of two waves per stage");
 };
+
+// Rows of a tile of V from `left` on lie past the sequence's end and repeat the last key's.  Their probabilities are 0, but 0 times a value that is not
+// finite is not, and the wave's rows may see the last key: if it has such a value these rows become 0.  Each wave does so in front of its own reads, all
+// write the same.  (Requests that take the rows from a row of zeroes, as in the 32-row form, make the loop longer: 640 rows on 28339 keys B4 H5 H_kv1 d80
+// 113.1 -> 118.2 us; so 113.5.)
+template <int D, bool kBf16>
+__device__ __forceinline__ void paged_clear_past(FA_LDS char* stage, int left, int lane)
+{
+    using T = PagedTile<D>;
+    const v4u row = *reinterpret_cast<FA_LDS const v4u*>(stage + left * T::ROW + (lane % T::CPR) * 16);
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd |= Elem<kBf16>::not_finite(row[e]);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) == 0, 1)) return;
+    const v4u z = {0u, 0u, 0u, 0u};
+    for (int at = left * T::ROW + lane * 16; at < T::BUF; at += 1024) *reinterpret_cast<FA_LDS v4u*>(stage + at) = z;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
 
 // Waves 0-3 and 4-7 run half an iteration apart (the second group passes one more barrier in front of the loop): while one wave of a
 // SIMD is at its softmax, the other is at its MFMAs.  A tile of 256 rows x 64 keys at d = 128 takes a CU 1.97 us, as in fwd_pp_kernel, 90 % of
@@ -1100,7 +1131,7 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
         const int rl = T::RPB * x + lane / T::CPR, c = T::k_chunk(lane % T::CPR, rl), row = first_row + rl;
         int head;
         const int tok = row_token(a, it, row < it.rows ? row : it.rows - 1, &head);
-        if (c * 8 < a.d) dma_kib_lanes(a.Q + (size_t)tok * a.q_token + (size_t)head * a.q_head + c * 16, qst + x * 1024);
+        if (c * 8 < a.d) dma_kib_lanes<false>(a.Q + (size_t)tok * a.q_token + (size_t)head * a.q_head + c * 16, qst + x * 1024);
     }
 #pragma unroll
     for (int t = 0; t < 3; ++t) {
@@ -1164,6 +1195,7 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
     for (; t < t_hi - 1; ++t)
         iteration(std::false_type{}, Vs + (t % NST) * T::BUF, Ks + ((t + 1) % NST) * T::BUF, Ks + ((t + 3) % NST) * T::BUF, Vs + ((t + 2) % NST) * T::BUF, t);
     if (t < t_hi) {
+        if (const int left = it.len - (tile0 + t) * BC; left < BC) paged_clear_past<D, kBf16>(Vs + (t % NST) * T::BUF, left, lane);
         iteration(std::true_type{}, Vs + (t % NST) * T::BUF, Ks + ((t + 1) % NST) * T::BUF, Ks + ((t + 3) % NST) * T::BUF, Vs + ((t + 2) % NST) * T::BUF, t);
         ++t;
     }
