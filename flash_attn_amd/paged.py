@@ -154,6 +154,14 @@ class _on:
         return self._device.__exit__(*exc)
 
 
+def _no_gradients(where, *tensors):
+    """Refuses tensors whose gradients nobody works out: the result would be detached from them without a word."""
+    import torch
+
+    _check(not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors),
+           f"{where} has no gradients: detach what requires one, or call it under torch.no_grad()")
+
+
 def _raise(rc, where):
     if rc != FLASH_OK:
         raise FlashError(rc, where)
@@ -338,7 +346,8 @@ def flash_append_paged(k, v, k_cache, v_cache, block_table, seqlens_k, cu_seqlen
     """Writes the new rows k, v [tokens,H_kv,d] into the sequences' pages, the last ones of seqlens_k keys each.
 
     With inv_freq K is turned on its way in as by flash_rotary, by its place in the sequence or by positions [tokens] where they are given, and
-    so is q [tokens,H,d], if it is given: returned, in `out` if that is given (q itself for in place).  Returns None without q."""
+    so is q [tokens,H,d], if it is given: returned, in `out` if that is given (q itself for in place).  Returns None without q.  For serving: tensors
+    that require a gradient are refused while gradients are recorded."""
     if stream is None:
         res = (_native or _front_end()).append(k, v, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, q, inv_freq, interleaved, factor, positions, out)
         if res is not NotImplemented:
@@ -346,6 +355,7 @@ def flash_append_paged(k, v, k_cache, v_cache, block_table, seqlens_k, cu_seqlen
     # arguments that the native front end leaves alone (those that raise among them)
     import torch
 
+    _no_gradients("flash_append_paged", k, v, k_cache, v_cache, q, inv_freq, out)
     _check(q is None or inv_freq is not None, "q is turned with inv_freq: without it there is nothing to do for q")
     _check(out is None or q is not None, "out is for q")
     _check(positions is None or inv_freq is not None, "positions are for inv_freq")
@@ -384,7 +394,8 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
     missing or meaningless; max_seqlen_k: the longest sequence, which decides into how many splits its keys are cut (0: what the table can name).
     num_splits <= 0: the library's choice.
     workspace: (O_partial, LSE_partial) of at least the bytes that paged_workspace_bytes says, otherwise allocated here.
-    Rows that belong to no sequence are left as they are (new memory where out and lse are not given)."""
+    Rows that belong to no sequence are left as they are (new memory where out and lse are not given).  For serving: tensors that require a gradient
+    are refused while gradients are recorded."""
     if stream is None:
         res = (_native or _front_end()).paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
                                               window, num_splits, workspace, out, lse)
@@ -393,6 +404,7 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
     # arguments that the native front end leaves alone (those that raise among them)
     import torch
 
+    _no_gradients("flash_forward_paged", q, k_cache, v_cache, out, lse)
     _check(q.dim() == 3 and k_cache.dim() == 4, "q must be [tokens,H,d], caches [pages,H_kv,page_size,d]")
     T, H, d = q.shape
     Hk = k_cache.shape[1]
