@@ -11,7 +11,7 @@
 // Anything out of the ordinary -- an argument of another type, shapes or dtypes that do not fit, a workspace that is too
 // small, a program that wants to see its allocations -- returns NotImplemented with nothing allocated or launched; binding.py then takes its own path, which raises the
 // errors (and serves the debug outputs).  Of the calls of paged.py it also leaves those on another stream or device than the current one
-// and those that need a gradient; the others took 15 us (rotary) to 29 us (paged forward in splits) each through ctypes.
+// and those that need a derivative; the others took 15 us (rotary) to 29 us (paged forward in splits) each through ctypes.
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
@@ -305,12 +305,13 @@ bool fits_int(const at::Tensor& t)
 // on the GPU that is current, whose current stream the call goes to
 bool is_here(const at::Tensor& t) { return t.is_cuda() && t.device().index() == c10::hip::current_device(); }
 at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef size, at::ScalarType type) { return at::detail::empty_cuda(size, type, like.device(), std::nullopt); }
-// whether results would be detached from one of them without a word (paged.py refuses it, or works out the gradient)
-bool wants_gradient(std::initializer_list<const at::Tensor*> tensors)
+// whether results would be detached from one of them without a word, of its gradient or of a forward-mode derivative (paged.py refuses it, or works
+// out the gradient)
+bool wants_derivative(std::initializer_list<const at::Tensor*> tensors)
 {
-    if (!at::GradMode::is_enabled()) return false;
+    const bool grad = at::GradMode::is_enabled();
     for (const at::Tensor* t : tensors)
-        if (t && t->requires_grad()) return true;
+        if (t && ((grad && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
     return false;
 }
 bool positions_ok(const at::Tensor& t) { return (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && unit_stride(t) && is_here(t); }
@@ -331,7 +332,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n)
         p.interleaved = args[3] == Py_True, p.inverse = args[5] == Py_True;
         const int64_t dims = x->dim();
         if ((dims != 3 && dims != 4) || (p.dtype = dtype_of(*x)) < 0 || !unit_stride(*x) || !fits_int(*x) || !is_here(*x)) return not_implemented();
-        if (wants_gradient({x, f, out})) return not_implemented();
+        if (wants_derivative({x, f, out})) return not_implemented();
         const bool tokens = dims == 3;
         p.B = tokens ? 1 : (int)x->size(0), p.H = (int)x->size(1), p.N = (int)x->size(tokens ? 0 : 2), p.d = (int)x->size(-1);
         if (!positions_ok(*pos) || !frequencies_ok(*f, p.d)) return not_implemented();
@@ -396,7 +397,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n)
         if (!k || !v || !parse_cache(args + 2, p) || !optional_tensor(args[7], &q) || !optional_tensor(args[8], &f) || !optional_tensor(args[11], &pos) ||
             !optional_tensor(args[12], &out) || !PyBool_Check(args[9]) || !real(args[10], &p.factor))
             return not_implemented();
-        if (wants_gradient({k, v, tensor_of(args[2]), tensor_of(args[3]), q, f, out})) return not_implemented();
+        if (wants_derivative({k, v, tensor_of(args[2]), tensor_of(args[3]), q, f, out})) return not_implemented();
         if ((q && !f) || (out && !q) || (pos && !f) || k->dim() != 3 || (q && q->dim() != 3) || k->size(0) > INT32_MAX) return not_implemented();
         const int64_t T = k->size(0), H = q ? q->size(1) : p.H_kv;
         if (H > INT32_MAX || !rows_ok(*k, T, p.H_kv, p) || !rows_ok(*v, T, p.H_kv, p) || (q && !rows_ok(*q, T, H, p)) || (out && !rows_ok(*out, T, H, p))) return not_implemented();
@@ -426,7 +427,7 @@ PyObject* paged(PyObject*, PyObject* const* args, Py_ssize_t n)
         const at::Tensor *q = tensor_of(args[0]), *out, *lse;
         flash_paged_params p{};
         if (!q || !parse_cache(args + 1, p) || !optional_tensor(args[13], &out) || !optional_tensor(args[14], &lse)) return not_implemented();
-        if (wants_gradient({q, tensor_of(args[1]), tensor_of(args[2]), out, lse})) return not_implemented();
+        if (wants_derivative({q, tensor_of(args[1]), tensor_of(args[2]), out, lse})) return not_implemented();
         if (!small_int(args[6], &p.max_seqlen_q) || !small_int(args[7], &p.max_seqlen_k) || !PyBool_Check(args[9]) || !small_int(args[11], &p.num_splits)) return not_implemented();
         if (args[8] == Py_None) p.softmax_scale = (float)std::pow((double)p.d, -0.5);
         else if (!real(args[8], &p.softmax_scale)) return not_implemented();

@@ -158,8 +158,16 @@ def _no_gradients(where, *tensors):
     """Refuses tensors whose gradients nobody works out: the result would be detached from them without a word."""
     import torch
 
+    _no_tangents(where, *tensors)
     _check(not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors),
            f"{where} has no gradients: detach what requires one, or call it under torch.no_grad()")
+
+
+def _no_tangents(where, *tensors):
+    """Refuses tensors with a forward-mode derivative, which nobody works out."""
+    from torch.autograd import forward_ad
+
+    _check(all(t is None or forward_ad.unpack_dual(t).tangent is None for t in tensors), f"{where} has no forward-mode derivatives")
 
 
 def _raise(rc, where):
@@ -296,6 +304,7 @@ def flash_rotary(x, positions, inv_freq, interleaved=False, factor=1.0, inverse=
     # arguments that the native front end leaves alone (those that raise among them)
     import torch
 
+    _no_tangents("flash_rotary", x, inv_freq, out)
     if torch.is_grad_enabled() and x.requires_grad:
         _check(out is None, "out cannot be given for an x that requires a gradient")
         _check(not inv_freq.requires_grad, "inv_freq gets no gradient: detach it")

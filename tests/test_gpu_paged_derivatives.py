@@ -33,3 +33,19 @@ def test_tensors_that_require_a_gradient(fa, own_stream):
                 got = f(**args, stream=stream)
             for a, b in zip(got, want):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_forward_mode(fa, own_stream):
+    from torch.autograd import forward_ad
+
+    stream = torch.cuda.current_stream() if own_stream else None
+    step = setup(fa)
+    rotary = dict(x=step[0]["q"], positions=torch.arange(3, device="cuda"), inv_freq=step[0]["inv_freq"])
+    with forward_ad.dual_level(), torch.no_grad():
+        for f, args in ((fa.flash_append_paged, step[0]), (fa.flash_forward_paged, step[1]), (fa.flash_rotary, rotary)):
+            for name, t in args.items():
+                if t.is_floating_point():
+                    with pytest.raises(ValueError, match="has no forward-mode derivatives"):
+                        f(**dict(args, **{name: forward_ad.make_dual(t, torch.ones_like(t))}), stream=stream)
+            f(**args, stream=stream)

@@ -33,3 +33,24 @@ def test_tensors_that_require_a_gradient(fa, name):
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="must be on the GPU"):  # (gets past that)
             call()
+
+
+@pytest.mark.parametrize("name", [x for x, t in tensors().items() if t.is_floating_point()])
+def test_forward_mode(fa, name):
+    from torch.autograd import forward_ad
+
+    def give_tangent(t):
+        t[name] = forward_ad.make_dual(t[name], torch.ones_like(t[name]))
+        return t
+
+    with forward_ad.dual_level():
+        for names, f in ((APPEND, fa.flash_append_paged), (FORWARD, fa.flash_forward_paged)):
+            if name in names:
+                t = give_tangent(tensors())
+                with pytest.raises(ValueError, match="has no forward-mode derivatives"):
+                    f(**{x: t[x] for x in names})
+        if name in ("q", "inv_freq", "out"):  # (rotary's x, inv_freq and out)
+            t = give_tangent(tensors())
+            for x in (t["q"], t["q"].detach().requires_grad_()) if name != "q" else (t["q"],):
+                with pytest.raises(ValueError, match="has no forward-mode derivatives"):
+                    fa.flash_rotary(x, torch.arange(3), t["inv_freq"], out=t["out"])
