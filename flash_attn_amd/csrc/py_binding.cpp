@@ -314,6 +314,12 @@ bool wants_derivative(std::initializer_list<const at::Tensor*> tensors)
         if (t && ((grad && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
     return false;
 }
+// Tells autograd that the caller's tensors have been written, so that a backward pass that has saved one of them notices.
+void written(std::initializer_list<const at::Tensor*> tensors)
+{
+    for (const at::Tensor* t : tensors)
+        if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 bool positions_ok(const at::Tensor& t) { return (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && unit_stride(t) && is_here(t); }
 bool frequencies_ok(const at::Tensor& f, int64_t d)
 {
@@ -353,7 +359,9 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n)
         p.inv_freq = static_cast<const float*>(f->data_ptr());
         void* const stream = c10::hip::getCurrentHIPStream().stream();
         const int rc = g_rotary(&p, stream);
-        return rc != FLASH_OK ? raise(rc, "flash_rotary") : THPVariable_Wrap(y);
+        if (rc != FLASH_OK) return raise(rc, "flash_rotary");
+        written({out});
+        return THPVariable_Wrap(y);
     });
 }
 
@@ -414,6 +422,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n)
         }
         const int rc = g_append(&p, c10::hip::getCurrentHIPStream().stream());
         if (rc != FLASH_OK) return raise(rc, "flash_append_paged");
+        written({tensor_of(args[2]), tensor_of(args[3]), out});
         if (q) return THPVariable_Wrap(y);
         Py_RETURN_NONE;
     });
@@ -445,9 +454,10 @@ PyObject* paged(PyObject*, PyObject* const* args, Py_ssize_t n)
         if (S < 0) return raise(S, "flash_forward_paged_resolve_splits");
         const int64_t rows = S > 1 ? T * H * S : 0;
         at::Tensor own;  // workspace of this call, both parts in one allocation
+        const at::Tensor *wo = nullptr, *wl = nullptr;
         if (args[12] != Py_None) {
             if (!PyTuple_CheckExact(args[12]) || PyTuple_GET_SIZE(args[12]) != 2) return not_implemented();
-            const at::Tensor *wo = tensor_of(PyTuple_GET_ITEM(args[12], 0)), *wl = tensor_of(PyTuple_GET_ITEM(args[12], 1));
+            wo = tensor_of(PyTuple_GET_ITEM(args[12], 0)), wl = tensor_of(PyTuple_GET_ITEM(args[12], 1));
             for (const at::Tensor* t : {wo, wl})
                 if (!t || t->scalar_type() != at::kFloat || !is_here(*t) || !t->is_contiguous()) return not_implemented();
             if (wo->numel() < rows * d || wl->numel() < rows) return not_implemented();
@@ -463,6 +473,7 @@ PyObject* paged(PyObject*, PyObject* const* args, Py_ssize_t n)
         p.q_token = q->stride(0), p.q_head = q->stride(1), p.o_token = o.stride(0), p.o_head = o.stride(1);
         const int rc = g_paged(&p, c10::hip::getCurrentHIPStream().stream());
         if (rc != FLASH_OK) return raise(rc, "flash_forward_paged");
+        written({out, lse, wo, wl});
         PyObject* res = PyTuple_New(2);
         if (!res) return nullptr;
         PyTuple_SET_ITEM(res, 0, THPVariable_Wrap(o));

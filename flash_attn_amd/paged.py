@@ -175,6 +175,15 @@ def _raise(rc, where):
         raise FlashError(rc, where)
 
 
+def _written(*tensors):
+    """Tells autograd that the caller's tensors have been written, so that a backward pass that has saved one of them notices."""
+    import torch
+
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 # ---------------------------------------------------------------------------------------------------- rotary positions
 
 
@@ -263,6 +272,7 @@ def _rotary(x, positions, inv_freq, interleaved, factor, inverse, out, stream):
         p.inv_freq, p.factor = inv_freq.data_ptr(), float(factor)
         p.interleaved, p.inverse = int(bool(interleaved)), int(bool(inverse))
         _raise(L.flash_rotary(C.byref(p), handle), "flash_rotary")
+    _written(out)
     return y
 
 
@@ -383,6 +393,7 @@ def flash_append_paged(k, v, k_cache, v_cache, block_table, seqlens_k, cu_seqlen
         _check(positions.dim() == 1 and positions.shape[0] == T and _positions_ok(positions), "positions must be int32 or int64 [tokens]")
         p.positions, p.positions_64 = positions.data_ptr(), int(positions.dtype == torch.int64)
     device = _same_device(k, v, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, q, inv_freq, positions, out)
+    given = out
     with _on(device, stream) as handle:
         if q is not None:
             p.q_token, p.q_head = _rows(q, "q", p.H, d, k_cache.dtype, T)
@@ -391,6 +402,7 @@ def flash_append_paged(k, v, k_cache, v_cache, block_table, seqlens_k, cu_seqlen
             p.o_token, p.o_head = _rows(out, "out", p.H, d, k_cache.dtype, T)
             p.Q, p.O = q.data_ptr(), out.data_ptr()
         _raise(_lib().flash_append_paged(C.byref(p), handle), "flash_append_paged")
+    _written(k_cache, v_cache, given)
     return out
 
 
@@ -448,6 +460,7 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
                    f"workspace too small for {S} splits: need {rows * d} and {rows} fp32 elements")
             p.O_partial, p.LSE_partial = workspace[0].data_ptr(), workspace[1].data_ptr()
         _raise(L.flash_forward_paged(C.byref(p), handle), "flash_forward_paged")
+    _written(out, lse, *given)
     return o, l
 
 

@@ -49,3 +49,33 @@ def test_forward_mode(fa, own_stream):
                     with pytest.raises(ValueError, match="has no forward-mode derivatives"):
                         f(**dict(args, **{name: forward_ad.make_dual(t, torch.ones_like(t))}), stream=stream)
             f(**args, stream=stream)
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_tensors_that_are_written(fa, own_stream):
+    """A backward pass that has saved a tensor which a call then writes must not go on with what it finds there; what a call reads alone stays as it was,
+    and tensors of inference mode, which count nothing, are written too."""
+    stream = torch.cuda.current_stream() if own_stream else None
+    append, forward = setup(fa)
+    rotary = dict(x=append["q"], positions=torch.arange(3, device="cuda"), inv_freq=append["inv_freq"], out=append["out"])
+    forward.update(num_splits=2, workspace=(torch.empty(100000, device="cuda"), torch.empty(1000, device="cuda")))
+    in_place = dict(rotary, x=rotary["out"])
+    for f, args, writes in ((fa.flash_rotary, rotary, ("out",)), (fa.flash_rotary, in_place, ("x",)), (fa.flash_append_paged, append, ("k_cache", "v_cache", "out")),
+                            (fa.flash_forward_paged, forward, ("out", "lse"))):
+        given = {n: t for n, t in args.items() if isinstance(t, torch.Tensor)}
+        for name in writes:
+            w = torch.ones((), device="cuda", dtype=given[name].dtype, requires_grad=True)
+            loss = (w * given[name]).sum()
+            f(**args, stream=stream)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward()
+        before = {n: t._version for n, t in given.items()}
+        f(**args, stream=stream)
+        written = {n for n, t in given.items() if t._version != before[n]}
+        assert written - {"x", "out"} == set(writes) - {"x", "out"} and set(writes) <= written, f
+    assert all(t._version > 0 for t in forward["workspace"])
+    with torch.inference_mode():
+        append, forward = setup(fa)
+        fa.flash_append_paged(**append, stream=stream)
+        fa.flash_forward_paged(**forward, stream=stream)
+        fa.flash_rotary(append["q"], rotary["positions"], rotary["inv_freq"], out=append["q"], stream=stream)
