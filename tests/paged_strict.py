@@ -59,7 +59,7 @@ def attention(q, k_cache, v_cache, table, lens, cu, scale=None, causal=False, wi
             p = torch.where(weighs, torch.exp(s - torch.where(top == -math.inf, 0.0, top)), 0.0)
             total = p.sum(1, keepdim=True)
             w = p / torch.where(total > 0, total, torch.where(torch.isnan(total), total, 1.0))
-            fine = torch.where(torch.isfinite(v), v, 0.0)
+            fine = torch.where(torch.isfinite(v) & weighs.any(0)[:, None], v, 0.0)
             o = w @ fine
             big = torch.where(weighs, size, 0.0).amax(1)
             # what is not finite among the values that the row gives a weight

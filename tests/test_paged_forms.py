@@ -2,6 +2,7 @@
 from paged_launches import call, record
 
 import test_gpu_paged_last_key as last_key
+import test_gpu_paged_odd_scores as odd_scores
 import test_gpu_paged_tall as tall
 
 
@@ -45,3 +46,10 @@ def test_ordered_tests_reach_ordered_launches():
     c = tall.CAPTURED
     x, = record([call(c["news"], c["lens"], c["Hk"] * c["G"], c["Hk"], c["d"], max_seqlen_q=600, max_seqlen_k=700, num_splits=3, causal=True)])
     assert x["form"] == "tall" and x["pieces"]
+
+
+def test_odd_scores_reach_both_forms():
+    for shapes, form in ((odd_scores.FEW, "few"), (odd_scores.TALL, "tall")):
+        calls = [call(*shape, d, max_seqlen_q=max(shape[0]), num_splits=splits, **mask) for shape in shapes for d in (40, 64, 128) for splits in (1, 2)
+                 for mask in (dict(), dict(causal=True), dict(causal=True, window=(30, -1)), dict(window=(60, 2)))]
+        assert {x["form"] for x in record(calls)} == {form}
