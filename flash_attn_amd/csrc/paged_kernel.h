@@ -963,7 +963,7 @@ __device__ __forceinline__ void paged_clear_past(FA_LDS char* stage, int left, i
 
 // Waves 0-3 and 4-7 run half an iteration apart (the second group passes one more barrier in front of the loop): while one wave of a
 // SIMD is at its softmax, the other is at its MFMAs.  A tile of 256 rows x 64 keys at d = 128 takes a CU 1.97 us, as in fwd_pp_kernel, 90 % of
-// what that mix of MFMAs and softmax reaches without any waits; ragged prompts up to 4096 H32 H_kv4 fp16 372 us, 0.92 PFLOP/s.  V(t + 2) is
+// what that mix of MFMAs and softmax reaches without any waits; ragged prompts up to 4096 H32 H_kv4 fp16 362-372 us, 0.92-0.95 PFLOP/s.  V(t + 2) is
 // requested at the start of iteration t and waited for at its end, K(t + 3) at its end and waited for at the next one's; their slots were last
 // read two barriers before.
 // DU: columns that are worked on, a multiple of 16 from d on, the scores in steps of 16, O in blocks of 32 (rows in LDS have D): with DU = D the

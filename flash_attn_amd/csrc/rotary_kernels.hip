@@ -11,7 +11,7 @@
 // and cosines, a pair each, into LDS of the wave's own, and then walk the rows (heads) of the token in pieces of a pair of 16-byte chunks, whose
 // angles they read back from there.  So an angle costs its 64-bit products and its sine once per token, not once per head.  Tokens of
 // short launches are shared out among `parts` waves.  Measured on one MI355X: rotary B4 H32 N4096 d128 bf16 43-52 us (5.2-6.2 TB/s read and
-// written, a copy of that size 4.7-4.9), append of 16384 tokens H32 H_kv8 d128 with Q 79 us (5.1 TB/s), one token H32 2.2 us and 64 of them into
+// written, a copy of that size 4.7-4.9), fp32 101 us (a copy 100), append of 16384 tokens H32 H_kv8 d128 with Q 79 us (5.1 TB/s), one token H32 2.2 us and 64 of them into
 // their pages 4 us of GPU time (a launch).  (The rows' first pieces requested in front of the angles: d80 6.3 -> 6.1 us, but N4096 43.1 -> 47.4.)
 #include "rotary_kernels.h"
 

@@ -262,13 +262,14 @@ typedef struct flash_paged_params {
     int positions_64;
 } flash_paged_params;
 
-/* New rows of K, turned as by flash_rotary, and of V into their pages; Q, if it is given, turned into O by the same launch.  Two tokens whose
+/* New rows of K, turned as by flash_rotary, and of V into their pages; Q, if it is given, turned into O by the same launch.  Rows whose place
+ * is in front of key 0 or one that the table cannot name are not written.  Two tokens whose
  * rows are the same row of the cache (sequences that share a page that is still written) leave one of the two there. */
 int flash_append_paged(const flash_paged_params *p, void *stream);
 
 /* O = softmax(mask(Q K^T * scale)) V of every sequence's new tokens over its pages, down to one token per sequence, and LSE.  Rows that
  * see no key get O = 0 and LSE = -inf.  A value that is not finite in a row of V that a query does not see, or behind a
- * sequence's end, does not reach that query's O. */
+ * sequence's end, does not reach that query's O; one that it sees does (an infinity as NaN where its probability rounds to 0 in the caches' type). */
 int flash_forward_paged(const flash_paged_params *p, void *stream);
 
 /* The split count that flash_forward_paged uses for p, and the bytes of its workspace (0 for one split).  They depend on the sizes (B, H, H_kv, d,
