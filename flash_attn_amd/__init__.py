@@ -25,11 +25,17 @@ from .binding import (  # noqa: F401
     lib,
 )
 from .paged import (  # noqa: F401
+    FLASH_MAX_SOFTCAP,
+    FLASH_MAX_TREE_TOKENS,
+    KeepParams,
     PagedParams,
     RotaryParams,
+    TreeParams,
     flash_append_paged,
     flash_forward_paged,
+    flash_keep_paged,
     flash_rotary,
+    flash_tree_mask,
     paged_resolve_splits,
     paged_workspace_bytes,
     rotary_frequencies,

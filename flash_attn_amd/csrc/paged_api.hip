@@ -1,10 +1,11 @@
-// C entry points of rotary positions and of the paged cache (include/flash_attn_mi355.h): argument checks, split count, launches.
+// C entry points of rotary positions, of the paged cache and of drafted tokens (include/flash_attn_mi355.h): argument checks, split count, launches.
 #include "flash_attn_mi355.h"
 
 #include <cmath>
 #include <cstring>
 
 #include "api_common.h"
+#include "draft_kernels.h"
 #include "paged_kernel.h"
 #include "rotary_kernels.h"
 
@@ -85,6 +86,20 @@ int validate_paged(const flash_paged_params* p, bool* empty)
     return FLASH_OK;
 }
 
+// what the forward has beside them: scores and masks of other kinds
+int validate_scores(const flash_paged_params* p)
+{
+    if (!(p->softcap >= 0.0f) || p->softcap > FLASH_MAX_SOFTCAP) return FLASH_EINVAL;
+    if (misaligned(p->alibi_slopes, 4) || misaligned(p->prefix_lens, 4) || misaligned(p->tree_mask, 8)) return FLASH_EALIGN;
+    if (!p->tree_mask) return FLASH_OK;
+    // (the mask says what the chunk's tokens see of each other)
+    if (p->tree_words < 1 || p->tree_words > FLASH_MAX_TREE_TOKENS / 64 || p->tree_stride < 0 || p->prefix_lens || p->window_right >= 0) return FLASH_EINVAL;
+    const int chunk = p->max_seqlen_q > 0 && p->max_seqlen_q < p->total_q ? p->max_seqlen_q : p->total_q;
+    if (chunk > 64 * p->tree_words) return FLASH_EINVAL;
+    // (... all that are on a path, which the window does not cut)
+    return p->window_left >= 0 && p->window_left < chunk - 1 ? FLASH_EINVAL : FLASH_OK;
+}
+
 // the cache's strides, bases and index tensors; `launch` alone has pointers
 int validate_cache(const flash_paged_params* p)
 {
@@ -125,6 +140,7 @@ long long blocks_of(const flash_paged_params* p, int br)
 }
 
 // bounds that can never cut are none: the kernels' position + right stays in an int
+bool causal_of(const flash_paged_params* p) { return p->is_causal != 0 && !p->tree_mask; }
 int window_left_of(const flash_paged_params* p) { return p->window_left >= capacity_of(p) ? -1 : p->window_left; }
 // (the last row stands at the last key, and no row more than a chunk in front of it)
 int window_right_of(const flash_paged_params* p) { return p->window_right >= p->total_q ? -1 : p->window_right; }
@@ -139,9 +155,9 @@ int keys_of(const flash_paged_params* p)
 // tiles of 64 keys that the masks leave a block of br rows, at most
 int window_tiles(const flash_paged_params* p, int br)
 {
-    const int wl = window_left_of(p), wr = window_right_of(p);
-    if (wl < 0 || (!p->is_causal && wr < 0)) return 0x7fffffff;
-    return (int)(((long long)wl + 1 + (p->is_causal ? 0 : wr) + (br + group_of(p) - 1) / group_of(p) + 63 + 63) / 64);
+    const int wl = window_left_of(p), wr = p->tree_mask ? longest_chunk(p) : window_right_of(p);
+    if (wl < 0 || (!causal_of(p) && wr < 0) || p->prefix_lens) return 0x7fffffff;
+    return (int)(((long long)wl + 1 + (causal_of(p) ? 0 : wr) + (br + group_of(p) - 1) / group_of(p) + 63 + 63) / 64);
 }
 // ... and that it sees
 int most_tiles(const flash_paged_params* p, int br)
@@ -166,7 +182,7 @@ int rows_per_group(const flash_paged_params* p)
     if (chunk * group_of(p) <= kShortRows) return fa::kPagedFewRows;
     long long tiles = most_tiles(p, fa::kPagedFewRows);
     const long long keys = keys_of(p);
-    if (p->is_causal && tiles > (keys - chunk / 2) / 64 + 1) tiles = (keys > chunk / 2 ? keys - chunk / 2 : 0) / 64 + 1;  // (the mean row's)
+    if (causal_of(p) && tiles > (keys - chunk / 2) / 64 + 1) tiles = (keys > chunk / 2 ? keys - chunk / 2 : 0) / 64 + 1;  // (the mean row's)
     return groups <= kShortGroups && groups * tiles <= (p->d <= 64 ? kShortUnits64 : kShortUnits) ? fa::kPagedFewRows : fa::kPagedTallRows;
 }
 
@@ -175,7 +191,7 @@ int rows_per_group(const flash_paged_params* p)
 // there, stay in the order that leaves row blocks of the same keys to the same XCD.)
 bool real_pieces(const flash_paged_params* p, int br, int splits)
 {
-    if (splits < 2 || (long long)p->B * splits > 64 || window_left_of(p) >= 0 || (!p->is_causal && window_right_of(p) < 0)) return false;
+    if (splits < 2 || (long long)p->B * splits > 64 || window_left_of(p) >= 0 || (!causal_of(p) && window_right_of(p) < 0)) return false;
     return br == fa::kPagedTallRows || ((long long)longest_chunk(p) * group_of(p) > br && keys_of(p) / 2 <= longest_chunk(p));
 }
 
@@ -192,7 +208,7 @@ int splits_by_estimate(const flash_paged_params* p, int br, int nt)
 {
     // row blocks of a chunk of mean length behind the longest sequence's keys
     const bool tall = br == fa::kPagedTallRows, narrow = p->d <= 64;
-    const int G = group_of(p), keys = keys_of(p), reach = p->is_causal ? 0 : window_right_of(p);
+    const int G = group_of(p), keys = keys_of(p), reach = causal_of(p) ? 0 : window_right_of(p);
     const int mean = (p->total_q + p->B - 1) / p->B, chunk = mean < longest_chunk(p) ? mean : longest_chunk(p);
     const long long n = ((long long)chunk * G + br - 1) / br, parts = (long long)p->B * p->H_kv;
     const double begin_us = tall ? 7.0 : 4.5, merge_us = tall ? 8.0 : 3.0, tile_us = tall ? (narrow ? 0.95 : p->d <= 96 ? 1.35 : 1.53) : narrow ? 0.365 : 0.6;
@@ -278,12 +294,30 @@ bool ordered(const flash_paged_params* p, int br)
     return groups > kNumCU && groups <= (keys_of(p) > kShortKeys ? kOrderedGroups : kOrderedShort);
 }
 
+// a has what every launch has
+int launch_scored(const flash_paged_params* p, fa::ScoredArgs& a, int br, long long blocks, hipStream_t st)
+{
+    const bool bf16 = p->dtype == FLASH_BF16;
+    a.slopes = p->alibi_slopes, a.prefix = p->prefix_lens;
+    a.tree = reinterpret_cast<const uint64_t*>(p->tree_mask), a.tree_stride = p->tree_stride, a.tree_words = p->tree_words;
+    if (p->softcap > 0.0f) {
+        a.cap = p->softcap;
+        a.cap_in = (float)(2.0 * (double)fa::kLog2e * p->softmax_scale / p->softcap);
+        a.scale_log2 = 2.0f * p->softcap * fa::kLog2e;
+        a.slope_unit = 0.5f / p->softcap;
+        return a.slopes ? fa::launch_scored_both(a, bf16, br, blocks, st) : fa::launch_scored_capped(a, bf16, br, blocks, st);
+    }
+    a.slope_unit = 1.0f / p->softmax_scale;
+    return a.slopes ? fa::launch_scored_sloped(a, bf16, br, blocks, st) : fa::launch_scored_masked(a, bf16, br, blocks, st);
+}
+
 int run_forward(const flash_paged_params* p, hipStream_t st)
 {
     bool empty;
     int rc = validate_paged(p, &empty);
     if (rc != FLASH_OK) return rc;
     if (!(p->softmax_scale > 0.0f) || std::isinf(p->softmax_scale)) return FLASH_EINVAL;
+    if ((rc = validate_scores(p)) != FLASH_OK) return rc;
     if (empty) return FLASH_OK;
     if ((rc = validate_cache(p)) != FLASH_OK) return rc;
     if ((rc = rows_strides(p->q_token, p->q_head, p->Q)) != FLASH_OK || (rc = rows_strides(p->o_token, p->o_head, p->O)) != FLASH_OK) return rc;
@@ -297,7 +331,7 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     const long long blocks = blocks_of(p, br) * p->H_kv * splits;
     if (blocks * fa::paged_threads(br) >= 1LL << 32) return FLASH_EINVAL;
     if ((rc = device_usable()) != FLASH_OK) return rc;
-    fa::PagedArgs a{};
+    fa::ScoredArgs a{};
     a.Q = static_cast<const char*>(p->Q), a.K = static_cast<const char*>(p->K_cache), a.V = static_cast<const char*>(p->V_cache);
     a.O = static_cast<char*>(p->O), a.LSE = p->LSE, a.O_partial = p->O_partial, a.LSE_partial = p->LSE_partial;
     a.table = p->block_table, a.lens = p->seqlens_k, a.cu = p->cu_seqlens_q;
@@ -307,7 +341,7 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     a.table_stride = p->block_table_stride;
     a.B = p->B, a.H = p->H, a.Hk = p->H_kv, a.G = group_of(p), a.d = p->d, a.tokens = p->total_q, a.num_pages = p->num_pages, a.page = p->page_size;
     a.capacity = capacity_of(p);
-    a.causal = p->is_causal != 0, a.wl = window_left_of(p), a.wr = window_right_of(p);
+    a.causal = causal_of(p), a.wl = window_left_of(p), a.wr = window_right_of(p);
     a.scale_log2 = p->softmax_scale * fa::kLog2e;
     a.num_splits = splits, a.tiles_per_split = (nt + splits - 1) / splits, a.window_tiles = window_tiles(p, br);
     a.direct = (long long)longest_chunk(p) * a.G <= br;
@@ -316,7 +350,8 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     a.by_heads = fa::fast_div(a.Hk), a.by_group = fa::fast_div(a.G), a.by_page = fa::fast_div(a.page);
     a.by_splits = fa::fast_div(splits);
     const bool bf16 = p->dtype == FLASH_BF16;
-    rc = record_hip(p->d <= 64 ? fa::launch_paged_d64(a, bf16, br, blocks, st) : fa::launch_paged_d128(a, bf16, br, blocks, st));
+    if (p->softcap > 0.0f || p->alibi_slopes || p->prefix_lens || p->tree_mask) rc = record_hip(launch_scored(p, a, br, blocks, st));
+    else rc = record_hip(p->d <= 64 ? fa::launch_paged_d64(a, bf16, br, blocks, st) : fa::launch_paged_d128(a, bf16, br, blocks, st));
     if (rc != FLASH_OK || splits == 1) return rc;
     return record_hip(fa::launch_paged_merge(a, bf16, st));
 }
@@ -357,6 +392,60 @@ int run_append(const flash_paged_params* p, hipStream_t st)
     return record_hip(fa::launch_append(a, p->dtype, st));
 }
 
+// ---------------------------------------------------------------------------------------------- drafted tokens
+
+int run_tree_mask(const flash_tree_params* p, hipStream_t st)
+{
+    if (!p || p->B < 0 || p->B >= (1 << 24) || p->total_q < 0 || p->total_q > kMostTokens) return FLASH_EINVAL;
+    if (p->words < 1 || p->words > FLASH_MAX_TREE_TOKENS / 64 || p->mask_stride < p->words) return FLASH_EINVAL;
+    if (p->B == 0 || p->total_q == 0) return FLASH_OK;
+    if (!p->parents || !p->cu_seqlens_q || !p->mask) return FLASH_EINVAL;
+    if (misaligned(p->parents, 4) || misaligned(p->cu_seqlens_q, 4) || misaligned(p->seqlens_k, 4) || misaligned(p->mask, 8) || misaligned(p->positions, 4))
+        return FLASH_EALIGN;
+    if (const int rc = device_usable(); rc != FLASH_OK) return rc;
+    fa::TreeMaskArgs a{};
+    a.parents = p->parents, a.cu = p->cu_seqlens_q, a.lens = p->seqlens_k, a.mask = reinterpret_cast<uint64_t*>(p->mask), a.positions = p->positions;
+    a.mask_stride = p->mask_stride, a.B = p->B, a.tokens = p->total_q, a.words = p->words;
+    return record_hip(fa::launch_tree_mask(a, st));
+}
+
+int run_keep(const flash_keep_params* p, hipStream_t st)
+{
+    if (!p || p->B < 0 || p->H_kv <= 0 || p->d <= 0 || p->layers < 0 || p->num_pages < 0 || p->page_size <= 0 || p->max_pages < 0 || p->max_path < 0) return FLASH_EINVAL;
+    if (p->d > FLASH_MAX_HEAD_DIM) return FLASH_EHEADDIM;
+    if (p->d % 8 != 0 || p->page_size % 16 != 0 || (long long)p->page_size * p->max_pages > (1LL << 30) || (long long)p->H_kv * p->d > kMostOfToken) return FLASH_EINVAL;
+    for (int64_t s : {p->kc_layer, p->kc_page, p->kc_head, p->kc_row, p->vc_layer, p->vc_page, p->vc_head, p->vc_row})
+        if (s < 0 || odd_stride(s) || s > (1LL << 60)) return FLASH_EINVAL;
+    if (p->block_table_stride < 0 || p->path_stride < 0) return FLASH_EINVAL;
+    if (p->B == 0 || p->layers == 0) return FLASH_OK;
+    const long long parts = (2LL * p->H_kv * (p->d / 8) + 255) / 256;  // (work-groups: a launch is limited to 2^32 threads)
+    if (parts >= 1 << 24 || (long long)p->B * p->layers >= 1 << 24 || parts * p->B * p->layers >= 1 << 24) return FLASH_EINVAL;
+    if (!p->seqlens_k || !p->cu_seqlens_q || !p->accepted || !p->seqlens_out || (p->max_path > 0 && !p->path) || (p->max_pages > 0 && !p->block_table)) return FLASH_EINVAL;
+    if (misaligned(p->seqlens_k, 4) || misaligned(p->cu_seqlens_q, 4) || misaligned(p->accepted, 4) || misaligned(p->seqlens_out, 4) || misaligned(p->path, 4) ||
+        misaligned(p->block_table, 4))
+        return FLASH_EALIGN;
+    // (other work-groups still read the lengths when the first one writes)
+    const int32_t *const o = p->seqlens_out, *const o_end = o + p->B;
+    auto apart_from = [&](const int32_t* t, long long n) { return n <= 0 || o_end <= t || t + n <= o; };
+    if (!apart_from(p->seqlens_k, p->B) || !apart_from(p->cu_seqlens_q, p->B + 1LL) || !apart_from(p->accepted, p->B)) return FLASH_EINVAL;
+    if (p->num_pages > 0) {
+        if (!p->K_cache || !p->V_cache || p->K_cache == p->V_cache) return FLASH_EINVAL;
+        if (misaligned(p->K_cache, 16) || misaligned(p->V_cache, 16)) return FLASH_EALIGN;
+        if (!apart(p->kc_page, p->kc_head, p->num_pages, p->H_kv) || p->kc_row == 0 || (p->layers > 1 && p->kc_layer == 0)) return FLASH_EINVAL;
+        if (!apart(p->vc_page, p->vc_head, p->num_pages, p->H_kv) || p->vc_row == 0 || (p->layers > 1 && p->vc_layer == 0)) return FLASH_EINVAL;
+    }
+    if (const int rc = device_usable(); rc != FLASH_OK) return rc;
+    fa::KeepArgs a{};
+    a.table = p->block_table, a.lens = p->seqlens_k, a.cu = p->cu_seqlens_q, a.path = p->path, a.accepted = p->accepted, a.lens_out = p->seqlens_out;
+    a.K = static_cast<char*>(p->K_cache), a.V = static_cast<char*>(p->V_cache);
+    a.k_layer = 2 * p->kc_layer, a.k_page = 2 * p->kc_page, a.k_head = 2 * p->kc_head, a.k_row = 2 * p->kc_row;
+    a.v_layer = 2 * p->vc_layer, a.v_page = 2 * p->vc_page, a.v_head = 2 * p->vc_head, a.v_row = 2 * p->vc_row;
+    a.table_stride = p->block_table_stride, a.path_stride = p->path_stride;
+    a.B = p->B, a.layers = p->layers, a.Hk = p->H_kv, a.d = p->d, a.num_pages = p->num_pages, a.page = p->page_size;
+    a.capacity = p->num_pages > 0 ? p->page_size * p->max_pages : 0, a.most = p->max_path;
+    return record_hip(fa::launch_keep(a, st));
+}
+
 }  // namespace
 
 #define FLASH_EXPORT __attribute__((visibility("default")))
@@ -369,10 +458,15 @@ FLASH_EXPORT int flash_append_paged(const flash_paged_params* p, void* stream) {
 
 FLASH_EXPORT int flash_forward_paged(const flash_paged_params* p, void* stream) { return run_forward(p, static_cast<hipStream_t>(stream)); }
 
+FLASH_EXPORT int flash_tree_mask(const flash_tree_params* p, void* stream) { return run_tree_mask(p, static_cast<hipStream_t>(stream)); }
+
+FLASH_EXPORT int flash_keep_paged(const flash_keep_params* p, void* stream) { return run_keep(p, static_cast<hipStream_t>(stream)); }
+
 FLASH_EXPORT int flash_forward_paged_resolve_splits(const flash_paged_params* p)
 {
     bool empty;
-    const int rc = validate_paged(p, &empty);
+    int rc = validate_paged(p, &empty);
+    if (rc == FLASH_OK) rc = validate_scores(p);
     if (rc != FLASH_OK) return rc;
     return empty ? 1 : splits_of(p);
 }
@@ -380,7 +474,8 @@ FLASH_EXPORT int flash_forward_paged_resolve_splits(const flash_paged_params* p)
 FLASH_EXPORT int flash_forward_paged_workspace_bytes(const flash_paged_params* p, size_t* o_partial_bytes, size_t* lse_partial_bytes)
 {
     bool empty;
-    const int rc = validate_paged(p, &empty);
+    int rc = validate_paged(p, &empty);
+    if (rc == FLASH_OK) rc = validate_scores(p);
     if (rc != FLASH_OK) return rc;
     const int splits = empty ? 1 : splits_of(p);
     const size_t rows = splits > 1 ? (size_t)p->total_q * p->H * splits : 0;
@@ -404,6 +499,18 @@ FLASH_EXPORT void flash_paged_params_init(flash_paged_params* p)
     p->factor = 1.0f;
 }
 
+FLASH_EXPORT void flash_tree_params_init(flash_tree_params* p)
+{
+    if (p) std::memset(p, 0, sizeof(*p));
+}
+
+FLASH_EXPORT void flash_keep_params_init(flash_keep_params* p)
+{
+    if (p) std::memset(p, 0, sizeof(*p));
+}
+
+FLASH_EXPORT size_t flash_tree_params_size(void) { return sizeof(flash_tree_params); }
+FLASH_EXPORT size_t flash_keep_params_size(void) { return sizeof(flash_keep_params); }
 FLASH_EXPORT size_t flash_rotary_params_size(void) { return sizeof(flash_rotary_params); }
 FLASH_EXPORT size_t flash_paged_params_size(void) { return sizeof(flash_paged_params); }
 

@@ -65,6 +65,24 @@ struct PagedArgs {
     float scale_log2;
 };
 
+// Scores and masks beside those of flash_forward (flash_paged_params: softcap, alibi_slopes, prefix_lens, tree_mask); instances of their own, kScores:
+enum { kScoresPlain, kScoresMasked, kScoresCapped, kScoresSloped, kScoresBoth };  // kScoresMasked: a prefix or a tree alone, which all but kScoresPlain take
+constexpr bool has_cap(int scores) { return scores == kScoresCapped || scores == kScoresBoth; }
+constexpr bool has_slopes(int scores) { return scores == kScoresSloped || scores == kScoresBoth; }
+
+constexpr int kTreeTokens = 256;  // drafted tokens of a sequence that a mask can name
+struct ScoredArgs : PagedArgs {
+    const float* slopes;        // [H]
+    const int32_t* prefix;      // [B], or null
+    const uint64_t* tree;       // [tokens, tree_words], or null.  With a tree `causal` is 0 and `wr` is -1
+    int64_t tree_stride;
+    int tree_words;
+    float cap_in, cap;          // exp2 of cap_in times a product is e^(2 score / cap)
+    float slope_unit;           // of the slopes, to the units of what they are added to
+};
+template <int kScores>
+using ArgsOf = std::conditional_t<kScores == kScoresPlain, PagedArgs, ScoredArgs>;
+
 // What the merge needs of them (short arguments launch faster: common.h)
 struct PagedMergeArgs {
     char* O;
@@ -148,13 +166,22 @@ __device__ __forceinline__ int splits_of_sequence(const PagedArgs& a, int len, i
     return nt <= each ? 1 : (int)((uint32_t)(nt + each - 1) / (uint32_t)each);
 }
 
+// Keys at the begin of sequence b that all its tokens see
+template <class A>
+__device__ __forceinline__ int prefix_of(const A& a, int b)
+{
+    if constexpr (std::is_same_v<A, ScoredArgs>) return a.prefix ? clamp_int(a.prefix[b], 0, a.capacity) : 0;
+    else return 0;
+}
+
 // Of a sequence's n row blocks those that see key c or one behind it: its last ones, as ends do not fall.
-template <int BR>
-__device__ __forceinline__ int blocks_behind(const PagedArgs& a, int tokens, int keys, int n, int c)
+template <int BR, class A>
+__device__ __forceinline__ int blocks_behind(const A& a, int tokens, int keys, int n, int c, int prefix)
 {
     const int reach = a.causal ? 0 : a.wr;
     int x = max(c - (keys - tokens), -(1 << 30)) - reach;  // the first token that sees key c
     x = reach < 0 ? 0 : max(x, 0);
+    if constexpr (std::is_same_v<A, ScoredArgs>) x = c < prefix ? 0 : x;
     return keys <= c || x >= tokens ? 0 : n - x * a.G / BR;
 }
 
@@ -165,8 +192,8 @@ __device__ __forceinline__ int blocks_behind(const PagedArgs& a, int tokens, int
 // under a causal mask is heaviest first; a.ordered: those of all sequences, by the piece of nine of the longest length in which their keys end,
 // the last piece first, a piece's sequences in turn.  a.pieces: first splits of a sequence's row blocks, second splits of those that have one, ...: under a
 // causal mask the others would stand between them with nothing to do, and what comes behind the places of the GPU waits for a round.
-template <int BR>
-__device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedItem* it)
+template <int BR, class A>
+__device__ __forceinline__ bool paged_item(const A& a, int lane, PagedItem* it)
 {
     const int block = blockIdx.x, w = a.by_heads.quotient(block);
     it->hk = block - w * a.Hk;
@@ -184,7 +211,8 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
             first = clamp_int(first, 0, a.tokens), end = clamp_int(end, first, a.tokens), keys = clamp_int(keys, 0, a.capacity);
         }
         const int n = ((end - first) * a.G + BR - 1) / BR;
-        auto ends_behind = [&](int t) { return blocks_behind<BR>(a, end - first, keys, n, a.ordered * t); };
+        const int prefix = prefix_of(a, lane < a.B ? lane : 0);
+        auto ends_behind = [&](int t) { return blocks_behind<BR>(a, end - first, keys, n, a.ordered * t, prefix); };
         int t0 = 0, f0 = n, f1 = 0, before = 0;  // blocks behind the piece's begin (0: all) and behind its end (none behind the last); f1 of all lanes
 #pragma unroll
         for (int step = 3; step > 0; step -= 2) {
@@ -215,7 +243,7 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
             splits_of_sequence(a, keys, &each);
         }
         const int n = ((end - first) * a.G + BR - 1) / BR;
-        const int there = s == 0 ? n : blocks_behind<BR>(a, end - first, keys, n, (int)min((int64_t)s * each * 64, (int64_t)keys));
+        const int there = s == 0 ? n : blocks_behind<BR>(a, end - first, keys, n, (int)min((int64_t)s * each * 64, (int64_t)keys), prefix_of(a, bl < a.B ? bl : 0));
         const int upto = wave_prefix(there, lane);
         const uint64_t past = __builtin_amdgcn_ballot_w64(upto > w);
         if (past == 0) return false;
@@ -266,7 +294,8 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
     it->splits = splits_of_sequence(a, len, &it->per);
     if (a.pieces) {  // of the row block
         const int last = min(it->row0 + BR, it->rows) - 1, reach = a.causal ? 0 : a.wr;
-        const int hi = reach < 0 ? len : min(len, a.by_group.quotient(last) + it->shift + reach + 1);
+        int hi = reach < 0 ? len : min(len, a.by_group.quotient(last) + it->shift + reach + 1);
+        if constexpr (std::is_same_v<A, ScoredArgs>) hi = max(hi, min(len, prefix_of(a, b)));
         it->splits = hi <= it->per * 64 ? 1 : (int)((uint32_t)((hi + 63) / 64 + it->per - 1) / (uint32_t)it->per);
     }
     return it->row0 < it->rows && it->split < it->splits;
@@ -274,8 +303,8 @@ __device__ __forceinline__ bool paged_item(const PagedArgs& a, int lane, PagedIt
 
 // keys [kmin, kmax) that some row of the work-group sees, of those its split's share: the range of the row block is cut, not the
 // sequence, so that windows and short chunks in long caches divide evenly
-template <int BR>
-__device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedItem& it, int* kmin, int* kmax)
+template <int BR, class A>
+__device__ __forceinline__ void paged_range(const A& a, const PagedItem& it, int* kmin, int* kmax)
 {
     const int last = it.row0 + BR < it.rows ? it.row0 + BR - 1 : it.rows - 1;
     const int p0 = a.by_group.quotient(it.row0) + it.shift, p1 = a.by_group.quotient(last) + it.shift;
@@ -283,6 +312,10 @@ __device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedItem&
     if (a.wl >= 0) lo = max(0, p0 - a.wl);
     if (a.causal) hi = min(hi, p1 + 1);
     if (a.wr >= 0) hi = min(hi, p1 + a.wr + 1);
+    if constexpr (std::is_same_v<A, ScoredArgs>) {
+        if (a.tree && a.wl >= 0) lo = max(0, it.shift - a.wl);  // (no token of a tree stands in front of the first one's place)
+        hi = max(hi, min(it.len, prefix_of(a, it.b)));
+    }
     if (it.splits > 1) {
         const int64_t s0 = ((int64_t)(lo >> 6) + (int64_t)it.split * it.per) * 64;
         lo = (int)max((int64_t)lo, min(s0, (int64_t)max(hi, lo)));
@@ -475,6 +508,190 @@ struct PagedSoftmax {
     }
 };
 
+// ---------------------------------------------------------------------------------------------- scores and masks of other kinds
+//
+// A cap turns a score x into c tanh(x / c).  tanh(z) = 1 + 2 t with t = -1 / (1 + e^(2 z)), which grows with z from -1 to 0: the softmax goes by t in place
+// of the product, in units of 2 c log2 e, and the constant c that is missing is added to the LSE.  That is a product, two transcendental
+// instructions and a subtraction per score in front of the usual fma and exp2, 24 cycles of a SIMD beside the 24 that a plain score takes and the 32 of its
+// MFMAs at d = 128.  t is off by at most 3 half steps of 2^-24 (v_exp_f32, the subtraction and v_rcp_f32 one each), a score by 6 c 2^-24; a
+// polynomial for small z that stays relative takes as many cycles (measured: v_exp_f32 and v_rcp_f32 8 cycles a wave, other instructions 4).
+// A bias by distance, slope |p - j|, is the C operand of the scores' first MFMA, one instruction per score; behind a cap it is added to t.
+// A tree's tokens see the keys in front of the chunk, and of the chunk's those whose bit is set; they stand at the chunk's begin plus their depth, the number
+// of tokens that they see in the chunk less one.  The masks of the sequence's tokens and the depths lie in LDS; all they touch is the last tile or
+// the last few of a sequence, which take a mask of 64 bits per row.
+
+struct TreeTable {
+    FA_LDS uint64_t* words;  // [kTreeTokens][tree_words]
+    FA_LDS int* depth;       // [kTreeTokens]
+    int tokens;              // of the sequence, that have a row here
+};
+constexpr int kTreeLds = kTreeTokens * (kTreeTokens / 64) * 8 + kTreeTokens * 4;
+
+// Called by all threads of the work-group; a.tree is there.
+template <int kThreads>
+__device__ __forceinline__ void tree_setup(const ScoredArgs& a, const PagedItem& it, int tid, FA_LDS char* lds, TreeTable* tree)
+{
+    const int W = a.tree_words, n = min(it.len - it.shift, 64 * W);
+    tree->words = (FA_LDS uint64_t*)lds;
+    tree->depth = (FA_LDS int*)(lds + kTreeTokens * (kTreeTokens / 64) * 8);
+    tree->tokens = n;
+    for (int k = tid; k < n * W; k += kThreads) {
+        const int i = (int)((uint32_t)k / (uint32_t)W), w = k - i * W, left = n - 64 * w;  // (bits of tokens that there are not)
+        const uint64_t there = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+        tree->words[k] = a.tree[(int64_t)(it.tok0 + i) * a.tree_stride + w] & there;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+        int c = -1;
+        for (int w = 0; w < W; ++w) c += __builtin_popcountll(tree->words[i * W + w]);
+        tree->depth[i] = max(c, 0);
+    }
+    __syncthreads();
+}
+
+// Keys lo ... hi of the 64 that a tile begins with, counted from its first
+__device__ __forceinline__ uint64_t range_bits(int lo, int hi)
+{
+    const uint64_t below = hi < 0 ? 0ull : hi >= 63 ? ~0ull : (2ull << hi) - 1;
+    return below & (lo <= 0 ? ~0ull : lo > 63 ? 0ull : ~0ull << lo);
+}
+
+// What a lane knows of its row, and its wave of its rows
+template <int kScores>
+struct RowScores {
+    TreeTable tree;
+    int token, base;      // its index in the chunk; the chunk's first key
+    int kmin, kmax;       // keys of the work-group
+    int place, place_min; // position, and one that no row of the wave is in front of
+    float slope;
+
+    // keys [lo, hi] that row r sees, but for the chunk's own of a tree
+    __device__ __forceinline__ void set(const ScoredArgs& a, const PagedItem& it, int r, int kmin_, int kmax_, int* lo, int* hi)
+    {
+        const int rr = r < it.rows ? r : it.rows - 1, i = a.by_group.quotient(rr);
+        kmin = kmin_, kmax = kmax_, base = it.shift, token = i;
+        place = i + it.shift;
+        int l = kmin, h = kmax - 1;
+        if (a.tree) {
+            place = base + (i < tree.tokens ? tree.depth[i] : 0);
+            h = min(h, base - 1);
+        }
+        if (a.wl >= 0) l = max(l, place - a.wl);
+        if (a.causal) h = min(h, place);
+        if (a.wr >= 0) h = min(h, place + a.wr);
+        if (a.prefix) h = max(h, min(prefix_of(a, it.b), kmax) - 1);
+        *lo = l;
+        *hi = h;
+        if constexpr (has_slopes(kScores)) {
+            slope = a.slopes[it.hk * a.G + (rr - i * a.G)] * a.slope_unit;
+            place_min = a.tree ? base : __builtin_amdgcn_readfirstlane(place);
+        }
+    }
+    // the chunk's own keys among the 64 from kb0 on that the row sees
+    __device__ __forceinline__ uint64_t drafted_bits(const ScoredArgs& a, int kb0) const
+    {
+        if (token >= tree.tokens) return 0;
+        const int o = kb0 - base, W = a.tree_words, w = o >> 6, sh = o & 63;
+        const FA_LDS uint64_t* const row = tree.words + token * W;
+        const uint64_t w0 = w >= 0 && w < W ? row[w] : 0ull, w1 = w + 1 >= 0 && w + 1 < W ? row[w + 1] : 0ull;
+        return ((w0 >> sh) | (sh ? w1 << (64 - sh) : 0ull)) & range_bits(kmin - kb0, kmax - 1 - kb0);
+    }
+    __device__ __forceinline__ bool sees(const ScoredArgs& a, int j, int lo, int hi) const
+    {
+        return (j >= lo && j <= hi) || (a.tree && j >= base && (drafted_bits(a, j) & 1));
+    }
+    __device__ __forceinline__ float distance(const ScoredArgs& a, int j) const
+    {
+        int at = j;
+        if (a.tree && j >= base) at = base + (j - base < tree.tokens ? tree.depth[j - base] : 0);
+        return (float)(at - place);
+    }
+    // Bias of the tile at kb0, or what is added to it (C operands of 32 keys and 32 rows; g: lane / 32)
+    template <int KB, bool kAdd>
+    __device__ __forceinline__ void bias(const ScoredArgs& a, v16f (&s)[KB], int kb0, int g) const
+    {
+        const int k0 = kb0 + 4 * g;
+        auto put = [&](int kb, int r, float b) __attribute__((always_inline)) {
+            if constexpr (kAdd) s[kb][r] += b;
+            else s[kb][r] = b;
+        };
+        if (__builtin_expect(kb0 + 32 * KB - 1 <= place_min && (!a.tree || kb0 + 32 * KB <= base), 1)) {  // all keys in front of all rows
+            const float b0 = slope * (float)(k0 - place);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) put(kb, r, __builtin_fmaf(slope, (float)(32 * kb + 8 * (r >> 2) + (r & 3)), b0));
+        } else if (!a.tree || kb0 + 32 * KB <= base) {
+            const float x0 = (float)(k0 - place);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) put(kb, r, -slope * __builtin_fabsf(x0 + (float)(32 * kb + 8 * (r >> 2) + (r & 3))));
+        } else {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) put(kb, r, -slope * __builtin_fabsf(distance(a, k0 + 32 * kb + 8 * (r >> 2) + (r & 3))));
+        }
+    }
+    // From products to what the softmax goes by, masks applied.  sides: as in PagedSoftmax::tile
+    template <int KB>
+    __device__ __forceinline__ void finish(const ScoredArgs& a, v16f (&s)[KB], int kb0, int g, int sides, int lo, int hi) const
+    {
+        if constexpr (has_cap(kScores)) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_amdgcn_rcpf(-1.0f - fast_exp2(s[kb][r] * a.cap_in));
+            if constexpr (has_slopes(kScores)) bias<KB, true>(a, s, kb0, g);
+        }
+        if (__builtin_expect(sides != 0, 0)) {
+            if (a.tree) {
+                const uint64_t seen = (range_bits(lo - kb0, hi - kb0) | drafted_bits(a, kb0)) >> (4 * g);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    const uint32_t bits = (uint32_t)(seen >> (32 * kb));
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kb][r] = bits >> (8 * (r >> 2) + (r & 3)) & 1 ? s[kb][r] : -INFINITY;
+                }
+            } else if constexpr (KB == 2) {
+                mask_tile<false>(s[0], s[1], wave_uniform(mask_modes_general(sides)), lo - kb0 - 4 * g, hi - kb0 - 4 * g, -INFINITY);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = kb0 + 4 * g + 8 * (r >> 2) + (r & 3);
+                    s[0][r] = key < lo || key > hi ? -INFINITY : s[0][r];
+                }
+            }
+        }
+    }
+    // The same of one key's product, unmasked
+    __device__ __forceinline__ float one(const ScoredArgs& a, float s, int j) const
+    {
+        if constexpr (has_cap(kScores)) s = __builtin_amdgcn_rcpf(-1.0f - fast_exp2(s * a.cap_in));
+        if constexpr (has_slopes(kScores)) s -= slope * __builtin_fabsf(distance(a, j));
+        return s;
+    }
+};
+template <>
+struct RowScores<kScoresPlain> {};
+
+template <int kScores>
+__device__ __forceinline__ float lse_of(const ArgsOf<kScores>& a, float m, float l)
+{
+    const float lse = __builtin_fmaf(m, kLn2, fast_log2(l) * kLn2);
+    if constexpr (has_cap(kScores)) return lse + a.cap;
+    else return lse;
+}
+
+// of a wave's 32 rows (lanes 0 ... 31 and again 32 ... 63)
+__device__ __forceinline__ int rows_min(int v)
+{
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) v = min(v, __shfl_xor(v, m));
+    return wave_uniform(v);
+}
+
 __device__ __forceinline__ v8h as_fragment(const uint32_t (&p)[4])
 {
     const v4u t = {p[0], p[1], p[2], p[3]};
@@ -502,14 +719,15 @@ __device__ __forceinline__ void load_q(const PagedArgs& a, const PagedItem& it, 
 // which the row sees a part, or none.  Called once per wave, behind its loop, where some sum is not finite: looks for such
 // values among the wave's partly masked tiles and, if there are any, works out the rows in question once more key by key, visible
 // keys alone.  (Tiles first, first + step, ... of the range from key kb_first on.)
-template <int BC, int MB, bool kBf16>
-__device__ __forceinline__ void paged_rescue(const PagedArgs& a, const PagedItem& it, int r, int kmin, int kmax, int tile0, int ntiles, int first,
-                                                       int step, float m_ref, v16f (&oacc)[MB])
+template <int BC, int MB, bool kBf16, int kScores>
+__device__ __forceinline__ void paged_rescue(const ArgsOf<kScores>& a, const PagedItem& it, int r, int kmin, int kmax, int tile0, int ntiles, int first,
+                                                       int step, float m_ref, v16f (&oacc)[MB], RowScores<kScores>& row)
 {
     const int lane = threadIdx.x & 63, g = lane >> 5;
     const int32_t* const table_row = a.table + (size_t)it.b * a.table_stride;
     int lo, hi;
-    paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
+    if constexpr (kScores == kScoresPlain) paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
+    else row.set(a, it, r, kmin, kmax, &lo, &hi);
     auto row_of = [&](const char* base, uint32_t page_bytes, int64_t head_bytes, uint32_t row_bytes, int j) {
         const int pg = a.by_page.quotient(j);
         const PagedPlace at = {table_row[pg], j - pg * a.page};
@@ -522,7 +740,7 @@ __device__ __forceinline__ void paged_rescue(const PagedArgs& a, const PagedItem
         bool some = false;  // of the lanes' rows does one not see key j?  (the key is told to all rows in turn)
         for (int q = 0; q < 32; ++q) {
             const int l = __builtin_amdgcn_readlane(lo, q), h = __builtin_amdgcn_readlane(hi, q);
-            some |= j < l || j > h;
+            some |= j < l || j > h;  // (of a tree's own tokens all are looked at)
         }
         if (some && j < it.len) {
             const char* const v = row_of(a.V, a.v_page, a.v_head, a.v_row, j);
@@ -539,8 +757,12 @@ __device__ __forceinline__ void paged_rescue(const PagedArgs& a, const PagedItem
     const char* const q = a.Q + (size_t)tok * a.q_token + (size_t)head * a.q_head;
     for (int t = first; t < ntiles; t += step) {
         const int kb0 = (tile0 + t) * BC;
-        const int j0 = max(kb0, lo), j1 = min(kb0 + BC - 1, hi);
+        int j0 = max(kb0, lo), j1 = min(kb0 + BC - 1, hi);
+        if constexpr (kScores != kScoresPlain)
+            if (a.tree) j0 = max(kb0, kmin), j1 = min(kb0 + BC, kmax) - 1;
         for (int j = j0; j <= j1; ++j) {
+            if constexpr (kScores != kScoresPlain)
+                if (!row.sees(a, j, lo, hi)) continue;
             const char* const k = row_of(a.K, a.k_page, a.k_head, a.k_row, j);
             const char* const v = row_of(a.V, a.v_page, a.v_head, a.v_row, j);
             float s = 0.0f;
@@ -549,6 +771,7 @@ __device__ __forceinline__ void paged_rescue(const PagedArgs& a, const PagedItem
                 s = __builtin_fmaf(Elem<kBf16>::low(x), Elem<kBf16>::low(y), s);
                 s = __builtin_fmaf(Elem<kBf16>::high(x), Elem<kBf16>::high(y), s);
             }
+            if constexpr (kScores != kScoresPlain) s = row.one(a, s, j);
             const float e = fast_exp2(__builtin_fmaf(s, a.scale_log2, -m_ref)), p = Elem<kBf16>::low(Elem<kBf16>::pack(e, e));
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb)
@@ -608,8 +831,8 @@ struct FewCfg {
     static_assert(2 * SMEM <= 160 * 1024, "two work-groups per CU");
 };
 
-template <int D, bool kBf16>
-__global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
+template <int D, bool kBf16, int kScores>
+__device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
 {
     using C = FewCfg<D>;
     constexpr int BC = C::BC;
@@ -619,7 +842,7 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6), l32 = lane & 31, g = lane >> 5;
 
     PagedItem it;
-    if (!paged_item<kPagedFewRows>(a, lane, &it)) return;
+    if (!paged_item<kPagedFewRows, ArgsOf<kScores>>(a, lane, &it)) return;
     paged_mark_missing<kPagedFewRows, 256>(a, it, tid);
     int kmin, kmax;
     paged_range<kPagedFewRows>(a, it, &kmin, &kmax);
@@ -629,6 +852,9 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
     }
     const int tile0 = kmin / BC, ntiles = (kmax + BC - 1) / BC - tile0;
     const int len = it.len;
+    RowScores<kScores> row;
+    if constexpr (kScores != kScoresPlain)
+        if (a.tree) tree_setup<256>(a, it, tid, (FA_LDS char*)smem + C::SMEM, &row.tree);
     const int32_t* const table_row = a.table + (size_t)it.b * a.table_stride;
 
     FA_LDS char* const kst = (FA_LDS char*)smem + wave * C::WAVE;
@@ -697,7 +923,8 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
         for (int e = 0; e < 16; ++e) oacc[mb][e] = 0.0f;
 
     int lo, hi;
-    paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
+    if constexpr (kScores == kScoresPlain) paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
+    else row.set(a, it, r, kmin, kmax, &lo, &hi);
     int lo_max = lo, hi_min = hi;
     if (wave < ntiles) {
         ask(wave);
@@ -706,6 +933,8 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
         request_v(wave);
         lo_max = __builtin_amdgcn_readlane(lo, 31);  // (bounds do not fall from row to row)
         hi_min = __builtin_amdgcn_readlane(hi, 0);
+        if constexpr (kScores != kScoresPlain)
+            if (a.tree) lo_max = -rows_min(-lo);  // (but a tree's do)
     }
     const float c2 = a.scale_log2, inv_c2 = __builtin_amdgcn_rcpf(c2);
     const int k_rd = T::k_lane(lane), v_rd = T::v_lane(lane);
@@ -722,16 +951,23 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
         {
             const uint32_t kbase = fragment_base(kst, k_rd);
             const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+            if constexpr (kScores == kScoresSloped) row.template bias<KB, false>(a, s, kb0, g);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) s[kb] = Elem<kBf16>::mfma(k_fragment<D>(kbase, ks, kb), qf[ks], ks == 0 ? z : s[kb]);
+                for (int kb = 0; kb < KB; ++kb)
+                    s[kb] = Elem<kBf16>::mfma(k_fragment<D>(kbase, ks, kb), qf[ks], ks == 0 && kScores != kScoresSloped ? z : s[kb]);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the fragments have been read
         if (more) request_k(t + 4);
         uint32_t p[KB][2][4];
         const int sides = is_negative(kb0 - lo_max) | is_negative(hi_min - (BC - 1) - kb0) << 1;
-        soft.tile(s, oacc, p, c2, inv_c2, sides, lo - kb0 - 4 * g, hi - kb0 - 4 * g);
+        if constexpr (kScores == kScoresPlain) {
+            soft.tile(s, oacc, p, c2, inv_c2, sides, lo - kb0 - 4 * g, hi - kb0 - 4 * g);
+        } else {
+            row.finish(a, s, kb0, g, sides, lo, hi);
+            soft.tile(s, oacc, p, c2, inv_c2, 0, 0, 0);
+        }
         if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         {
@@ -745,7 +981,7 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
         if (more) request_v(t + 4);
     }
     if (wave < ntiles && __builtin_expect(any_not_finite<MB>(oacc), 0))
-        paged_rescue<BC, MB, kBf16>(a, it, r, kmin, kmax, tile0, ntiles, wave, 4, soft.m_ref, oacc);
+        paged_rescue<BC, MB, kBf16, kScores>(a, it, r, kmin, kmax, tile0, ntiles, wave, 4, soft.m_ref, oacc, row);
 
     // ---- merge of the four waves: reference of a row = the largest of theirs
     const int nrows = min(kPagedFewRows, it.rows - it.row0);
@@ -785,7 +1021,7 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
             for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf(f, src[e], o[e]);
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const float lse = l == 0.0f ? -INFINITY : __builtin_fmaf(m, kLn2, fast_log2(l) * kLn2);
+        const float lse = l == 0.0f ? -INFINITY : lse_of<kScores>(a, m, l);
         int head;
         const int tok = row_token(a, it, it.row0 + row, &head);
         const size_t at = (size_t)tok * a.H + head;
@@ -804,6 +1040,17 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
             if (c == 0) a.LSE[at] = lse;
         }
     }
+}
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedArgs a)
+{
+    few_rows<D, kBf16, kScoresPlain>(a);
+}
+template <int D, bool kBf16, int kScores>
+__global__ void __launch_bounds__(256, 2) scored_few_kernel(const ScoredArgs a)
+{
+    few_rows<D, kBf16, kScores>(a);
 }
 
 // ---------------------------------------------------------------------------------------------- tiles that waves share
@@ -883,8 +1130,8 @@ __device__ __forceinline__ void paged_barrier_keep()
 }
 
 // Results of a wave's 32 rows from first_row on (r: the lane's).  `ost`: LDS of the wave's own, 32 rows of D columns.
-template <int D, int MB, bool kBf16>
-__device__ __forceinline__ void paged_store_rows(const PagedArgs& a, const PagedItem& it, int first_row, int r, int lane, int g, float m_ref, float l_run,
+template <int D, int MB, bool kBf16, int kScores>
+__device__ __forceinline__ void paged_store_rows(const ArgsOf<kScores>& a, const PagedItem& it, int first_row, int r, int lane, int g, float m_ref, float l_run,
                                                  const v16f (&oacc)[MB], FA_LDS char* ost)
 {
     using T = PagedTile<D>;
@@ -892,7 +1139,7 @@ __device__ __forceinline__ void paged_store_rows(const PagedArgs& a, const Paged
     const int l32 = lane & 31;
     const float l = xhalf_sum(l_run);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const float lse = l == 0.0f ? -INFINITY : __builtin_fmaf(m_ref, kLn2, fast_log2(l) * kLn2);
+    const float lse = l == 0.0f ? -INFINITY : lse_of<kScores>(a, m_ref, l);
     int head;
     const int tok = row_token(a, it, r < it.rows ? r : it.rows - 1, &head);
     const size_t at = (size_t)tok * a.H + head;
@@ -969,8 +1216,8 @@ __device__ __forceinline__ void paged_clear_past(FA_LDS char* stage, int left, i
 // DU: columns that are worked on, a multiple of 16 from d on, the scores in steps of 16, O in blocks of 32 (rows in LDS have D): with DU = D the
 // products of d = 80 meet zeroes in every third MFMA (a window of 512 keys B3 H12 N1777, DU 128, 96, 80: 32.1, 29.8, 29.3 us; 8 x up to 2000 rows H16
 // 69.9 -> 67.0 with 80; d = 40 on 8000 keys 89.7 -> 86.6 with 48; d = 112 138.0 -> 136.2 with 112).
-template <int D, int DU, bool kBf16>
-__global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const PagedArgs a)
+template <int D, int DU, bool kBf16, int kScores>
+__device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
 {
     using T = PagedTile<D>;
     using C = TallCfg<D>;
@@ -982,7 +1229,7 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6), grp = wave >> 2, l32 = lane & 31, g = lane >> 5;
 
     PagedItem it;
-    if (!paged_item<kPagedTallRows>(a, lane, &it)) return;
+    if (!paged_item<kPagedTallRows, ArgsOf<kScores>>(a, lane, &it)) return;
     paged_mark_missing<kPagedTallRows, 512>(a, it, tid);
     int kmin, kmax;
     paged_range<kPagedTallRows>(a, it, &kmin, &kmax);
@@ -1006,11 +1253,19 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
 
     // ---- what the rows of this wave see
     int lo, hi, lo_max, hi_min, lo_min, hi_max;
-    paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
+    RowScores<kScores> row;
+    if constexpr (kScores == kScoresPlain) {
+        paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
+    } else {
+        if (a.tree) tree_setup<512>(a, it, tid, (FA_LDS char*)smem + C::SMEM, &row.tree);
+        row.set(a, it, r, kmin, kmax, &lo, &hi);
+    }
     lo_min = __builtin_amdgcn_readlane(lo, 0);
     hi_min = __builtin_amdgcn_readlane(hi, 0);
     lo_max = __builtin_amdgcn_readlane(lo, 31);  // (bounds do not fall from row to row)
     hi_max = __builtin_amdgcn_readlane(hi, 31);
+    if constexpr (kScores != kScoresPlain)
+        if (a.tree) lo_min = rows_min(lo), lo_max = -rows_min(-lo), hi_max = kmax - 1;  // (but a tree's do)
 
     v8h qf[KS];
     v16f oacc[MB], s[2];
@@ -1043,13 +1298,17 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) s[kb] = E::mfma(kf[ks][kb], qf[ks], s[kb]);
     };
-    auto s_clear = [&]() {
+    auto s_clear = [&](int kb0) __attribute__((always_inline)) {  // kb0: of the tile whose scores come next
+        if constexpr (kScores == kScoresSloped) {
+            row.template bias<2, false>(a, s, kb0, g);
+        } else {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[kb][e] = 0.0f;
+                for (int e = 0; e < 16; ++e) s[kb][e] = 0.0f;
+        }
     };
-    auto mfma_phase = [&](auto last_c, uint32_t vbase, uint32_t kbase) __attribute__((always_inline)) {
+    auto mfma_phase = [&](auto last_c, uint32_t vbase, uint32_t kbase, int kb0) __attribute__((always_inline)) {
         constexpr bool kLast = decltype(last_c)::value;
         // step st: reads of V step st + VPD (behind the last ones: of K), MFMAs of step st
         pv_mfma(0);
@@ -1064,7 +1323,7 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
             pv_mfma(st);
         }
         if constexpr (!kLast) {
-            s_clear();
+            s_clear(kb0 + BC);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if (ks + KPD < KS) k_read(kbase, ks + KPD);
@@ -1100,7 +1359,12 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
                          FA_LDS char* __restrict__ wrv, int t) __attribute__((always_inline)) {
         const int kb0 = (tile0 + t) * BC;
         if (t + 2 < ntiles) req.load_v(a, t + 2, wrv);
-        soft.tile(s, oacc, p, c2, inv_c2, mask_sides(kb0, lo_max, hi_min), lo - kb0 - 4 * g, hi - kb0 - 4 * g);
+        if constexpr (kScores == kScoresPlain) {
+            soft.tile(s, oacc, p, c2, inv_c2, mask_sides(kb0, lo_max, hi_min), lo - kb0 - 4 * g, hi - kb0 - 4 * g);
+        } else {
+            row.finish(a, s, kb0, g, mask_sides(kb0, lo_max, hi_min), lo, hi);
+            soft.tile(s, oacc, p, c2, inv_c2, 0, 0, 0);
+        }
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t vbase = fragment_base(rdv, v_rd);
         const uint32_t kbase = fragment_base(rdk, k_rd);
@@ -1109,7 +1373,7 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
         v_read(vbase, 1);
         paged_barrier_keep<2 * VPD * MB>();
         __builtin_amdgcn_s_setprio(1);
-        mfma_phase(last_c, vbase, kbase);
+        mfma_phase(last_c, vbase, kbase, kb0);
         __builtin_amdgcn_s_setprio(0);
         tail_requests(t, wrk);
         paged_barrier();
@@ -1158,7 +1422,7 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
         const uint32_t kbase = fragment_base(Ks, k_rd);
 #pragma unroll
         for (int ks = 0; ks < KPD; ++ks) k_read(kbase, ks);
-        s_clear();
+        s_clear(tile0 * BC);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             if (ks + KPD < KS) k_read(kbase, ks + KPD);
@@ -1204,8 +1468,19 @@ __global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const
     if (first_row >= it.rows) return;
 
     // ---- epilogue
-    if (__builtin_expect(any_not_finite<MB>(oacc), 0)) paged_rescue<BC, MB, kBf16>(a, it, r, kmin, kmax, tile0, ntiles, 0, 1, soft.m_ref, oacc);
-    paged_store_rows<D, MB, kBf16>(a, it, first_row, r, lane, g, soft.m_ref, soft.l_run, oacc, Ks + wave * (32 * T::ROW));
+    if (__builtin_expect(any_not_finite<MB>(oacc), 0)) paged_rescue<BC, MB, kBf16, kScores>(a, it, r, kmin, kmax, tile0, ntiles, 0, 1, soft.m_ref, oacc, row);
+    paged_store_rows<D, MB, kBf16, kScores>(a, it, first_row, r, lane, g, soft.m_ref, soft.l_run, oacc, Ks + wave * (32 * T::ROW));
+}
+
+template <int D, int DU, bool kBf16>
+__global__ void __launch_bounds__(512, DU == 32 ? 4 : 2) paged_tall_kernel(const PagedArgs a)
+{
+    tall_rows<D, DU, kBf16, kScoresPlain>(a);
+}
+template <int D, int DU, bool kBf16, int kScores>
+__global__ void __launch_bounds__(512, 2) scored_tall_kernel(const ScoredArgs a)
+{
+    tall_rows<D, DU, kBf16, kScores>(a);
 }
 
 // ---------------------------------------------------------------------------------------------- merge of splits
@@ -1318,6 +1593,39 @@ inline int launch_paged_bucket(const PagedArgs& a, bool bf16, int rows, long lon
 {
     return bf16 ? launch_paged_type<D, true>(a, rows, blocks, st) : launch_paged_type<D, false>(a, rows, blocks, st);
 }
+
+template <int D, int DU, bool kBf16, int kScores, int kRows>
+inline hipError_t launch_scored_instance(const ScoredArgs& a, long long blocks, hipStream_t st)
+{
+    const auto kern = [] {
+        if constexpr (kRows == kPagedFewRows) return scored_few_kernel<D, kBf16, kScores>;
+        else return scored_tall_kernel<D, DU, kBf16, kScores>;
+    }();
+    constexpr int tiles = kRows == kPagedFewRows ? FewCfg<D>::SMEM : TallCfg<D>::SMEM, most = tiles + kTreeLds;
+    static_assert(most * (kRows == kPagedFewRows ? 2 : 1) <= 160 * 1024, "work-groups per CU");
+    static DeviceFlags attr_done;  // per instantiation and device
+    if (hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), most, attr_done); e != hipSuccess) return e;
+    return launch_kernel(kern, dim3((unsigned)blocks), dim3(paged_threads(kRows)), a.tree ? most : tiles, st, a);
+}
+template <int kScores, bool kBf16>
+inline int launch_scored_type(const ScoredArgs& a, int rows, long long blocks, hipStream_t st)
+{
+    if (rows == kPagedFewRows)
+        return (int)(a.d <= 64 ? launch_scored_instance<64, 64, kBf16, kScores, kPagedFewRows>(a, blocks, st)
+                               : launch_scored_instance<128, 128, kBf16, kScores, kPagedFewRows>(a, blocks, st));
+    if (a.d <= 64) return (int)launch_scored_instance<64, 64, kBf16, kScores, kPagedTallRows>(a, blocks, st);
+    if (a.d <= 96) return (int)launch_scored_instance<128, 96, kBf16, kScores, kPagedTallRows>(a, blocks, st);
+    return (int)launch_scored_instance<128, 128, kBf16, kScores, kPagedTallRows>(a, blocks, st);
+}
+template <int kScores>
+inline int launch_scored_kind(const ScoredArgs& a, bool bf16, int rows, long long blocks, hipStream_t st)
+{
+    return bf16 ? launch_scored_type<kScores, true>(a, rows, blocks, st) : launch_scored_type<kScores, false>(a, rows, blocks, st);
+}
+int launch_scored_masked(const ScoredArgs& a, bool bf16, int rows, long long blocks, hipStream_t st);
+int launch_scored_capped(const ScoredArgs& a, bool bf16, int rows, long long blocks, hipStream_t st);
+int launch_scored_sloped(const ScoredArgs& a, bool bf16, int rows, long long blocks, hipStream_t st);
+int launch_scored_both(const ScoredArgs& a, bool bf16, int rows, long long blocks, hipStream_t st);
 
 int launch_paged_d64(const PagedArgs& a, bool bf16, int rows, long long blocks, hipStream_t st);
 int launch_paged_d128(const PagedArgs& a, bool bf16, int rows, long long blocks, hipStream_t st);

@@ -284,6 +284,10 @@ typedef int (*paged_fn)(const flash_paged_params*, void*);
 typedef int (*paged_resolve_fn)(const flash_paged_params*);
 rotary_fn g_rotary = nullptr;
 paged_fn g_append = nullptr, g_paged = nullptr;
+typedef int (*tree_fn)(const flash_tree_params*, void*);
+typedef int (*keep_fn)(const flash_keep_params*, void*);
+tree_fn g_tree = nullptr;
+keep_fn g_keep = nullptr;
 paged_resolve_fn g_paged_resolve = nullptr;
 
 int dtype_of(const at::Tensor& t)
@@ -428,15 +432,92 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n)
     });
 }
 
-// paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, causal, window, num_splits, workspace, out, lse)
+// rows [T, words] of a tree's mask
+bool tree_ok(const at::Tensor& t, int64_t T)
+{
+    return t.scalar_type() == at::kLong && t.dim() == 2 && t.size(0) == T && t.size(1) >= 1 && t.size(1) <= FLASH_MAX_TREE_TOKENS / 64 && unit_stride(t) && is_here(t);
+}
+int64_t tree_stride(const at::Tensor& t) { return t.size(0) <= 1 ? std::max<int64_t>(t.stride(0), t.size(1)) : t.stride(0); }
+// int32 with so many dimensions, the last one contiguous
+bool index_ok(const at::Tensor& t, int64_t dims) { return t.scalar_type() == at::kInt && t.dim() == dims && unit_stride(t) && is_here(t) && fits_int(t); }
+
+// tree_mask(parents, cu_seqlens_q, seqlens_k, max_seqlen_q, mask, positions)
+PyObject* tree_mask(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    return guarded([&]() -> PyObject* {
+        if (n != 6 || !g_tree || !allocates_plainly()) return not_implemented();
+        const at::Tensor *parents = tensor_of(args[0]), *cu = tensor_of(args[1]), *lens, *mask, *pos;
+        int most;
+        if (!parents || !cu || !optional_tensor(args[2], &lens) || !small_int(args[3], &most) || !optional_tensor(args[4], &mask) || !optional_tensor(args[5], &pos))
+            return not_implemented();
+        if (!index_ok(*parents, 1) || !index_ok(*cu, 1) || cu->size(0) < 1 || (lens && (!index_ok(*lens, 1) || lens->size(0) != cu->size(0) - 1))) return not_implemented();
+        const int64_t T = parents->size(0), longest = most > 0 && most < T ? most : T, words = longest > 64 ? (longest + 63) / 64 : 1;
+        if (longest > FLASH_MAX_TREE_TOKENS || (mask && (!tree_ok(*mask, T) || mask->size(1) < words)) || (pos && (!index_ok(*pos, 1) || pos->size(0) != T)))
+            return not_implemented();
+        const at::Tensor m = mask ? *mask : empty_on(*parents, {T, words}, at::kLong), y = pos ? *pos : empty_on(*parents, {T}, at::kInt);
+        flash_tree_params p{};
+        p.parents = static_cast<const int32_t*>(parents->data_ptr()), p.cu_seqlens_q = static_cast<const int32_t*>(cu->data_ptr());
+        p.seqlens_k = lens ? static_cast<const int32_t*>(lens->data_ptr()) : nullptr;
+        p.mask = static_cast<int64_t*>(m.data_ptr()), p.positions = static_cast<int32_t*>(y.data_ptr());
+        p.B = (int)cu->size(0) - 1, p.total_q = (int)T, p.words = (int)m.size(1), p.mask_stride = tree_stride(m);
+        const int rc = g_tree(&p, c10::hip::getCurrentHIPStream().stream());
+        if (rc != FLASH_OK) return raise(rc, "flash_tree_mask");
+        written({mask, pos});
+        PyObject* res = PyTuple_New(2);
+        if (!res) return nullptr;
+        PyTuple_SET_ITEM(res, 0, THPVariable_Wrap(m));
+        PyTuple_SET_ITEM(res, 1, THPVariable_Wrap(y));
+        return res;
+    });
+}
+
+// keep(k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, path, accepted, out)
+PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    return guarded([&]() -> PyObject* {
+        if (n != 8 || !g_keep || !allocates_plainly()) return not_implemented();
+        const at::Tensor* t[7];
+        for (int i = 0; i < 7; ++i)
+            if (!(t[i] = tensor_of(args[i])) || !is_here(*t[i]) || !fits_int(*t[i])) return not_implemented();
+        const at::Tensor &k = *t[0], &v = *t[1], &table = *t[2], &lens = *t[3], &cu = *t[4], &path = *t[5], &accepted = *t[6];
+        const at::Tensor* out;
+        if (!optional_tensor(args[7], &out) || wants_derivative({&k, &v})) return not_implemented();
+        const int64_t dims = k.dim(), B = lens.dim() == 1 ? lens.size(0) : -1;
+        if ((dims != 4 && dims != 5) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || (k.scalar_type() != at::kHalf && k.scalar_type() != at::kBFloat16))
+            return not_implemented();
+        if (k.stride(-1) != 1 || v.stride(-1) != 1 || !index_ok(table, 2) || !index_ok(lens, 1) || !index_ok(cu, 1) || !index_ok(path, 2) || !index_ok(accepted, 1))
+            return not_implemented();
+        if (table.size(0) != B || cu.size(0) != B + 1 || path.size(0) != B || accepted.size(0) != B || (out && (!index_ok(*out, 1) || out->size(0) != B))) return not_implemented();
+        const at::Tensor o = out ? *out : empty_on(lens, {B}, at::kInt);
+        flash_keep_params p{};
+        p.K_cache = k.data_ptr(), p.V_cache = v.data_ptr();
+        p.block_table = static_cast<const int32_t*>(table.data_ptr()), p.seqlens_k = static_cast<const int32_t*>(lens.data_ptr());
+        p.cu_seqlens_q = static_cast<const int32_t*>(cu.data_ptr()), p.path = static_cast<const int32_t*>(path.data_ptr());
+        p.accepted = static_cast<const int32_t*>(accepted.data_ptr()), p.seqlens_out = static_cast<int32_t*>(o.data_ptr());
+        p.B = (int)B, p.layers = dims == 5 ? (int)k.size(0) : 1, p.max_pages = (int)table.size(1), p.max_path = (int)path.size(1);
+        p.num_pages = (int)k.size(-4), p.H_kv = (int)k.size(-3), p.page_size = (int)k.size(-2), p.d = (int)k.size(-1);
+        p.kc_layer = dims == 5 ? k.stride(0) : 0, p.kc_page = k.stride(-4), p.kc_head = k.stride(-3), p.kc_row = k.stride(-2);
+        p.vc_layer = dims == 5 ? v.stride(0) : 0, p.vc_page = v.stride(-4), p.vc_head = v.stride(-3), p.vc_row = v.stride(-2);
+        p.block_table_stride = table.stride(0), p.path_stride = path.stride(0);
+        const int rc = g_keep(&p, c10::hip::getCurrentHIPStream().stream());
+        if (rc != FLASH_OK) return raise(rc, "flash_keep_paged");
+        written({&k, &v, out});
+        return THPVariable_Wrap(o);
+    });
+}
+
+// paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, causal, window, num_splits, workspace, out, lse
+//       [, softcap, alibi_slopes, prefix_lens, tree_mask])
 PyObject* paged(PyObject*, PyObject* const* args, Py_ssize_t n)
 {
     return guarded([&]() -> PyObject* {
-        if (n != 15 || !g_paged || !allocates_plainly()) return not_implemented();
-        const at::Tensor *q = tensor_of(args[0]), *out, *lse;
+        if ((n != 15 && n != 19) || !g_paged || !allocates_plainly()) return not_implemented();
+        const at::Tensor *q = tensor_of(args[0]), *out, *lse, *slopes = nullptr, *prefix = nullptr, *tree = nullptr;
         flash_paged_params p{};
         if (!q || !parse_cache(args + 1, p) || !optional_tensor(args[13], &out) || !optional_tensor(args[14], &lse)) return not_implemented();
-        if (wants_derivative({q, tensor_of(args[1]), tensor_of(args[2]), out, lse})) return not_implemented();
+        if (n == 19 && (!real(args[15], &p.softcap) || !optional_tensor(args[16], &slopes) || !optional_tensor(args[17], &prefix) || !optional_tensor(args[18], &tree)))
+            return not_implemented();
+        if (wants_derivative({q, tensor_of(args[1]), tensor_of(args[2]), out, lse, slopes})) return not_implemented();
         if (!small_int(args[6], &p.max_seqlen_q) || !small_int(args[7], &p.max_seqlen_k) || !PyBool_Check(args[9]) || !small_int(args[11], &p.num_splits)) return not_implemented();
         if (args[8] == Py_None) p.softmax_scale = (float)std::pow((double)p.d, -0.5);
         else if (!real(args[8], &p.softmax_scale)) return not_implemented();
@@ -450,6 +531,18 @@ PyObject* paged(PyObject*, PyObject* const* args, Py_ssize_t n)
         if (lse && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != T || lse->size(1) != H || !lse->is_contiguous() || !is_here(*lse)))
             return not_implemented();
         p.total_q = (int)T, p.H = (int)H;
+        if (slopes) {
+            if (slopes->scalar_type() != at::kFloat || slopes->dim() != 1 || slopes->size(0) != H || !slopes->is_contiguous() || !is_here(*slopes)) return not_implemented();
+            p.alibi_slopes = static_cast<const float*>(slopes->data_ptr());
+        }
+        if (prefix) {
+            if (!index_ok(*prefix, 1) || prefix->size(0) != p.B) return not_implemented();
+            p.prefix_lens = static_cast<const int32_t*>(prefix->data_ptr());
+        }
+        if (tree) {
+            if (!tree_ok(*tree, T) || T == 0) return not_implemented();
+            p.tree_mask = static_cast<const int64_t*>(tree->data_ptr()), p.tree_words = (int)tree->size(1), p.tree_stride = tree_stride(*tree);
+        }
         const int S = g_paged_resolve(&p);
         if (S < 0) return raise(S, "flash_forward_paged_resolve_splits");
         const int64_t rows = S > 1 ? T * H * S : 0;
@@ -482,11 +575,14 @@ PyObject* paged(PyObject*, PyObject* const* args, Py_ssize_t n)
     });
 }
 
-// bind_paged(addresses of flash_rotary, flash_append_paged, flash_forward_paged, flash_forward_paged_resolve_splits), behind bind()
+// bind_paged(addresses of flash_rotary, flash_append_paged, flash_forward_paged, flash_forward_paged_resolve_splits, flash_tree_mask, flash_keep_paged), behind
+// bind()
 PyObject* bind_paged(PyObject*, PyObject* args)
 {
-    unsigned long long r, a, f, s;
-    if (!PyArg_ParseTuple(args, "KKKK", &r, &a, &f, &s)) return nullptr;
+    unsigned long long r, a, f, s, t, k;
+    if (!PyArg_ParseTuple(args, "KKKKKK", &r, &a, &f, &s, &t, &k)) return nullptr;
+    g_tree = reinterpret_cast<tree_fn>(t);
+    g_keep = reinterpret_cast<keep_fn>(k);
     g_rotary = reinterpret_cast<rotary_fn>(r);
     g_append = reinterpret_cast<paged_fn>(a);
     g_paged = reinterpret_cast<paged_fn>(f);
@@ -516,6 +612,8 @@ PyMethodDef methods[] = {
     {"bind_paged", bind_paged, METH_VARARGS, nullptr},
     {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
+    {"tree_mask", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(tree_mask)), METH_FASTCALL, nullptr},
+    {"keep", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(keep)), METH_FASTCALL, nullptr},
     {"paged", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

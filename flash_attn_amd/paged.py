@@ -1,5 +1,5 @@
-"""Rotary positions and attention over a paged K/V cache: the Python side of flash_rotary, flash_append_paged and
-flash_forward_paged (include/flash_attn_mi355.h).
+"""Rotary positions, attention over a paged K/V cache and drafted tokens: the Python side of flash_rotary, flash_append_paged, flash_forward_paged,
+flash_tree_mask and flash_keep_paged (include/flash_attn_mi355.h).
 
 A serving loop keeps K and V in pages of a pool, `[pages, H_kv, page_size, d]`, a table that names each sequence's pages, and the
 sequences' lengths.  One step takes the new tokens of all sequences, `[tokens, H, d]`, one after the other:
@@ -7,7 +7,14 @@ sequences' lengths.  One step takes the new tokens of all sequences, `[tokens, H
     q = flash_append_paged(k, v, k_cache, v_cache, table, lens, cu, q=q, inv_freq=inv_freq)
     o, lse = flash_forward_paged(q, k_cache, v_cache, table, lens, cu, max_seqlen_q, max_seqlen_k, causal=True)
 
-Everything that changes from step to step is read on the GPU (lengths, table, positions), so that a captured graph follows it.
+A step that checks a tree of drafted tokens per sequence has three more arguments and one more call:
+
+    mask, positions = flash_tree_mask(parents, cu, lens, max_seqlen_q)
+    q = flash_append_paged(k, v, k_cache, v_cache, table, lens, cu, q=q, inv_freq=inv_freq, positions=positions)
+    o, lse = flash_forward_paged(q, k_cache, v_cache, table, lens, cu, max_seqlen_q, max_seqlen_k, tree_mask=mask)
+    lens = flash_keep_paged(k_caches, v_caches, table, lens, cu, path, accepted)   # once the answers have said which path stays
+
+Everything that changes from step to step is read on the GPU (lengths, table, positions, masks, paths), so that a captured graph follows it.
 """
 import ctypes as C
 import math
@@ -46,6 +53,33 @@ class PagedParams(C.Structure):
         ("is_causal", C.c_int), ("window_left", C.c_int), ("window_right", C.c_int), ("num_splits", C.c_int),
         ("inv_freq", C.c_void_p), ("rot", C.c_int), ("interleaved", C.c_int), ("factor", C.c_float),
         ("positions", C.c_void_p), ("positions_64", C.c_int),
+        ("softcap", C.c_float), ("alibi_slopes", C.c_void_p), ("prefix_lens", C.c_void_p),
+        ("tree_mask", C.c_void_p), ("tree_words", C.c_int), ("tree_stride", C.c_int64),
+    ]
+
+
+FLASH_MAX_SOFTCAP = 1000.0
+FLASH_MAX_TREE_TOKENS = 256
+
+
+class TreeParams(C.Structure):
+    """struct flash_tree_params, field for field."""
+    _fields_ = [
+        ("parents", C.c_void_p), ("cu_seqlens_q", C.c_void_p), ("seqlens_k", C.c_void_p), ("mask", C.c_void_p), ("positions", C.c_void_p),
+        ("B", C.c_int), ("total_q", C.c_int), ("words", C.c_int), ("mask_stride", C.c_int64),
+    ]
+
+
+class KeepParams(C.Structure):
+    """struct flash_keep_params, field for field."""
+    _fields_ = [
+        ("K_cache", C.c_void_p), ("V_cache", C.c_void_p), ("block_table", C.c_void_p), ("seqlens_k", C.c_void_p), ("cu_seqlens_q", C.c_void_p),
+        ("path", C.c_void_p), ("accepted", C.c_void_p), ("seqlens_out", C.c_void_p),
+        ("B", C.c_int), ("H_kv", C.c_int), ("d", C.c_int), ("layers", C.c_int), ("num_pages", C.c_int), ("page_size", C.c_int), ("max_pages", C.c_int),
+        ("max_path", C.c_int),
+        ("kc_layer", C.c_int64), ("kc_page", C.c_int64), ("kc_head", C.c_int64), ("kc_row", C.c_int64),
+        ("vc_layer", C.c_int64), ("vc_page", C.c_int64), ("vc_head", C.c_int64), ("vc_row", C.c_int64),
+        ("block_table_stride", C.c_int64), ("path_stride", C.c_int64),
     ]
 
 
@@ -58,11 +92,13 @@ def _lib():
         L = binding.lib()
         rp, pp = C.POINTER(RotaryParams), C.POINTER(PagedParams)
         for name, args in (("flash_rotary", [rp, C.c_void_p]), ("flash_append_paged", [pp, C.c_void_p]), ("flash_forward_paged", [pp, C.c_void_p]),
+                           ("flash_tree_mask", [C.POINTER(TreeParams), C.c_void_p]), ("flash_keep_paged", [C.POINTER(KeepParams), C.c_void_p]),
                            ("flash_forward_paged_resolve_splits", [pp]),
                            ("flash_forward_paged_workspace_bytes", [pp, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)])):
             f = getattr(L, name)
             f.restype, f.argtypes = C.c_int, args
-        for name, p in (("flash_rotary_params", RotaryParams), ("flash_paged_params", PagedParams)):
+        for name, p in (("flash_rotary_params", RotaryParams), ("flash_paged_params", PagedParams), ("flash_tree_params", TreeParams),
+                        ("flash_keep_params", KeepParams)):
             size, init = getattr(L, name + "_size"), getattr(L, name + "_init")
             size.restype, init.restype, init.argtypes = C.c_size_t, None, [C.POINTER(p)]
             if size() != C.sizeof(p):
@@ -78,7 +114,7 @@ class _NoFrontEnd:
     def rotary(*args):
         return NotImplemented
 
-    append = paged = rotary
+    append = paged = tree_mask = keep = rotary
 
 
 _native = None
@@ -90,7 +126,7 @@ def _front_end():
     L, n = _lib(), binding._native or binding._front_end()
     if hasattr(n, "bind_paged"):
         n.bind_paged(*(C.cast(f, C.c_void_p).value for f in (L.flash_rotary, L.flash_append_paged, L.flash_forward_paged,
-                                                             L.flash_forward_paged_resolve_splits)))
+                                                             L.flash_forward_paged_resolve_splits, L.flash_tree_mask, L.flash_keep_paged)))
         _native = n
     else:
         _native = _NoFrontEnd
@@ -407,7 +443,8 @@ def flash_append_paged(k, v, k_cache, v_cache, block_table, seqlens_k, cu_seqlen
 
 
 def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, max_seqlen_q=0, max_seqlen_k=0, softmax_scale=None, causal=False,
-                        window=(-1, -1), num_splits=0, workspace=None, out=None, lse=None, stream=None):
+                        window=(-1, -1), num_splits=0, workspace=None, out=None, lse=None, stream=None, softcap=0.0, alibi_slopes=None, prefix_lens=None,
+                        tree_mask=None):
     """Attention of the new tokens q [tokens,H,d] over their sequences' pages: (O [tokens,H,d], LSE fp32 [tokens,H]).
 
     Query head h reads K/V head h / (H / H_kv).  Token i of n stands at position seqlens_k - n + i; causal and window (left, right) are as in
@@ -416,16 +453,27 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
     num_splits <= 0: the library's choice.
     workspace: (O_partial, LSE_partial) of at least the bytes that paged_workspace_bytes says, otherwise allocated here.
     Rows that belong to no sequence are left as they are (new memory where out and lse are not given).  For serving: tensors that require a gradient
-    are refused while gradients are recorded."""
+    are refused while gradients are recorded.
+
+    softcap > 0: scores x become softcap * tanh(x / softcap), up to FLASH_MAX_SOFTCAP.  alibi_slopes: fp32 [H], finite, score -= slope[h] * |i - j| of
+    the positions, behind the cap.  prefix_lens: int32 [B], keys in front of it are seen by all of a sequence's tokens, whatever causal and a
+    right window say.  tree_mask: int64 [tokens, words] (flash_tree_mask): bit j % 64 of word j / 64 says whether a token sees new token j of its
+    sequence, in place of causal; with it max_seqlen_q is at most 64 * words, tokens stand at the chunk's begin plus their depth (bits less one), a right
+    window and a prefix are refused, and a left window must reach over a chunk."""
     if stream is None:
-        res = (_native or _front_end()).paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
-                                              window, num_splits, workspace, out, lse)
+        native = _native or _front_end()
+        if softcap == 0 and alibi_slopes is None and prefix_lens is None and tree_mask is None:
+            res = native.paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, causal, window,
+                               num_splits, workspace, out, lse)
+        else:
+            res = native.paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, causal, window,
+                               num_splits, workspace, out, lse, softcap, alibi_slopes, prefix_lens, tree_mask)
         if res is not NotImplemented:
             return res
     # arguments that the native front end leaves alone (those that raise among them)
     import torch
 
-    _no_gradients("flash_forward_paged", q, k_cache, v_cache, out, lse)
+    _no_gradients("flash_forward_paged", q, k_cache, v_cache, out, lse, alibi_slopes)
     _check(q.dim() == 3 and k_cache.dim() == 4, "q must be [tokens,H,d], caches [pages,H_kv,page_size,d]")
     T, H, d = q.shape
     Hk = k_cache.shape[1]
@@ -438,8 +486,19 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
     p.is_causal = int(bool(causal))
     p.window_left, p.window_right = _int(window[0]), _int(window[1])
     p.num_splits = _int(num_splits)
+    p.softcap = float(softcap)
+    if alibi_slopes is not None:
+        _check(alibi_slopes.dtype == torch.float32 and tuple(alibi_slopes.shape) == (H,) and alibi_slopes.is_contiguous(), "alibi_slopes must be contiguous fp32 [H]")
+        p.alibi_slopes = alibi_slopes.data_ptr()
+    if prefix_lens is not None:
+        _check(prefix_lens.dtype == torch.int32 and tuple(prefix_lens.shape) == (p.B,) and prefix_lens.is_contiguous(), "prefix_lens must be contiguous int32 [B]")
+        p.prefix_lens = prefix_lens.data_ptr()
+    if tree_mask is not None:
+        p.tree_words, p.tree_stride = _tree_rows(tree_mask, T)
+        p.tree_mask = tree_mask.data_ptr()
+        _check(T == 0 or tree_mask.data_ptr() != 0, "tree_mask is empty")
     given = workspace if workspace is not None else ()
-    device = _same_device(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, out, lse, *given)
+    device = _same_device(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, out, lse, alibi_slopes, prefix_lens, tree_mask, *given)
     L = _lib()
     S = L.flash_forward_paged_resolve_splits(C.byref(p))
     if S < 0:
@@ -464,7 +523,104 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
     return o, l
 
 
-def _paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k, causal, window, num_splits):
+def _tree_rows(mask, tokens):
+    """(words, stride) of a mask [tokens, words]"""
+    import torch
+
+    _check(mask.dtype == torch.int64 and mask.dim() == 2 and mask.shape[0] == tokens and 1 <= mask.shape[1] <= FLASH_MAX_TREE_TOKENS // 64,
+           f"a tree's mask must be int64 [tokens,words] with 1 ... {FLASH_MAX_TREE_TOKENS // 64} words")
+    _check(mask.shape[1] == 1 or mask.stride(1) == 1, "the last dimension of a tree's mask must be contiguous")
+    return mask.shape[1], max(mask.stride(0), mask.shape[1]) if tokens <= 1 else mask.stride(0)
+
+
+def flash_tree_mask(parents, cu_seqlens_q, seqlens_k=None, max_seqlen_q=0, mask=None, positions=None, stream=None):
+    """(mask int64 [tokens, words], positions int32 [tokens]) of the trees whose tokens have these parents, int32 [tokens], numbered within their chunk.
+
+    A parent stands in front of its children; a number that is not below the token's own, or negative, says that it has none and hangs on the keys in
+    front of the chunk.  A token's row has the bits of the tokens on its path, its own among them, and it stands at seqlens_k - n + (tokens on the
+    path) - 1, without seqlens_k counted from the chunk's begin.  max_seqlen_q: at least the longest chunk (0: the number of tokens), which
+    decides the words, 64 tokens each, up to FLASH_MAX_TREE_TOKENS.  mask, positions: where to."""
+    if stream is None:
+        res = (_native or _front_end()).tree_mask(parents, cu_seqlens_q, seqlens_k, max_seqlen_q, mask, positions)
+        if res is not NotImplemented:
+            return res
+    import torch
+
+    for t, name in ((parents, "parents"), (cu_seqlens_q, "cu_seqlens_q"), (seqlens_k, "seqlens_k")):
+        _check(t is None or (t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()), f"{name} must be contiguous int32 with one dimension")
+    T, B = parents.shape[0], cu_seqlens_q.shape[0] - 1
+    _check(B >= 0 and (seqlens_k is None or seqlens_k.shape[0] == B), "cu_seqlens_q and seqlens_k must be [B + 1] and [B]")
+    _check(max(T, B) <= _INT_MAX, "tensors are too large")
+    most = min(T, max_seqlen_q) if max_seqlen_q > 0 else T
+    _check(most <= FLASH_MAX_TREE_TOKENS, f"trees have at most {FLASH_MAX_TREE_TOKENS} tokens (max_seqlen_q)")
+    words = max(1, -(-most // 64))
+    device = _same_device(parents, cu_seqlens_q, seqlens_k, mask, positions)
+    given = (mask, positions)
+    with _on(device, stream) as handle:
+        if mask is None:
+            mask = torch.empty((T, words), dtype=torch.int64, device=device)
+        if positions is None:
+            positions = torch.empty(T, dtype=torch.int32, device=device)
+        p = TreeParams()
+        p.words, p.mask_stride = _tree_rows(mask, T)
+        _check(p.words >= words, "mask has too few words")
+        _check(positions.dtype == torch.int32 and tuple(positions.shape) == (T,) and positions.is_contiguous(), "positions must be contiguous int32 [tokens]")
+        p.parents, p.cu_seqlens_q, p.mask, p.positions = parents.data_ptr(), cu_seqlens_q.data_ptr(), mask.data_ptr(), positions.data_ptr()
+        p.seqlens_k = seqlens_k.data_ptr() if seqlens_k is not None else None
+        p.B, p.total_q = B, T
+        _raise(_lib().flash_tree_mask(C.byref(p), handle), "flash_tree_mask")
+    _written(*given)
+    return mask, positions
+
+
+def flash_keep_paged(k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, path, accepted, out=None, stream=None):
+    """Moves the rows of the accepted path of each sequence's drafted tokens to the places behind the keys in front of them; returns the lengths, int32 [B].
+
+    Caches [pages,H_kv,page_size,d], or [layers,pages,H_kv,page_size,d] for all layers at once.  path: int32 [B, L], the path's tokens by their numbers in
+    the chunk, which grow; accepted: int32 [B], how many of them stay.  Row path[b, i] of the chunk goes to its row i; a path ends in front of the
+    first number that does not grow or is not a token of the chunk.  Returned: seqlens_k - n + tokens that stay, in `out` if that is given, which cannot
+    be seqlens_k itself."""
+    if stream is None:
+        res = (_native or _front_end()).keep(k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, path, accepted, out)
+        if res is not NotImplemented:
+            return res
+    import torch
+
+    _no_gradients("flash_keep_paged", k_cache, v_cache)
+    _check(k_cache.dim() in (4, 5) and k_cache.shape == v_cache.shape, "k_cache and v_cache must be [pages,H_kv,page_size,d] or [layers,pages,H_kv,page_size,d]")
+    many = k_cache.dim() == 5
+    _check(k_cache.dtype in (torch.float16, torch.bfloat16) and v_cache.dtype == k_cache.dtype, "caches must be fp16 or bf16")
+    _check(k_cache.stride(-1) == 1 and v_cache.stride(-1) == 1, "the last dimension of the caches must be contiguous")
+    for t, name, dim in ((block_table, "block_table", 2), (path, "path", 2), (seqlens_k, "seqlens_k", 1), (cu_seqlens_q, "cu_seqlens_q", 1), (accepted, "accepted", 1),
+                         (out, "out", 1)):
+        _check(t is None or (t.dtype == torch.int32 and t.dim() == dim and (t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1)),
+               f"{name} must be int32 with {dim} dimension(s), the last contiguous")
+    B = seqlens_k.shape[0]
+    _check(block_table.shape[0] == B and path.shape[0] == B and accepted.shape[0] == B and cu_seqlens_q.shape[0] == B + 1 and (out is None or out.shape[0] == B),
+           "block_table, path, accepted, seqlens_k and cu_seqlens_q must be [B,pages], [B,L], [B], [B] and [B + 1]")
+    _check(max(*k_cache.shape, *block_table.shape, *path.shape) <= _INT_MAX, "tensors are too large")
+    device = _same_device(k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, path, accepted, out)
+    given = out
+    with _on(device, stream) as handle:
+        if out is None:
+            out = torch.empty(B, dtype=torch.int32, device=device)
+        p = KeepParams()
+        p.K_cache, p.V_cache = k_cache.data_ptr(), v_cache.data_ptr()
+        p.block_table, p.seqlens_k, p.cu_seqlens_q = block_table.data_ptr(), seqlens_k.data_ptr(), cu_seqlens_q.data_ptr()
+        p.path, p.accepted, p.seqlens_out = path.data_ptr(), accepted.data_ptr(), out.data_ptr()
+        p.num_pages, p.H_kv, p.page_size, p.d = k_cache.shape[-4:]
+        p.B, p.layers, p.max_pages, p.max_path = B, k_cache.shape[0] if many else 1, block_table.shape[1], path.shape[1]
+        p.kc_page, p.kc_head, p.kc_row = k_cache.stride()[-4:-1]
+        p.vc_page, p.vc_head, p.vc_row = v_cache.stride()[-4:-1]
+        if many:
+            p.kc_layer, p.vc_layer = k_cache.stride(0), v_cache.stride(0)
+        p.block_table_stride, p.path_stride = block_table.stride(0), path.stride(0)
+        _raise(_lib().flash_keep_paged(C.byref(p), handle), "flash_keep_paged")
+    _written(k_cache, v_cache, given)
+    return out
+
+
+def _paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k, causal, window, num_splits, prefix, tree_words):
     _check(max(B, H, H_kv, d, total_q, page_size, max_pages) <= _INT_MAX, "sizes are too large")
     p = PagedParams()
     _lib().flash_paged_params_init(C.byref(p))
@@ -472,22 +628,29 @@ def _paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max
     p.num_pages = 1
     p.max_seqlen_q, p.max_seqlen_k = _int(max_seqlen_q), _int(max_seqlen_k)
     p.is_causal, p.window_left, p.window_right, p.num_splits = int(bool(causal)), _int(window[0]), _int(window[1]), _int(num_splits)
+    # (only whether they are there matters)
+    if prefix:
+        p.prefix_lens = 16
+    if tree_words:
+        p.tree_mask, p.tree_words, p.tree_stride = 16, _int(tree_words), _int(tree_words)
     return p
 
 
-def paged_resolve_splits(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q=0, max_seqlen_k=0, causal=False, window=(-1, -1), num_splits=0):
-    """The split count that flash_forward_paged will use for such a call."""
+def paged_resolve_splits(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q=0, max_seqlen_k=0, causal=False, window=(-1, -1), num_splits=0,
+                         prefix=False, tree_words=0):
+    """The split count that flash_forward_paged will use for such a call.  prefix: whether it has prefix_lens; tree_words: of its tree_mask."""
     S = _lib().flash_forward_paged_resolve_splits(C.byref(_paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k,
-                                                                       causal, window, num_splits)))
+                                                                       causal, window, num_splits, prefix, tree_words)))
     if S < 0:
         raise FlashError(S, "flash_forward_paged_resolve_splits")
     return S
 
 
-def paged_workspace_bytes(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q=0, max_seqlen_k=0, causal=False, window=(-1, -1), num_splits=0):
+def paged_workspace_bytes(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q=0, max_seqlen_k=0, causal=False, window=(-1, -1), num_splits=0,
+                          prefix=False, tree_words=0):
     """Bytes of (O_partial, LSE_partial) for flash_forward_paged calls of these sizes and masks."""
     ob, lb = C.c_size_t(), C.c_size_t()
     _raise(_lib().flash_forward_paged_workspace_bytes(C.byref(_paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k,
-                                                                           causal, window, num_splits)), C.byref(ob), C.byref(lb)),
+                                                                           causal, window, num_splits, prefix, tree_words)), C.byref(ob), C.byref(lb)),
            "flash_forward_paged_workspace_bytes")
     return ob.value, lb.value

@@ -260,7 +260,21 @@ typedef struct flash_paged_params {
     float factor;
     const void *positions;     /* NULL: the places in the sequence; otherwise [total_q], for the angles alone */
     int positions_64;
+    /* forward: scores and masks beside the above */
+    float softcap;             /* > 0: scores x = scale q.k become softcap * tanh(x / softcap); up to FLASH_MAX_SOFTCAP.  0: they stay */
+    const float *alibi_slopes; /* fp32 [H], finite, or NULL: score -= slope[h] * |i - j| of the positions, behind the cap */
+    const int32_t *prefix_lens;   /* [B], or NULL: keys j < prefix_lens[b] are seen whatever is_causal and window_right say */
+    const int64_t *tree_mask;  /* [total_q] rows of tree_words words, or NULL: the new tokens are a tree's, and bit j % 64 of word j / 64 of a token's row says
+                                * whether it sees new token j of its sequence (itself among them).  It takes the place of is_causal; window_right and
+                                * prefix_lens must be off.  A token stands at position seqlens_k[b] - n + depth, where depth is the number of
+                                * bits of its row, those past n not counted, less one (0 for a row without any), for the bias and window_left,
+                                * which must reach over a chunk (max_seqlen_q - 1) */
+    int tree_words;            /* 1 ... FLASH_MAX_TREE_TOKENS / 64, 64 bits for each token of the longest chunk (max_seqlen_q) */
+    int64_t tree_stride;       /* words from row to row */
 } flash_paged_params;
+
+#define FLASH_MAX_SOFTCAP 1000.0f
+#define FLASH_MAX_TREE_TOKENS 256
 
 /* New rows of K, turned as by flash_rotary, and of V into their pages; Q, if it is given, turned into O by the same launch.  Rows whose place
  * is in front of key 0 or one that the table cannot name are not written.  Two tokens whose
@@ -273,15 +287,57 @@ int flash_append_paged(const flash_paged_params *p, void *stream);
 int flash_forward_paged(const flash_paged_params *p, void *stream);
 
 /* The split count that flash_forward_paged uses for p, and the bytes of its workspace (0 for one split).  They depend on the sizes (B, H, H_kv, d,
- * total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k), the masks and num_splits. */
+ * total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k), the masks (of prefix_lens and tree_mask: whether they are there, and tree_words) and num_splits. */
 int flash_forward_paged_resolve_splits(const flash_paged_params *p);
 int flash_forward_paged_workspace_bytes(const flash_paged_params *p, size_t *o_partial_bytes, size_t *lse_partial_bytes);
+
+/* Drafted tokens.  A step that checks a tree of them per sequence: count them into seqlens_k, flash_tree_mask, flash_append_paged with the positions,
+ * flash_forward_paged with the mask, choose a path by the model's answers, flash_keep_paged.  All index tensors are device memory, so that one captured
+ * graph serves all steps. */
+
+/* Masks and positions from the parents of a tree's tokens: row i of a sequence's n has the bits of the tokens on its path from the root, its own
+ * among them, and stands at seqlens_k[b] - n + (tokens on the path) - 1. */
+typedef struct flash_tree_params {
+    const int32_t *parents;       /* [total_q]: index of a token's parent within the chunk.  Parents stand in front of their children: a number that is
+                                   * not below the token's own, or below 0, is none, and the token hangs on the keys in front of the chunk */
+    const int32_t *cu_seqlens_q;  /* [B + 1], as in flash_paged_params */
+    const int32_t *seqlens_k;     /* [B], or NULL: positions count from the chunk's begin */
+    int64_t *mask;                /* [total_q], rows of `words` words (flash_paged_params::tree_mask) */
+    int32_t *positions;           /* [total_q], or NULL */
+    int B, total_q;
+    int words;                    /* 1 ... FLASH_MAX_TREE_TOKENS / 64.  Tokens from 64 * words on in a chunk get a row of zeroes and the chunk's begin */
+    int64_t mask_stride;          /* words from row to row, at least `words` */
+} flash_tree_params;
+
+int flash_tree_mask(const flash_tree_params *p, void *stream);
+
+/* Moves the rows of an accepted path to the chunk's begin: for i < accepted[b], row base + path[b][i] of sequence b's keys in K_cache and V_cache goes to
+ * row base + i, with base = seqlens_k[b] - n and n the chunk's tokens, and seqlens_out[b] = base + accepted[b].  Path numbers are below n and grow from entry to
+ * entry (parents stand in front of their children); a path ends in front of the first that does not, and seqlens_out says so.  Keys keep the positions
+ * that they were appended with, which flash_tree_mask's are right for.  Rows past seqlens_out are left as they are, and so are those on
+ * pages that the cache does not have. */
+typedef struct flash_keep_params {
+    void *K_cache, *V_cache;      /* [layers, num_pages, H_kv, page_size, d], any strides, not the same memory; fp16 or bf16 */
+    const int32_t *block_table, *seqlens_k, *cu_seqlens_q;   /* as in flash_paged_params, of all layers */
+    const int32_t *path;          /* [B, max_path] */
+    const int32_t *accepted;      /* [B], cut to 0 ... max_path */
+    int32_t *seqlens_out;         /* [B], none of the other tensors */
+    int B, H_kv, d, layers, num_pages, page_size, max_pages, max_path;   /* d: a multiple of 8 up to FLASH_MAX_HEAD_DIM */
+    int64_t kc_layer, kc_page, kc_head, kc_row, vc_layer, vc_page, vc_head, vc_row;   /* elements, multiples of 8 */
+    int64_t block_table_stride, path_stride;
+} flash_keep_params;
+
+int flash_keep_paged(const flash_keep_params *p, void *stream);
 
 /* Defaults: all pointers NULL, all sizes 0, factor 1, no window, num_splits 0 (paged).  And the sizes of the structs, as flash_params_size. */
 void flash_rotary_params_init(flash_rotary_params *p);
 void flash_paged_params_init(flash_paged_params *p);
+void flash_tree_params_init(flash_tree_params *p);
+void flash_keep_params_init(flash_keep_params *p);
 size_t flash_rotary_params_size(void);
 size_t flash_paged_params_size(void);
+size_t flash_tree_params_size(void);
+size_t flash_keep_params_size(void);
 
 /* Text of the last HIP error seen by this thread inside the library ("" if none). */
 const char *flash_last_hip_error(void);
