@@ -1,6 +1,7 @@
 // C entry points of rotary positions, of the paged cache and of drafted tokens (include/flash_attn_mi355.h): argument checks, split count, launches.
 #include "flash_attn_mi355.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -249,11 +250,22 @@ int splits_by_estimate(const flash_paged_params* p, int br, int nt)
 // outlast the others.  The merge reads 8 B H d bytes per split and token more, which is little next to the keys of a piece.  Its launch costs 3 us, in
 // which a work-group of 32 rows walks some tiles: shorter ranges stay whole.  Whole / in splits, single tokens, H 8, H_kv 2, one MI355X: d = 128
 // 256 keys 6.3 / 9.3 us, 512 keys 8.6 / 9.3, 1024 keys 13.6 / 9.2; d = 64, G = 1: 512 keys 6.3 / 9.5, 1024 keys 8.9 / 9.5, 2048 keys 14.7 / 9.1.
-constexpr int kFewestTiles = 32, kMostGroups = 2048, kWholeTiles = 8, kWholeTiles64 = 16;
-int splits_of(const flash_paged_params* p)
+constexpr long long kMostMerged = 1LL << 26;  // rows: the merge has a wave for each, and a launch is limited to 2^32 threads
+// splits of nt tiles, at most s, without empty ones
+int whole_pieces(int nt, long long s)
 {
-    const int br = rows_per_group(p), nt = most_tiles(p, br);
-    if (nt <= 1 || (long long)p->total_q * p->H >= 1LL << 26) return 1;  // (the merge has a wave per row: 2^32 threads)
+    if (s > nt) s = nt;
+    if (s > FLASH_MAX_SPLITS) s = FLASH_MAX_SPLITS;
+    if (s < 1) s = 1;
+    const int per = (int)((nt + s - 1) / s);
+    return (nt + per - 1) / per;
+}
+constexpr int kFewestRows = 16;  // fewer than half a row block: 32 rows whatever the scores
+constexpr int kFewestTiles = 32, kMostGroups = 2048, kWholeTiles = 8, kWholeTiles64 = 16;
+int splits_of(const flash_paged_params* p, int br)
+{
+    const int nt = most_tiles(p, br);
+    if (nt <= 1 || (long long)p->total_q * p->H >= kMostMerged) return 1;
     long long s = p->num_splits;
     if (s <= 0) {
         const long long groups = blocks_of(p, br) * p->H_kv;
@@ -271,11 +283,82 @@ int splits_of(const flash_paged_params* p)
             if (more > s) s = more;
         }
     }
-    if (s > nt) s = nt;
-    if (s > FLASH_MAX_SPLITS) s = FLASH_MAX_SPLITS;
-    if (s < 1) s = 1;
-    const int per = (int)((nt + s - 1) / s);
-    return (nt + per - 1) / per;
+    return whole_pieces(nt, s);
+}
+
+// ---- form and splits of launches with other scores and masks
+bool scored(const flash_paged_params* p) { return p->softcap > 0.0f || p->alibi_slopes || p->prefix_lens || p->tree_mask; }
+
+// Such launches have a third form, 128 rows, and their form and splits are those of a plain launch unless an estimate in us says that others
+// gain 2 % and more:
+//     begin + max(walk, load, bytes) + 0.2 min(walk, load) + [splits > 1] (merge + partial results)
+// walk: tiles of a piece, each `tile` long, `more` than that where work-groups share a CU (256 rows: where more than half of their waves have rows);
+// load: all row blocks' tiles, `unit` each where the GPU is full, and `slot` for the begin of each work-group in its place; bytes: all keys from memory; the
+// last two and a part of the last round of work-groups that is not.  Lengths are the host's: the longest, of which chunks of mixed lengths stand for
+// 0.79.  One MI355X, 1266 random launches of 11 us and more (trees, chunks, prompts, single tokens, all scores and masks; the constants were fitted
+// to half of them), against the fastest of all forms in 1 to 32 splits: 1.05 on average for either half, 1.3 or less in 97 of 100, worst 1.8; with
+// form and splits of plain launches 1.10, worst 2.45 (23 trees up to 128 on 17800 keys H4 d128 capped 238 -> 100 us).  Pieces by the lengths of all
+// sequences, worked out by every work-group, gained nothing over it on 120 launches.
+struct FormCost { int rows; double begin, tile, more, unit, slot; int places; };
+constexpr FormCost kForms[] = {{fa::kPagedFewRows, 5.0, 0.73, 0.18, 0.00165, 4.7, 2 * kNumCU},
+                               {fa::kPagedMidRows, 8.4, 1.3, 0.37, 0.0037, 3.0, 2 * kNumCU},
+                               {fa::kPagedTallRows, 10.3, 1.0, 0.29, 0.0055, 3.7, kNumCU}};
+constexpr double kNarrowTile = 0.69, kNarrowUnit = 0.61, kMixed = 0.79, kMergeUs = 4.8, kMergeTimes = 1.23, kCapped = 1.05, kRound = 0.24, kBytesRound = 0.5, kBoth = 0.2;
+constexpr double kKeyBytesPerUs = 1e7;  // (of lengths that are shorter than the longest)
+constexpr double kGain = 0.98, kSoonest = 8.0;  // (us: no other can be much faster)
+
+struct Estimate {
+    int nt, places;
+    bool full;  // (256 rows)
+    double begin, tile, more, groups, load, slot, bytes, merge;
+    Estimate(const flash_paged_params* p, const FormCost& f)
+    {
+        nt = std::max(most_tiles(p, f.rows), 1);
+        const long long chunk = longest_chunk(p), keys = keys_of(p), G = group_of(p);
+        const bool mixed = p->total_q < (long long)p->B * chunk, narrow = p->d <= 64;
+        const double share = mixed && p->B > 1 ? kMixed : 1.0, capped = p->softcap > 0.0f ? kCapped : 1.0;
+        double tiles = nt;  // of the mean row block
+        if (causal_of(p) && chunk > 1 && window_left_of(p) < 0) tiles = std::max(1.0, std::min(tiles, (keys - 0.5 * chunk) / 64 + 1));
+        const double blocks = std::min((double)p->B * (double)((chunk * G + f.rows - 1) / f.rows), (double)p->total_q * G / f.rows + (mixed ? 0.5 : 1.0) * p->B);
+        groups = blocks * p->H_kv * tiles * share / nt;
+        load = groups * nt * f.unit * (narrow ? kNarrowUnit : 1.0) * capped;
+        bytes = share * p->B * p->H_kv * nt * 256.0 * p->d / kKeyBytesPerUs;
+        begin = f.begin, slot = f.slot, places = f.places, full = f.rows == fa::kPagedTallRows && chunk * G > f.rows / 2;
+        tile = f.tile * (narrow ? kNarrowTile : 1.0) * capped, more = f.more * (narrow ? kNarrowTile : 1.0) * capped;
+        merge = kMergeTimes * share * 8.0 * p->d * p->total_q * p->H / kPartialBytesPerUs;
+    }
+    double us(int splits) const
+    {
+        const double n = groups * splits, per = (nt + splits - 1) / splits;
+        const double walk = per * (tile + (full || (places > kNumCU && n > kNumCU) ? more : 0.0));
+        const double rest = n > places ? std::ceil(n / places) * places / n - 1 : 0.0;
+        const double all = std::max((load + n * slot / places) * (1 + kRound * rest), bytes * (1 + kBytesRound * rest));
+        const double us = begin + std::max(walk, all) + kBoth * std::min(walk, all);
+        return splits > 1 ? us + kMergeUs + merge * splits : us;
+    }
+};
+
+struct Plan { int rows, splits; };
+Plan plan_of(const flash_paged_params* p)
+{
+    Plan plan = {rows_per_group(p), 1};
+    plan.splits = splits_of(p, plan.rows);
+    if (!scored(p) || p->total_q == 0) return plan;
+    const FormCost& now = kForms[plan.rows == fa::kPagedFewRows ? 0 : 2];
+    double best = kGain * Estimate(p, now).us(plan.splits);
+    if (best <= kSoonest) return plan;
+    for (const FormCost& f : kForms) {
+        if (f.rows != fa::kPagedFewRows && (long long)longest_chunk(p) * group_of(p) <= kFewestRows) break;
+        const Estimate e(p, f);
+        for (const int count : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32}) {
+            const int s = whole_pieces(e.nt, p->num_splits > 0 ? p->num_splits : count);
+            if (s > 1 && (long long)p->total_q * p->H >= kMostMerged) break;
+            const double us = e.us(s);
+            if (us < best) best = us, plan = {f.rows, s};
+            if (p->num_splits > 0 || count >= e.nt) break;
+        }
+    }
+    return plan;
 }
 
 // Whether the row blocks of all sequences are started by the end of their keys, heaviest first under a causal mask, instead of sequence by sequence:
@@ -323,7 +406,8 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     if ((rc = rows_strides(p->q_token, p->q_head, p->Q)) != FLASH_OK || (rc = rows_strides(p->o_token, p->o_head, p->O)) != FLASH_OK) return rc;
     if (!p->LSE || !apart(p->o_token, p->o_head, p->total_q, p->H)) return FLASH_EINVAL;
     if (misaligned(p->LSE, 4)) return FLASH_EALIGN;
-    const int br = rows_per_group(p), splits = splits_of(p), nt = most_tiles(p, br);
+    const Plan plan = plan_of(p);
+    const int br = plan.rows, splits = plan.splits, nt = most_tiles(p, br);
     if (splits > 1) {
         if (!p->O_partial || !p->LSE_partial) return FLASH_EWORKSPACE;
         if (misaligned(p->O_partial, 16) || misaligned(p->LSE_partial, 4)) return FLASH_EALIGN;
@@ -350,7 +434,7 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     a.by_heads = fa::fast_div(a.Hk), a.by_group = fa::fast_div(a.G), a.by_page = fa::fast_div(a.page);
     a.by_splits = fa::fast_div(splits);
     const bool bf16 = p->dtype == FLASH_BF16;
-    if (p->softcap > 0.0f || p->alibi_slopes || p->prefix_lens || p->tree_mask) rc = record_hip(launch_scored(p, a, br, blocks, st));
+    if (scored(p)) rc = record_hip(launch_scored(p, a, br, blocks, st));
     else rc = record_hip(p->d <= 64 ? fa::launch_paged_d64(a, bf16, br, blocks, st) : fa::launch_paged_d128(a, bf16, br, blocks, st));
     if (rc != FLASH_OK || splits == 1) return rc;
     return record_hip(fa::launch_paged_merge(a, bf16, st));
@@ -468,7 +552,7 @@ FLASH_EXPORT int flash_forward_paged_resolve_splits(const flash_paged_params* p)
     int rc = validate_paged(p, &empty);
     if (rc == FLASH_OK) rc = validate_scores(p);
     if (rc != FLASH_OK) return rc;
-    return empty ? 1 : splits_of(p);
+    return empty ? 1 : plan_of(p).splits;
 }
 
 FLASH_EXPORT int flash_forward_paged_workspace_bytes(const flash_paged_params* p, size_t* o_partial_bytes, size_t* lse_partial_bytes)
@@ -477,7 +561,7 @@ FLASH_EXPORT int flash_forward_paged_workspace_bytes(const flash_paged_params* p
     int rc = validate_paged(p, &empty);
     if (rc == FLASH_OK) rc = validate_scores(p);
     if (rc != FLASH_OK) return rc;
-    const int splits = empty ? 1 : splits_of(p);
+    const int splits = empty ? 1 : plan_of(p).splits;
     const size_t rows = splits > 1 ? (size_t)p->total_q * p->H * splits : 0;
     if (o_partial_bytes) *o_partial_bytes = rows * p->d * sizeof(float);
     if (lse_partial_bytes) *lse_partial_bytes = rows * sizeof(float);

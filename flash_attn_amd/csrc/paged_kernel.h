@@ -42,7 +42,7 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
-constexpr int kPagedTallRows = 256, kPagedFewRows = 32;  // rows of a work-group
+constexpr int kPagedTallRows = 256, kPagedMidRows = 128, kPagedFewRows = 32;  // rows of a work-group
 constexpr int paged_threads(int rows) { return rows == kPagedTallRows ? 512 : 256; }
 
 struct PagedArgs {
@@ -69,6 +69,13 @@ struct PagedArgs {
 enum { kScoresPlain, kScoresMasked, kScoresCapped, kScoresSloped, kScoresBoth };  // kScoresMasked: a prefix or a tree alone, which all but kScoresPlain take
 constexpr bool has_cap(int scores) { return scores == kScoresCapped || scores == kScoresBoth; }
 constexpr bool has_slopes(int scores) { return scores == kScoresSloped || scores == kScoresBoth; }
+
+// With a bias by distance the tiles come last first: the nearest keys' scores are the largest, and the running maximum hardly ever moves behind them, where from
+// the front it is raised, and O scaled, tile by tile (six prompts up to 2048 H16 d64 53.7 -> 49.5 us).
+constexpr bool last_first(int scores) { return has_slopes(scores); }
+// Tile of the range that comes in place t, for places past the end too
+template <int kScores>
+__device__ __forceinline__ int tile_of(int t, int ntiles) { return last_first(kScores) ? max(ntiles - 1 - t, 0) : t; }
 
 constexpr int kTreeTokens = 256;  // drafted tokens of a sequence that a mask can name
 struct ScoredArgs : PagedArgs {
@@ -454,6 +461,20 @@ __device__ __forceinline__ v8h k_fragment(uint32_t kbase, int ks, int kb)
     return *reinterpret_cast<FA_LDS const v8h*>(lds_at(kbase ^ (uint32_t)(ks << 5)) + kb * (32 * PagedTile<D>::ROW));
 }
 
+// Reads of LDS and MFMAs in turn, kAhead fragments (of kReads reads each) in front: left to itself the compiler waits for every fragment where it is used, 120
+// cycles for an MFMA of 32.  Stands behind the code that it orders.
+template <int kFragments, int kReads, int kAhead, bool kFirstAreThere = false>
+__device__ __forceinline__ void order_reads_and_mfmas()
+{
+    constexpr int ahead = kAhead < kFragments ? kAhead : kFragments;
+    if constexpr (!kFirstAreThere) __builtin_amdgcn_sched_group_barrier(0x100, kReads * ahead, 0);
+#pragma unroll
+    for (int x = 0; x < kFragments; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (x + ahead < kFragments) __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+    }
+}
+
 constexpr float kPagedTau = 8.0f;                       // powers of two by which a row may outgrow its running maximum
 constexpr float kPagedNothing = -3.402823466e38f;       // running maximum of a row that has seen no key
 
@@ -462,7 +483,9 @@ constexpr float kPagedNothing = -3.402823466e38f;       // running maximum of a 
 template <bool kBf16, int MB, int KB>
 struct PagedSoftmax {
     float m_ref = kPagedNothing, m_thr = -INFINITY, l_run = 0.0f;
-    __device__ __forceinline__ void tile(v16f (&s)[KB], v16f (&oacc)[MB], uint32_t (&p)[KB][2][4], float c2, float inv_c2, int sides, int lo_rel, int hi_rel)
+    // kOffset: all scores of the row are larger by `off`
+    template <bool kOffset = false>
+    __device__ __forceinline__ void tile(v16f (&s)[KB], v16f (&oacc)[MB], uint32_t (&p)[KB][2][4], float c2, float inv_c2, int sides, int lo_rel, int hi_rel, float off = 0.0f)
     {
         if (__builtin_expect(sides != 0, 0)) {
             if constexpr (KB == 2) {
@@ -482,7 +505,8 @@ struct PagedSoftmax {
         for (int r = 0; r < 16; ++r)
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) mk[kb] = fmaxf(mk[kb], s[kb][r]);
-        const float mx = fmaxf(mk[0], mk[KB - 1]);
+        float mx = fmaxf(mk[0], mk[KB - 1]);
+        if constexpr (kOffset) mx += off;
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m_thr) != 0ull, 0)) {
             const float m_new = fmaxf(m_ref, xhalf_max(mx) * c2);  // c2 > 0
             float alpha = fast_exp2(m_ref - m_new);
@@ -495,12 +519,13 @@ struct PagedSoftmax {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) oacc[mb][r] *= alpha;
         }
-        float rs = 0.0f;
+        float rs = 0.0f, from = m_ref;
+        if constexpr (kOffset) from = __builtin_fmaf(-off, c2, m_ref);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                const float p0 = fast_exp2(__builtin_fmaf(s[kb][r], c2, -m_ref)), p1 = fast_exp2(__builtin_fmaf(s[kb][r + 1], c2, -m_ref));
+                const float p0 = fast_exp2(__builtin_fmaf(s[kb][r], c2, -from)), p1 = fast_exp2(__builtin_fmaf(s[kb][r + 1], c2, -from));
                 rs = kb == 0 && r == 0 ? p0 + p1 : rs + p0 + p1;
                 p[kb][r >> 3][(r & 7) >> 1] = Elem<kBf16>::pack(p0, p1);
             }
@@ -515,7 +540,8 @@ struct PagedSoftmax {
 // instructions and a subtraction per score in front of the usual fma and exp2, 24 cycles of a SIMD beside the 24 that a plain score takes and the 32 of its
 // MFMAs at d = 128.  t is off by at most 3 half steps of 2^-24 (v_exp_f32, the subtraction and v_rcp_f32 one each), a score by 6 c 2^-24; a
 // polynomial for small z that stays relative takes as many cycles (measured: v_exp_f32 and v_rcp_f32 8 cycles a wave, other instructions 4).
-// A bias by distance, slope |p - j|, is the C operand of the scores' first MFMA, one instruction per score; behind a cap it is added to t.
+// A bias by distance, -slope |p - j|, begins as slope (j - p), which a product of its own and an offset of the tile work out; tiles with keys that stand
+// otherwise and may be seen get the difference.  Behind a cap it is added to t, one instruction per score.
 // A tree's tokens see the keys in front of the chunk, and of the chunk's those whose bit is set; they stand at the chunk's begin plus their depth, the number
 // of tokens that they see in the chunk less one.  The masks of the sequence's tokens and the depths lie in LDS; all they touch is the last tile or
 // the last few of a sequence, which take a mask of 64 bits per row.
@@ -527,20 +553,29 @@ struct TreeTable {
 };
 constexpr int kTreeLds = kTreeTokens * (kTreeTokens / 64) * 8 + kTreeTokens * 4;
 
-// Called by all threads of the work-group; a.tree is there.
+// Word w of the mask of the chunk's token i, of n: bits of tokens that there are not cleared
+__device__ __forceinline__ uint64_t tree_word(const ScoredArgs& a, const PagedItem& it, int i, int w, int n)
+{
+    const int left = n - 64 * w;
+    const uint64_t there = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+    return a.tree[(int64_t)(it.tok0 + i) * a.tree_stride + w] & there;
+}
+
+// Called by all threads of a work-group whose keys reach the chunk's own, where there is a tree: behind the requests for its first tiles, so that what
+// is loaded here is on its way together with them.  depths: whether they are asked for
 template <int kThreads>
-__device__ __forceinline__ void tree_setup(const ScoredArgs& a, const PagedItem& it, int tid, FA_LDS char* lds, TreeTable* tree)
+__device__ __forceinline__ void tree_setup(const ScoredArgs& a, const PagedItem& it, int tid, FA_LDS char* lds, bool depths, TreeTable* tree)
 {
     const int W = a.tree_words, n = min(it.len - it.shift, 64 * W);
     tree->words = (FA_LDS uint64_t*)lds;
     tree->depth = (FA_LDS int*)(lds + kTreeTokens * (kTreeTokens / 64) * 8);
     tree->tokens = n;
     for (int k = tid; k < n * W; k += kThreads) {
-        const int i = (int)((uint32_t)k / (uint32_t)W), w = k - i * W, left = n - 64 * w;  // (bits of tokens that there are not)
-        const uint64_t there = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
-        tree->words[k] = a.tree[(int64_t)(it.tok0 + i) * a.tree_stride + w] & there;
+        const int i = (int)((uint32_t)k / (uint32_t)W);
+        tree->words[k] = tree_word(a, it, i, k - i * W, n);
     }
     __syncthreads();
+    if (!depths) return;
     for (int i = tid; i < n; i += kThreads) {
         int c = -1;
         for (int w = 0; w < W; ++w) c += __builtin_popcountll(tree->words[i * W + w]);
@@ -562,10 +597,11 @@ struct RowScores {
     TreeTable tree;
     int token, base;      // its index in the chunk; the chunk's first key
     int kmin, kmax;       // keys of the work-group
-    int place, place_min; // position, and one that no row of the wave is in front of
+    int place;            // position
+    int bent;             // first key whose bias may not be slope (key - place)
     float slope;
 
-    // keys [lo, hi] that row r sees, but for the chunk's own of a tree
+    // keys [lo, hi] that row r sees, but for the chunk's own of a tree, whose table must be there where the work-group's keys reach them
     __device__ __forceinline__ void set(const ScoredArgs& a, const PagedItem& it, int r, int kmin_, int kmax_, int* lo, int* hi)
     {
         const int rr = r < it.rows ? r : it.rows - 1, i = a.by_group.quotient(rr);
@@ -573,7 +609,13 @@ struct RowScores {
         place = i + it.shift;
         int l = kmin, h = kmax - 1;
         if (a.tree) {
-            place = base + (i < tree.tokens ? tree.depth[i] : 0);
+            place = base;
+            const int n = min(it.len - it.shift, 64 * a.tree_words);
+            if ((has_slopes(kScores) || a.wl >= 0) && i < n) {
+                int c = -1;
+                for (int w = 0; w < a.tree_words; ++w) c += __builtin_popcountll(tree_word(a, it, i, w, n));
+                place += max(c, 0);
+            }
             h = min(h, base - 1);
         }
         if (a.wl >= 0) l = max(l, place - a.wl);
@@ -584,7 +626,8 @@ struct RowScores {
         *hi = h;
         if constexpr (has_slopes(kScores)) {
             slope = a.slopes[it.hk * a.G + (rr - i * a.G)] * a.slope_unit;
-            place_min = a.tree ? base : __builtin_amdgcn_readfirstlane(place);
+            if constexpr (!has_cap(kScores)) set_slant(threadIdx.x & 31, (threadIdx.x & 63) >> 5);
+            bent = a.tree ? base : a.causal && !a.prefix ? 0x7fffffff : __builtin_amdgcn_readfirstlane(place) + 1;  // (under a causal mask alone nobody sees one)
         }
     }
     // the chunk's own keys among the 64 from kb0 on that the row sees
@@ -606,34 +649,53 @@ struct RowScores {
         if (a.tree && j >= base) at = base + (j - base < tree.tokens ? tree.depth[j - base] : 0);
         return (float)(at - place);
     }
-    // Bias of the tile at kb0, or what is added to it (C operands of 32 keys and 32 rows; g: lane / 32)
-    template <int KB, bool kAdd>
-    __device__ __forceinline__ void bias(const ScoredArgs& a, v16f (&s)[KB], int kb0, int g) const
+    // Bias of keys in front of the row, slope (key - place): the tile's part, slope (kb0 - place), is the softmax's offset; what the keys' places in the tile
+    // add comes out of a product of its own, 16 columns of which three are used: the slope in three parts of eight bits (bf16, whatever the caches hold)
+    // times the place, 0 ... 63, which is exact.  One MFMA per 32 keys, 32 cycles, where sixteen additions per lane would take 64 of the softmax's.
+    v8h q_slant, k_slant[2];
+    __device__ __forceinline__ void set_slant(int l32, int g)
     {
-        const int k0 = kb0 + 4 * g;
-        auto put = [&](int kb, int r, float b) __attribute__((always_inline)) {
-            if constexpr (kAdd) s[kb][r] += b;
-            else s[kb][r] = b;
-        };
-        if (__builtin_expect(kb0 + 32 * KB - 1 <= place_min && (!a.tree || kb0 + 32 * KB <= base), 1)) {  // all keys in front of all rows
-            const float b0 = slope * (float)(k0 - place);
+        const float hi = Elem<true>::low(Elem<true>::pack(slope, slope)), mid = Elem<true>::low(Elem<true>::pack(slope - hi, slope - hi)), lo = slope - hi - mid;
+        const float on = g == 0 ? 1.0f : 0.0f;
+        const uint32_t q[4] = {Elem<true>::pack(hi * on, mid * on), Elem<true>::pack(lo * on, 0.0f), 0u, 0u};
+        q_slant = fragment_of(q);
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) put(kb, r, __builtin_fmaf(slope, (float)(32 * kb + 8 * (r >> 2) + (r & 3)), b0));
-        } else if (!a.tree || kb0 + 32 * KB <= base) {
-            const float x0 = (float)(k0 - place);
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) put(kb, r, -slope * __builtin_fabsf(x0 + (float)(32 * kb + 8 * (r >> 2) + (r & 3))));
-        } else {
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) put(kb, r, -slope * __builtin_fabsf(distance(a, k0 + 32 * kb + 8 * (r >> 2) + (r & 3))));
+        for (int kb = 0; kb < 2; ++kb) {
+            const float key = (float)(l32 + 32 * kb) * on;
+            const uint32_t k[4] = {Elem<true>::pack(key, key), Elem<true>::pack(key, 0.0f), 0u, 0u};
+            k_slant[kb] = fragment_of(k);
         }
     }
+    __device__ __forceinline__ v16f slant(int kb) const
+    {
+        const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        return Elem<true>::mfma(k_slant[kb], q_slant, z);
+    }
+    static __device__ __forceinline__ v8h fragment_of(const uint32_t (&p)[4])
+    {
+        const v4u t = {p[0], p[1], p[2], p[3]};
+        return __builtin_bit_cast(v8h, t);
+    }
+    // (behind a cap the two halves of the lanes, whose keys are 4 apart, have offsets of their own: the larger score of a row is looked for with them)
+    __device__ __forceinline__ float offset(int kb0, int g) const
+    {
+        return !has_slopes(kScores) ? 0.0f : has_cap(kScores) ? slope * (float)(kb0 + 4 * g - place) : slope * (float)(kb0 - place);
+    }
+    // ... and what makes it that of the others, as far as a row may see them: keys behind it, and a tree's, which stand at their depths
+    template <int KB>
+    __device__ __forceinline__ void bend(const ScoredArgs& a, v16f (&s)[KB], int kb0, int g) const
+    {
+        const int k0 = kb0 + 4 * g;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int key = k0 + 32 * kb + 8 * (r >> 2) + (r & 3);
+                s[kb][r] -= slope * (__builtin_fabsf(distance(a, key)) + (float)(key - place));  // (0 for the others)
+            }
+    }
+    // t of a product
+    __device__ __forceinline__ float capped(const ScoredArgs& a, float s) const { return __builtin_amdgcn_rcpf(-1.0f - fast_exp2(s * a.cap_in)); }
     // From products to what the softmax goes by, masks applied.  sides: as in PagedSoftmax::tile
     template <int KB>
     __device__ __forceinline__ void finish(const ScoredArgs& a, v16f (&s)[KB], int kb0, int g, int sides, int lo, int hi) const
@@ -642,9 +704,15 @@ struct RowScores {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_amdgcn_rcpf(-1.0f - fast_exp2(s[kb][r] * a.cap_in));
-            if constexpr (has_slopes(kScores)) bias<KB, true>(a, s, kb0, g);
+                for (int r = 0; r < 16; ++r) s[kb][r] = capped(a, s[kb][r]);
+            if constexpr (has_slopes(kScores)) {  // (to t, and the lane's 4 g)
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(slope, (float)(32 * kb + 8 * (r >> 2) + (r & 3)), s[kb][r]);
+            }
         }
+        if (has_slopes(kScores) && __builtin_expect(kb0 + 32 * KB > bent, 0)) bend(a, s, kb0, g);
         if (__builtin_expect(sides != 0, 0)) {
             if (a.tree) {
                 const uint64_t seen = (range_bits(lo - kb0, hi - kb0) | drafted_bits(a, kb0)) >> (4 * g);
@@ -668,7 +736,7 @@ struct RowScores {
     // The same of one key's product, unmasked
     __device__ __forceinline__ float one(const ScoredArgs& a, float s, int j) const
     {
-        if constexpr (has_cap(kScores)) s = __builtin_amdgcn_rcpf(-1.0f - fast_exp2(s * a.cap_in));
+        if constexpr (has_cap(kScores)) s = capped(a, s);
         if constexpr (has_slopes(kScores)) s -= slope * __builtin_fabsf(distance(a, j));
         return s;
     }
@@ -853,8 +921,6 @@ __device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
     const int tile0 = kmin / BC, ntiles = (kmax + BC - 1) / BC - tile0;
     const int len = it.len;
     RowScores<kScores> row;
-    if constexpr (kScores != kScoresPlain)
-        if (a.tree) tree_setup<256>(a, it, tid, (FA_LDS char*)smem + C::SMEM, &row.tree);
     const int32_t* const table_row = a.table + (size_t)it.b * a.table_stride;
 
     FA_LDS char* const kst = (FA_LDS char*)smem + wave * C::WAVE;
@@ -883,14 +949,25 @@ __device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
     PagedPlace place[GROUPS];  // of the tile to request next
     auto ask = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < GROUPS; ++s) place[s].ask(a, table_row, len, (tile0 + t) * BC + 16 * s);
+        for (int s = 0; s < GROUPS; ++s) place[s].ask(a, table_row, len, (tile0 + tile_of<kScores>(t, ntiles)) * BC + 16 * s);
     };
     // the rows of tile t (its places asked for) of K or V
     auto request = [&](auto is_v_c, int t, const char* head, uint32_t page_bytes, uint32_t row_bytes, const uint32_t (&off)[kPer], const bool (&ok)[kPer],
                        FA_LDS char* dst) __attribute__((always_inline)) {
         constexpr bool kIsV = decltype(is_v_c)::value;
-        const int kb0 = (tile0 + t) * BC;
+        const int kb0 = (tile0 + tile_of<kScores>(t, ntiles)) * BC;
         const bool whole = kb0 + BC <= len;
+        if constexpr (kScores != kScoresPlain) {
+            if (__builtin_expect(whole && a.d == D, 1)) {  // (nearly all tiles: no branch per request)
+#pragma unroll
+                for (int s = 0; s < GROUPS; ++s) {
+                    const char* const at = place[s].in(a, head, page_bytes, row_bytes);
+#pragma unroll
+                    for (int x = 0; x < kPer; ++x) dma_kib_nt(at, off[x], dst + (s * kPer + x) * 1024);
+                }
+                return;
+            }
+        }
 #pragma unroll
         for (int s = 0; s < GROUPS; ++s) {
             const char* const at = place[s].in(a, head, page_bytes, row_bytes);
@@ -924,22 +1001,28 @@ __device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
 
     int lo, hi;
     if constexpr (kScores == kScoresPlain) paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
-    else row.set(a, it, r, kmin, kmax, &lo, &hi);
+    else lo = hi = 0;
     int lo_max = lo, hi_min = hi;
     if (wave < ntiles) {
         ask(wave);
         load_q<KS>(a, it, r, g, qf);
         request_k(wave);
         request_v(wave);
-        lo_max = __builtin_amdgcn_readlane(lo, 31);  // (bounds do not fall from row to row)
+        if constexpr (kScores == kScoresPlain) {
+            lo_max = __builtin_amdgcn_readlane(lo, 31);  // (bounds do not fall from row to row)
+            hi_min = __builtin_amdgcn_readlane(hi, 0);
+        }
+    }
+    if constexpr (kScores != kScoresPlain) {
+        if (a.tree && kmax > it.shift) tree_setup<256>(a, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
+        row.set(a, it, r, kmin, kmax, &lo, &hi);
+        lo_max = a.tree ? -rows_min(-lo) : __builtin_amdgcn_readlane(lo, 31);  // (a tree's bounds may fall)
         hi_min = __builtin_amdgcn_readlane(hi, 0);
-        if constexpr (kScores != kScoresPlain)
-            if (a.tree) lo_max = -rows_min(-lo);  // (but a tree's do)
     }
     const float c2 = a.scale_log2, inv_c2 = __builtin_amdgcn_rcpf(c2);
     const int k_rd = T::k_lane(lane), v_rd = T::v_lane(lane);
     for (int t = wave; t < ntiles; t += 4) {
-        const int kb0 = (tile0 + t) * BC;
+        const int kb0 = (tile0 + tile_of<kScores>(t, ntiles)) * BC;
         const bool more = t + 4 < ntiles;
         if (more) ask(t + 4);
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");  // K of this tile is there
@@ -951,12 +1034,17 @@ __device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
         {
             const uint32_t kbase = fragment_base(kst, k_rd);
             const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-            if constexpr (kScores == kScoresSloped) row.template bias<KB, false>(a, s, kb0, g);
+            if constexpr (kScores == kScoresSloped) {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) s[kb] = row.slant(kb);
+            }
+            if constexpr (kScores != kScoresPlain) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
                     s[kb] = Elem<kBf16>::mfma(k_fragment<D>(kbase, ks, kb), qf[ks], ks == 0 && kScores != kScoresSloped ? z : s[kb]);
+            if constexpr (kScores != kScoresPlain) order_reads_and_mfmas<KS * KB, 1, 6>();
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the fragments have been read
         if (more) request_k(t + 4);
@@ -966,22 +1054,24 @@ __device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
             soft.tile(s, oacc, p, c2, inv_c2, sides, lo - kb0 - 4 * g, hi - kb0 - 4 * g);
         } else {
             row.finish(a, s, kb0, g, sides, lo, hi);
-            soft.tile(s, oacc, p, c2, inv_c2, 0, 0, 0);
+            soft.template tile<has_slopes(kScores)>(s, oacc, p, c2, inv_c2, 0, 0, 0, row.offset(kb0, g));
         }
         if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         {
             const uint32_t vbase = fragment_base(vst, v_rd);
+            if constexpr (kScores != kScoresPlain) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int st = 0; st < 2 * KB; ++st)
 #pragma unroll
                 for (int mb = 0; mb < MB; ++mb) oacc[mb] = Elem<kBf16>::mfma(v_fragment<D>(vbase, st, mb), as_fragment(p[st >> 1][st & 1]), oacc[mb]);
+            if constexpr (kScores != kScoresPlain) order_reads_and_mfmas<2 * KB * MB, 2, 4>();
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more) request_v(t + 4);
     }
     if (wave < ntiles && __builtin_expect(any_not_finite<MB>(oacc), 0))
-        paged_rescue<BC, MB, kBf16, kScores>(a, it, r, kmin, kmax, tile0, ntiles, wave, 4, soft.m_ref, oacc, row);
+        paged_rescue<BC, MB, kBf16, kScores>(a, it, r, kmin, kmax, tile0, ntiles, last_first(kScores) ? (ntiles - 1 - wave) & 3 : wave, 4, soft.m_ref, oacc, row);
 
     // ---- merge of the four waves: reference of a row = the largest of theirs
     const int nrows = min(kPagedFewRows, it.rows - it.row0);
@@ -1100,6 +1190,20 @@ struct PagedRequests {
     {
 #pragma unroll
         for (int x = 0; x < NL; ++x) request(t, x, place[x].in(a, Kh, a.k_page, a.k_row), a.k_row, koff, kok, stage);
+    }
+    // Tile t of K and V, branches once for all requests: tiles that are not the last, rows without a gap behind them
+    __device__ __forceinline__ void load(const PagedArgs& a, int t, FA_LDS char* k_stage, FA_LDS char* v_stage)
+    {
+        if (__builtin_expect((tile0 + t + 1) * T::BC <= len && a.d == D, 1)) {
+#pragma unroll
+            for (int x = 0; x < NL; ++x) dma_kib(place[x].in(a, Kh, a.k_page, a.k_row), koff, k_stage + (wave + kWaves * x) * 1024);
+#pragma unroll
+            for (int x = 0; x < NL; ++x) dma_kib(place[x].in(a, Vh, a.v_page, a.v_row), voff, v_stage + (wave + kWaves * x) * 1024);
+        } else {
+            load_k(a, t, k_stage);
+            find_v(a);
+            load_v(a, t, v_stage);
+        }
     }
     __device__ __forceinline__ void find_v(const PagedArgs& a)
     {
@@ -1256,16 +1360,11 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
     RowScores<kScores> row;
     if constexpr (kScores == kScoresPlain) {
         paged_bounds(a, it, r, kmin, kmax, &lo, &hi);
-    } else {
-        if (a.tree) tree_setup<512>(a, it, tid, (FA_LDS char*)smem + C::SMEM, &row.tree);
-        row.set(a, it, r, kmin, kmax, &lo, &hi);
+        lo_min = __builtin_amdgcn_readlane(lo, 0);
+        hi_min = __builtin_amdgcn_readlane(hi, 0);
+        lo_max = __builtin_amdgcn_readlane(lo, 31);  // (bounds do not fall from row to row)
+        hi_max = __builtin_amdgcn_readlane(hi, 31);
     }
-    lo_min = __builtin_amdgcn_readlane(lo, 0);
-    hi_min = __builtin_amdgcn_readlane(hi, 0);
-    lo_max = __builtin_amdgcn_readlane(lo, 31);  // (bounds do not fall from row to row)
-    hi_max = __builtin_amdgcn_readlane(hi, 31);
-    if constexpr (kScores != kScoresPlain)
-        if (a.tree) lo_min = rows_min(lo), lo_max = -rows_min(-lo), hi_max = kmax - 1;  // (but a tree's do)
 
     v8h qf[KS];
     v16f oacc[MB], s[2];
@@ -1298,17 +1397,18 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) s[kb] = E::mfma(kf[ks][kb], qf[ks], s[kb]);
     };
-    auto s_clear = [&](int kb0) __attribute__((always_inline)) {  // kb0: of the tile whose scores come next
-        if constexpr (kScores == kScoresSloped) {
-            row.template bias<2, false>(a, s, kb0, g);
-        } else {
+    auto s_clear = [&]() {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb) {
+            if constexpr (kScores == kScoresSloped) {
+                s[kb] = row.slant(kb);
+            } else {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[kb][e] = 0.0f;
+            }
         }
     };
-    auto mfma_phase = [&](auto last_c, uint32_t vbase, uint32_t kbase, int kb0) __attribute__((always_inline)) {
+    auto mfma_phase = [&](auto last_c, uint32_t vbase, uint32_t kbase) __attribute__((always_inline)) {
         constexpr bool kLast = decltype(last_c)::value;
         // step st: reads of V step st + VPD (behind the last ones: of K), MFMAs of step st
         pv_mfma(0);
@@ -1323,7 +1423,7 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
             pv_mfma(st);
         }
         if constexpr (!kLast) {
-            s_clear(kb0 + BC);
+            s_clear();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if (ks + KPD < KS) k_read(kbase, ks + KPD);
@@ -1337,6 +1437,7 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
             __builtin_amdgcn_sched_group_barrier(0x008, MB, 0);
         }
         if constexpr (!kLast) {
+            if constexpr (kScores == kScoresSloped) __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if (ks + KPD < KS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
@@ -1347,9 +1448,9 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
     // what has to have landed at the end of iteration t, and the requests for what is to come
     auto tail_requests = [&](int t, FA_LDS char* wrk) __attribute__((always_inline)) {
         if (t + 3 < ntiles) {
-            req.load_k(a, t + 3, wrk);
+            req.load_k(a, tile_of<kScores>(t + 3, ntiles), wrk);
             req.find_v(a);
-            req.ask(a, t + 4);
+            req.ask(a, tile_of<kScores>(t + 4, ntiles));
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1357,13 +1458,13 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
     };
     auto iteration = [&](auto last_c, FA_LDS const char* __restrict__ rdv, FA_LDS const char* __restrict__ rdk, FA_LDS char* __restrict__ wrk,
                          FA_LDS char* __restrict__ wrv, int t) __attribute__((always_inline)) {
-        const int kb0 = (tile0 + t) * BC;
-        if (t + 2 < ntiles) req.load_v(a, t + 2, wrv);
+        const int kb0 = (tile0 + tile_of<kScores>(t, ntiles)) * BC;
+        if (t + 2 < ntiles) req.load_v(a, tile_of<kScores>(t + 2, ntiles), wrv);
         if constexpr (kScores == kScoresPlain) {
             soft.tile(s, oacc, p, c2, inv_c2, mask_sides(kb0, lo_max, hi_min), lo - kb0 - 4 * g, hi - kb0 - 4 * g);
         } else {
             row.finish(a, s, kb0, g, mask_sides(kb0, lo_max, hi_min), lo, hi);
-            soft.tile(s, oacc, p, c2, inv_c2, 0, 0, 0);
+            soft.template tile<has_slopes(kScores)>(s, oacc, p, c2, inv_c2, 0, 0, 0, row.offset(kb0, g));
         }
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t vbase = fragment_base(rdv, v_rd);
@@ -1373,7 +1474,7 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
         v_read(vbase, 1);
         paged_barrier_keep<2 * VPD * MB>();
         __builtin_amdgcn_s_setprio(1);
-        mfma_phase(last_c, vbase, kbase, kb0);
+        mfma_phase(last_c, vbase, kbase);
         __builtin_amdgcn_s_setprio(0);
         tail_requests(t, wrk);
         paged_barrier();
@@ -1385,7 +1486,7 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
     // 256 rows on 512 keys, B 128, H 8, d = 128 106.2 -> 103.0 us, 2048 rows, B 2, H 16, d = 80 51.8 -> 50.6 us.  What is
     // left before the first scores, about 3 us, is these bytes' way from L2 into the CU: the page numbers of all three tiles asked
     // for at once changed nothing.
-    req.ask(a, 0);
+    req.ask(a, tile_of<kScores>(0, ntiles));
     FA_LDS char* const qst = wave < 2   ? Ks + 2 * NST * T::BUF + wave * C::QBUF
                              : wave < 4 ? Vs + 2 * T::BUF + (wave - 2) * C::QBUF
                              : wave < 6 ? Ks + 3 * T::BUF + (wave - 4) * C::QBUF
@@ -1400,13 +1501,22 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
 #pragma unroll
     for (int t = 0; t < 3; ++t) {
         if (t < ntiles) {
-            if (t > 0) req.ask(a, t);
-            req.load_k(a, t, Ks + t * T::BUF);
+            if (t > 0) req.ask(a, tile_of<kScores>(t, ntiles));
+            req.load_k(a, tile_of<kScores>(t, ntiles), Ks + t * T::BUF);
             req.find_v(a);
-            if (t < 2) req.load_v(a, t, Vs + t * T::BUF);
+            if (t < 2) req.load_v(a, tile_of<kScores>(t, ntiles), Vs + t * T::BUF);
         }
     }
-    req.ask(a, 3);  // (vnext: of tile 2)
+    req.ask(a, tile_of<kScores>(3, ntiles));  // (vnext: of tile 2)
+    if constexpr (kScores != kScoresPlain) {
+        if (a.tree && kmax > it.shift) tree_setup<512>(a, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
+        row.set(a, it, r, kmin, kmax, &lo, &hi);
+        lo_min = __builtin_amdgcn_readlane(lo, 0);
+        hi_min = __builtin_amdgcn_readlane(hi, 0);
+        lo_max = __builtin_amdgcn_readlane(lo, 31);
+        hi_max = __builtin_amdgcn_readlane(hi, 31);
+        if (a.tree) lo_min = rows_min(lo), lo_max = -rows_min(-lo), hi_max = kmax - 1;  // (a tree's bounds may fall)
+    }
     if (ntiles > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * NL) : "memory");
     else if (ntiles == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NL) : "memory");
     else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
@@ -1422,7 +1532,7 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
         const uint32_t kbase = fragment_base(Ks, k_rd);
 #pragma unroll
         for (int ks = 0; ks < KPD; ++ks) k_read(kbase, ks);
-        s_clear(tile0 * BC);
+        s_clear();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             if (ks + KPD < KS) k_read(kbase, ks + KPD);
@@ -1443,7 +1553,7 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
 
     // Tiles of which no row of this wave sees a key: only the wave's share of the requests and the barriers.
     auto idle_iteration = [&](int t) {
-        if (t + 2 < ntiles) req.load_v(a, t + 2, Vs + ((t + 2) % NST) * T::BUF);
+        if (t + 2 < ntiles) req.load_v(a, tile_of<kScores>(t + 2, ntiles), Vs + ((t + 2) % NST) * T::BUF);
         paged_barrier();
         tail_requests(t, Ks + ((t + 3) % NST) * T::BUF);
         paged_barrier();
@@ -1452,14 +1562,20 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
     if (first_row < it.rows && hi_max >= lo_min) {
         t_lo = max(0, (lo_min >> 6) - tile0 - 1);  // (the tile in front of the first visible one brings that one's scores)
         t_hi = min(ntiles, (hi_max >> 6) - tile0 + 1);
+        if constexpr (last_first(kScores)) {
+            t_lo = max(0, ntiles - 1 - t_hi);
+            t_hi = ntiles - max(0, (lo_min >> 6) - tile0);
+        }
         t_lo = min(t_lo, t_hi);
     }
     int t = 0;
+    if constexpr (last_first(kScores))  // (the last tile's V is there)
+        if (const int left = it.len - (tile0 + ntiles - 1) * BC; t_lo == 0 && t_hi > 0 && left < BC) paged_clear_past<D, kBf16>(Vs, left, lane);
     for (; t < t_lo; ++t) idle_iteration(t);
     for (; t < t_hi - 1; ++t)
         iteration(std::false_type{}, Vs + (t % NST) * T::BUF, Ks + ((t + 1) % NST) * T::BUF, Ks + ((t + 3) % NST) * T::BUF, Vs + ((t + 2) % NST) * T::BUF, t);
     if (t < t_hi) {
-        if (const int left = it.len - (tile0 + t) * BC; left < BC) paged_clear_past<D, kBf16>(Vs + (t % NST) * T::BUF, left, lane);
+        if (const int left = it.len - (tile0 + t) * BC; !last_first(kScores) && left < BC) paged_clear_past<D, kBf16>(Vs + (t % NST) * T::BUF, left, lane);
         iteration(std::true_type{}, Vs + (t % NST) * T::BUF, Ks + ((t + 1) % NST) * T::BUF, Ks + ((t + 3) % NST) * T::BUF, Vs + ((t + 2) % NST) * T::BUF, t);
         ++t;
     }
@@ -1481,6 +1597,155 @@ template <int D, int DU, bool kBf16, int kScores>
 __global__ void __launch_bounds__(512, 2) scored_tall_kernel(const ScoredArgs a)
 {
     tall_rows<D, DU, kBf16, kScores>(a);
+}
+
+// ---------------------------------------------------------------------------------------------- rows between few and many
+//
+// 128 rows, four waves that share tiles of 64 keys: a chunk of some thirty to 128 tokens times heads, as a tree of drafted tokens is, leaves half of a
+// 256-row work-group's waves without rows, and in 32-row ones each row block asks the L2 for the tiles by itself.  One barrier per tile: behind it the
+// tile is there, and the stage that the one NST - 1 tiles ahead goes to has been read.  Two stages leave room for two work-groups per CU at D = 128, whose
+// waves fill in for each other; with four a work-group is alone there, but has three tiles on their way.
+template <int D, int NSTAGES>
+struct MidCfg {
+    static constexpr int kWaves = 4, NST = NSTAGES, STAGE = 2 * PagedTile<D>::BUF, SMEM = NST * STAGE;  // a stage: K, then V
+    static_assert(kWaves * 32 * PagedTile<D>::ROW <= STAGE, "Q lies in the last stage at first, O in the first one at last");
+};
+
+template <int D, int DU, int NSTAGES, bool kBf16, int kScores>
+__global__ void __launch_bounds__(256, 2) scored_mid_kernel(const ScoredArgs a)
+{
+    using T = PagedTile<D>;
+    using C = MidCfg<D, NSTAGES>;
+    using E = Elem<kBf16>;
+    constexpr int KS = DU / 16, MB = (DU + 31) / 32, BC = T::BC, NST = C::NST, NL = PagedRequests<D, C::kWaves>::NL;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    FA_LDS char* const stages = (FA_LDS char*)smem;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6), l32 = lane & 31, g = lane >> 5;
+
+    PagedItem it;
+    if (!paged_item<kPagedMidRows>(a, lane, &it)) return;
+    paged_mark_missing<kPagedMidRows, 256>(a, it, tid);
+    int kmin, kmax;
+    paged_range<kPagedMidRows>(a, it, &kmin, &kmax);
+    if (kmax <= kmin) {
+        paged_store_empty<kPagedMidRows, 256>(a, it, tid);
+        return;
+    }
+    const int tile0 = kmin >> 6, ntiles = ((kmax + 63) >> 6) - tile0;
+    if (a.d != D) {  // columns that no request writes
+        const v4u z = {0u, 0u, 0u, 0u};
+        for (int k = tid; k < C::SMEM / 16; k += 256) *reinterpret_cast<FA_LDS v4u*>(stages + 16 * k) = z;
+        paged_barrier();
+    }
+    const int first_row = it.row0 + wave * 32, r = first_row + l32;
+
+    // ---- Q, then the first NST - 1 tiles
+    PagedRequests<D, C::kWaves> req;
+    req.set(a, it, tile0, wave, lane);
+    req.ask(a, tile_of<kScores>(0, ntiles));
+    FA_LDS char* const qst = stages + (NST - 1) * C::STAGE + wave * (32 * T::ROW);
+#pragma unroll
+    for (int x = 0; x < 32 / T::RPB; ++x) {
+        const int rl = T::RPB * x + lane / T::CPR, c = T::k_chunk(lane % T::CPR, rl), row = first_row + rl;
+        int head;
+        const int tok = row_token(a, it, row < it.rows ? row : it.rows - 1, &head);
+        if (c * 8 < a.d) dma_kib_lanes<false>(a.Q + (size_t)tok * a.q_token + (size_t)head * a.q_head + c * 16, qst + x * 1024);
+    }
+    auto request = [&](int t) __attribute__((always_inline)) {  // tile t, whose places have been asked for
+        FA_LDS char* const st = stages + (t % NST) * C::STAGE;
+        req.load(a, tile_of<kScores>(t, ntiles), st, st + T::BUF);
+    };
+#pragma unroll
+    for (int t = 0; t < NST - 1; ++t) {
+        if (t < ntiles) {
+            if (t > 0) req.ask(a, tile_of<kScores>(t, ntiles));
+            request(t);
+        }
+    }
+    req.ask(a, tile_of<kScores>(NST - 1, ntiles));
+    RowScores<kScores> row;
+    if (a.tree && kmax > it.shift) tree_setup<256>(a, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
+    int lo, hi;
+    row.set(a, it, r, kmin, kmax, &lo, &hi);
+    int lo_min = __builtin_amdgcn_readlane(lo, 0), hi_min = __builtin_amdgcn_readlane(hi, 0);
+    int lo_max = __builtin_amdgcn_readlane(lo, 31), hi_max = __builtin_amdgcn_readlane(hi, 31);  // (bounds do not fall from row to row)
+    if (a.tree) lo_min = rows_min(lo), lo_max = -rows_min(-lo), hi_max = kmax - 1;               // (but a tree's do)
+
+    v8h qf[KS];
+    v16f oacc[MB];
+    PagedSoftmax<kBf16, MB, 2> soft;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[mb][e] = 0.0f;
+    const float c2 = a.scale_log2, inv_c2 = __builtin_amdgcn_rcpf(c2);
+    const int k_rd = T::k_lane(lane), v_rd = T::v_lane(lane);
+    for (int t = 0; t < ntiles; ++t) {
+        const int kb0 = (tile0 + tile_of<kScores>(t, ntiles)) * BC;
+        FA_LDS char* const kst = stages + (t % NST) * C::STAGE;
+        FA_LDS char* const vst = kst + T::BUF;
+        // tile t has landed when no more than the requests of those behind it are on their way (of each K and V, NL)
+        const int behind = min(NST - 2, ntiles - 1 - t);
+        if (NST > 3 && behind == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * NL) : "memory");
+        else if (NST > 2 && behind == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (t == 0) {  // (Q came in front of it)
+            const uint32_t qbase = fragment_base(qst, k_rd);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) qf[ks] = k_fragment<D>(qbase, ks, 0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
+        }
+        paged_barrier();
+        if (t + NST - 1 < ntiles) {
+            request(t + NST - 1);
+            req.ask(a, tile_of<kScores>(t + NST, ntiles));
+        }
+        if (first_row >= it.rows || kb0 > hi_max || kb0 + BC <= lo_min) continue;  // nothing that this wave's rows see
+        if (const int left = it.len - kb0; left < BC) paged_clear_past<D, kBf16>(vst, left, lane);
+        v16f s[2];
+        uint32_t p[2][2][4];
+        {
+            const uint32_t kbase = fragment_base(kst, k_rd);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                if constexpr (kScores == kScoresSloped) {
+                    s[kb] = row.slant(kb);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[kb][e] = 0.0f;
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) s[kb] = E::mfma(k_fragment<D>(kbase, ks, kb), qf[ks], s[kb]);
+            order_reads_and_mfmas<2 * KS, 1, 6>();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const uint32_t vbase = fragment_base(vst, v_rd);
+        v8h vf[4][MB];  // (the first step's are read while the softmax is worked out)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) vf[0][mb] = v_fragment<D>(vbase, 0, mb);
+        __builtin_amdgcn_sched_barrier(0);
+        row.finish(a, s, kb0, g, mask_sides(kb0, lo_max, hi_min), lo, hi);
+        soft.template tile<has_slopes(kScores)>(s, oacc, p, c2, inv_c2, 0, 0, 0, row.offset(kb0, g));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ps = 0; ps < 4; ++ps)
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+                if (ps > 0) vf[ps][mb] = v_fragment<D>(vbase, ps, mb);
+                oacc[mb] = E::mfma(vf[ps][mb], as_fragment(p[ps >> 1][ps & 1]), oacc[mb]);
+            }
+        order_reads_and_mfmas<4 * MB, 2, MB, true>();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    paged_barrier();  // every wave is done with the stages
+    if (first_row >= it.rows) return;
+    if (__builtin_expect(any_not_finite<MB>(oacc), 0)) paged_rescue<BC, MB, kBf16, kScores>(a, it, r, kmin, kmax, tile0, ntiles, 0, 1, soft.m_ref, oacc, row);
+    paged_store_rows<D, MB, kBf16, kScores>(a, it, first_row, r, lane, g, soft.m_ref, soft.l_run, oacc, stages + wave * (32 * T::ROW));
 }
 
 // ---------------------------------------------------------------------------------------------- merge of splits
@@ -1594,18 +1859,26 @@ inline int launch_paged_bucket(const PagedArgs& a, bool bf16, int rows, long lon
     return bf16 ? launch_paged_type<D, true>(a, rows, blocks, st) : launch_paged_type<D, false>(a, rows, blocks, st);
 }
 
-template <int D, int DU, bool kBf16, int kScores, int kRows>
+template <int kRows>
+inline hipError_t launch_scored_kernel(void (*kern)(ScoredArgs), int tiles, DeviceFlags& attr_done, const ScoredArgs& a, long long blocks, hipStream_t st)
+{
+    if (hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), tiles + kTreeLds, attr_done); e != hipSuccess) return e;
+    return launch_kernel(kern, dim3((unsigned)blocks), dim3(paged_threads(kRows)), a.tree ? tiles + kTreeLds : tiles, st, a);
+}
+template <int D, int DU, bool kBf16, int kScores, int kRows, int NSTAGES = 4>
 inline hipError_t launch_scored_instance(const ScoredArgs& a, long long blocks, hipStream_t st)
 {
-    const auto kern = [] {
-        if constexpr (kRows == kPagedFewRows) return scored_few_kernel<D, kBf16, kScores>;
-        else return scored_tall_kernel<D, DU, kBf16, kScores>;
-    }();
-    constexpr int tiles = kRows == kPagedFewRows ? FewCfg<D>::SMEM : TallCfg<D>::SMEM, most = tiles + kTreeLds;
-    static_assert(most * (kRows == kPagedFewRows ? 2 : 1) <= 160 * 1024, "work-groups per CU");
     static DeviceFlags attr_done;  // per instantiation and device
-    if (hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), most, attr_done); e != hipSuccess) return e;
-    return launch_kernel(kern, dim3((unsigned)blocks), dim3(paged_threads(kRows)), a.tree ? most : tiles, st, a);
+    if constexpr (kRows == kPagedFewRows) {
+        static_assert(2 * (FewCfg<D>::SMEM + kTreeLds) <= 160 * 1024, "two work-groups per CU");
+        return launch_scored_kernel<kRows>(scored_few_kernel<D, kBf16, kScores>, FewCfg<D>::SMEM, attr_done, a, blocks, st);
+    } else if constexpr (kRows == kPagedMidRows) {
+        static_assert((D == 128 && NSTAGES == 4 ? 1 : 2) * (MidCfg<D, NSTAGES>::SMEM + kTreeLds) <= 160 * 1024, "work-groups per CU");
+        return launch_scored_kernel<kRows>(scored_mid_kernel<D, DU, NSTAGES, kBf16, kScores>, MidCfg<D, NSTAGES>::SMEM, attr_done, a, blocks, st);
+    } else {
+        static_assert(TallCfg<D>::SMEM + kTreeLds <= 160 * 1024, "a work-group per CU");
+        return launch_scored_kernel<kRows>(scored_tall_kernel<D, DU, kBf16, kScores>, TallCfg<D>::SMEM, attr_done, a, blocks, st);
+    }
 }
 template <int kScores, bool kBf16>
 inline int launch_scored_type(const ScoredArgs& a, int rows, long long blocks, hipStream_t st)
@@ -1613,6 +1886,11 @@ inline int launch_scored_type(const ScoredArgs& a, int rows, long long blocks, h
     if (rows == kPagedFewRows)
         return (int)(a.d <= 64 ? launch_scored_instance<64, 64, kBf16, kScores, kPagedFewRows>(a, blocks, st)
                                : launch_scored_instance<128, 128, kBf16, kScores, kPagedFewRows>(a, blocks, st));
+    if (rows == kPagedMidRows) {
+        if (a.d <= 64) return (int)launch_scored_instance<64, 64, kBf16, kScores, kPagedMidRows>(a, blocks, st);
+        if (blocks <= 256) return (int)launch_scored_instance<128, 128, kBf16, kScores, kPagedMidRows, 4>(a, blocks, st);
+        return (int)launch_scored_instance<128, 128, kBf16, kScores, kPagedMidRows, 2>(a, blocks, st);
+    }
     if (a.d <= 64) return (int)launch_scored_instance<64, 64, kBf16, kScores, kPagedTallRows>(a, blocks, st);
     if (a.d <= 96) return (int)launch_scored_instance<128, 96, kBf16, kScores, kPagedTallRows>(a, blocks, st);
     return (int)launch_scored_instance<128, 128, kBf16, kScores, kPagedTallRows>(a, blocks, st);

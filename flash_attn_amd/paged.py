@@ -620,7 +620,7 @@ def flash_keep_paged(k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, pat
     return out
 
 
-def _paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k, causal, window, num_splits, prefix, tree_words):
+def _paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k, causal, window, num_splits, softcap, alibi, prefix, tree_words):
     _check(max(B, H, H_kv, d, total_q, page_size, max_pages) <= _INT_MAX, "sizes are too large")
     p = PagedParams()
     _lib().flash_paged_params_init(C.byref(p))
@@ -628,7 +628,10 @@ def _paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max
     p.num_pages = 1
     p.max_seqlen_q, p.max_seqlen_k = _int(max_seqlen_q), _int(max_seqlen_k)
     p.is_causal, p.window_left, p.window_right, p.num_splits = int(bool(causal)), _int(window[0]), _int(window[1]), _int(num_splits)
+    p.softcap = float(softcap)
     # (only whether they are there matters)
+    if alibi:
+        p.alibi_slopes = 16
     if prefix:
         p.prefix_lens = 16
     if tree_words:
@@ -637,20 +640,21 @@ def _paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max
 
 
 def paged_resolve_splits(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q=0, max_seqlen_k=0, causal=False, window=(-1, -1), num_splits=0,
-                         prefix=False, tree_words=0):
-    """The split count that flash_forward_paged will use for such a call.  prefix: whether it has prefix_lens; tree_words: of its tree_mask."""
+                         softcap=0.0, alibi=False, prefix=False, tree_words=0):
+    """The split count that flash_forward_paged will use for such a call.  alibi, prefix: whether it has alibi_slopes, prefix_lens; tree_words: of its
+    tree_mask."""
     S = _lib().flash_forward_paged_resolve_splits(C.byref(_paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k,
-                                                                       causal, window, num_splits, prefix, tree_words)))
+                                                                       causal, window, num_splits, softcap, alibi, prefix, tree_words)))
     if S < 0:
         raise FlashError(S, "flash_forward_paged_resolve_splits")
     return S
 
 
 def paged_workspace_bytes(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q=0, max_seqlen_k=0, causal=False, window=(-1, -1), num_splits=0,
-                          prefix=False, tree_words=0):
+                          softcap=0.0, alibi=False, prefix=False, tree_words=0):
     """Bytes of (O_partial, LSE_partial) for flash_forward_paged calls of these sizes and masks."""
     ob, lb = C.c_size_t(), C.c_size_t()
     _raise(_lib().flash_forward_paged_workspace_bytes(C.byref(_paged_shape(B, H, H_kv, d, total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k,
-                                                                           causal, window, num_splits, prefix, tree_words)), C.byref(ob), C.byref(lb)),
+                                                                           causal, window, num_splits, softcap, alibi, prefix, tree_words)), C.byref(ob), C.byref(lb)),
            "flash_forward_paged_workspace_bytes")
     return ob.value, lb.value

@@ -287,7 +287,8 @@ int flash_append_paged(const flash_paged_params *p, void *stream);
 int flash_forward_paged(const flash_paged_params *p, void *stream);
 
 /* The split count that flash_forward_paged uses for p, and the bytes of its workspace (0 for one split).  They depend on the sizes (B, H, H_kv, d,
- * total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k), the masks (of prefix_lens and tree_mask: whether they are there, and tree_words) and num_splits. */
+ * total_q, page_size, max_pages, max_seqlen_q, max_seqlen_k), the masks, num_splits, softcap, and
+ * whether alibi_slopes, prefix_lens and tree_mask (and how many tree_words) are there. */
 int flash_forward_paged_resolve_splits(const flash_paged_params *p);
 int flash_forward_paged_workspace_bytes(const flash_paged_params *p, size_t *o_partial_bytes, size_t *lse_partial_bytes);
 

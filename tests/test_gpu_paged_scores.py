@@ -9,9 +9,10 @@ from paged_reference import Batch
 
 pytestmark = pytest.mark.gpu
 
-# (new tokens, keys) per sequence, H, H_kv: what the 32-row and the 256-row form get
+# (new tokens, keys) per sequence, H, H_kv: what the forms of 32, 128 and 256 rows get (the last in so many splits)
 FEW = [([1, 1, 1, 1], [1, 70, 333, 1000], 8, 2), ([1, 0, 3, 5], [900, 17, 3, 130], 4, 4), ([7, 2], [300, 65], 15, 3)]
-TALL = [([300, 70, 1], [420, 200, 64], 96, 48), ([290, 0, 150], [280, 9, 700], 80, 40)]
+MID = [([300, 70, 1], [420, 200, 64], 96, 48), ([290, 0, 150], [280, 9, 700], 80, 40)]
+TALL = [([520], [2000], 32, 8, 3), ([1500], [1500], 32, 8, 1)]
 DIMS = [8, 40, 64, 80, 128]
 KINDS = ["cap", "slopes", "both", "prefix", "prefix window", "cap prefix", "slopes window", "slopes all"]
 
@@ -55,8 +56,19 @@ def test_few_rows(fa, kind, shape, d, dtype, splits):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("shape", range(2))
 @pytest.mark.parametrize("d,dtype,splits", [(40, torch.bfloat16, 1), (64, torch.float16, 3), (80, torch.bfloat16, 2), (128, torch.float16, 1), (128, torch.bfloat16, 3)])
-def test_many_rows(fa, kind, shape, d, dtype, splits):
-    news, lens, H, Hk = TALL[shape]
+def test_rows_between(fa, kind, shape, d, dtype, splits):
+    news, lens, H, Hk = MID[shape]
+    batch = Batch(news, lens, H, Hk, d, 64, dtype, seed=d + shape, behind=3)
+    how, kw = extras(kind, H, lens)
+    ref.check(*call(fa, batch, how, kw, num_splits=splits), want(batch, how, kw), kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("shape,d,dtype", [(0, 40, torch.bfloat16), (0, 64, torch.float16), (0, 80, torch.bfloat16), (0, 128, torch.float16), (1, 80, torch.float16), (1, 128, torch.bfloat16)])
+def test_many_rows(fa, kind, shape, d, dtype):
+    news, lens, H, Hk, splits = TALL[shape]
+    if shape == 1 and kind not in ("cap", "slopes", "prefix"):
+        pytest.skip("the smaller one has it")
     batch = Batch(news, lens, H, Hk, d, 64, dtype, seed=d + shape, behind=3)
     how, kw = extras(kind, H, lens)
     ref.check(*call(fa, batch, how, kw, num_splits=splits), want(batch, how, kw), kind)
@@ -65,7 +77,8 @@ def test_many_rows(fa, kind, shape, d, dtype, splits):
 # ---------------------------------------------------------------------------------------------------- trees
 
 TREES_FEW = [([5, 1, 13, 2], [5, 300, 130, 66], 4, 4), ([25], [1025], 8, 2), ([64, 7], [64, 400], 1, 1), ([100, 256], [777, 256], 1, 1)]
-TREES_TALL = [([64, 30, 1], [200, 31, 640], 320, 40), ([200, 256, 9], [263, 256, 700], 66, 33)]
+TREES_MID = [([64, 30, 1], [200, 31, 640], 320, 40), ([200, 256, 9], [263, 256, 700], 66, 33)]
+TREES_TALL = [([256, 200], [256, 1500], 64, 1, 3), ([128, 256], [3000, 1000], 64, 8, 1)]
 TREE_KINDS = ["", "cap", "slopes", "both", "window", "slopes window"]
 
 
@@ -94,8 +107,19 @@ def test_trees_few_rows(fa, kind, shape, d, dtype, splits):
 @pytest.mark.parametrize("kind", TREE_KINDS)
 @pytest.mark.parametrize("shape", range(2))
 @pytest.mark.parametrize("d,dtype,splits", [(64, torch.bfloat16, 1), (80, torch.float16, 3), (128, torch.float16, 1), (128, torch.bfloat16, 2)])
-def test_trees_many_rows(fa, kind, shape, d, dtype, splits):
-    news, lens, H, Hk = TREES_TALL[shape]
+def test_trees_rows_between(fa, kind, shape, d, dtype, splits):
+    news, lens, H, Hk = TREES_MID[shape]
+    batch = Batch(news, lens, H, Hk, d, 32, dtype, seed=d + shape)
+    how, kw = tree(news, kind, H, d + shape)
+    ref.check(*call(fa, batch, how, kw, num_splits=splits), want(batch, how, kw), kind)
+
+
+@pytest.mark.parametrize("kind", TREE_KINDS)
+@pytest.mark.parametrize("shape,d,dtype", [(0, 40, torch.float16), (0, 64, torch.bfloat16), (0, 80, torch.float16), (0, 128, torch.bfloat16), (1, 80, torch.bfloat16), (1, 128, torch.float16)])
+def test_trees_many_rows(fa, kind, shape, d, dtype):
+    news, lens, H, Hk, splits = TREES_TALL[shape]
+    if shape == 1 and kind not in ("", "both"):
+        pytest.skip("the smaller one has it")
     batch = Batch(news, lens, H, Hk, d, 32, dtype, seed=d + shape)
     how, kw = tree(news, kind, H, d + shape)
     ref.check(*call(fa, batch, how, kw, num_splits=splits), want(batch, how, kw), kind)
@@ -163,7 +187,7 @@ def test_infinite_scores_are_capped(fa):
 
 @pytest.mark.parametrize("cap", [1e-3, 0.5, 30.0, 1000.0])
 def test_small_and_large_caps(fa, cap):
-    for news, lens, H, Hk in ((FEW[0]), (TALL[1])):
+    for news, lens, H, Hk in (FEW[0], MID[1], TALL[0][:4]):
         batch = Batch(news, lens, H, Hk, 64, 16, torch.bfloat16, seed=5)
         batch.q *= 4
         how = {"causal": True, "softcap": cap}
@@ -184,7 +208,7 @@ def test_a_cap_alone_changes_what_it_should(fa):
 
 
 def test_rows_of_no_sequence_stay(fa):
-    for shape in (FEW[2], TALL[0]):
+    for shape in (FEW[2], MID[0], TALL[0][:4]):
         news, lens, H, Hk = shape
         batch = Batch(news, lens, H, Hk, 64, 16, torch.bfloat16, seed=7, first=3, behind=4)
         T = batch.q.shape[0]
@@ -197,7 +221,7 @@ def test_rows_of_no_sequence_stay(fa):
                 assert (t[:3] == 7).all() and (t[-4:] == 7).all()
 
 
-@pytest.mark.parametrize("shape", [FEW[2], TALL[0]])
+@pytest.mark.parametrize("shape", [FEW[2], MID[0], TALL[0][:4]])
 def test_strides_streams_and_both_ways_in(fa, shape):
     """Heads before or behind rows in a page, strided queries and results, a stream of the caller's, workspace of the caller's: always the same result."""
     news, lens, H, Hk = shape
