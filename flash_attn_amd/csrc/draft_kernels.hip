@@ -8,49 +8,49 @@ namespace {
 // ---- masks
 //
 // mask(i) = bit i | mask(parent(i)).  Pointers double: mask(i) |= mask(up(i)), up(i) = up(up(i)), so that a path of n tokens takes log2 n rounds in
-// LDS.  A thread per token that the mask can name, a work-group per sequence: of 64 tokens it is one wave, whose barriers cost nothing.
-__global__ void __launch_bounds__(256) tree_mask_kernel(const TreeMaskArgs a)
+// LDS, whose two halves take turns: one barrier a round.  A thread per token that the mask can name, a work-group per sequence: of 64 tokens it is one
+// wave, whose barriers cost nothing.
+template <int W>
+__global__ void __launch_bounds__(64 * W) tree_mask_kernel(const TreeMaskArgs a)
 {
-    __shared__ uint64_t words[256 * 4];
-    __shared__ int up[256];
-    const int b = blockIdx.x, i = threadIdx.x, W = a.words, threads = blockDim.x;  // (64 * W)
+    constexpr int kTokens = 64 * W;
+    __shared__ uint64_t words[2][W][kTokens];
+    __shared__ int up[2][kTokens];
+    const int b = blockIdx.x, i = threadIdx.x;
     int c0 = a.cu[b], c1 = a.cu[b + 1], len = a.lens ? a.lens[b] : 0;
     c0 = c0 < 0 ? 0 : c0 > a.tokens ? a.tokens : c0;
     c1 = c1 < c0 ? c0 : c1 > a.tokens ? a.tokens : c1;
     const int n = c1 - c0, base = a.lens ? (int)((uint32_t)len - (uint32_t)n) : 0;
     const bool mine = i < n;
     int p = mine ? a.parents[c0 + i] : -1;
-    if (p >= i) p = -1;  // a parent stands in front of its children
-    uint64_t w[4];
+    if (p >= i || p < 0) p = -1;  // a parent stands in front of its children
+    uint64_t w[W];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = i >> 6 == k ? 1ull << (i & 63) : 0ull;
-    for (;;) {
-        if (p < 0) p = -1;
+    for (int k = 0; k < W; ++k) w[k] = i >> 6 == k ? 1ull << (i & 63) : 0ull;
+    int half = 0;
+    for (int reach = 1; reach < min(n, kTokens); reach *= 2) {  // paths of so many tokens are complete
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < W) words[k * 256 + i] = w[k];
-        up[i] = p;
-        if (!__syncthreads_or(p >= 0)) break;
+        for (int k = 0; k < W; ++k) words[half][k][i] = w[k];
+        up[half][i] = p;
+        __syncthreads();
         if (p >= 0) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k < W) w[k] |= words[k * 256 + p];
-            p = up[p];
+            for (int k = 0; k < W; ++k) w[k] |= words[half][k][p];
+            p = up[half][p];
         }
-        __syncthreads();
+        half ^= 1;
     }
     if (mine) {
         int depth = -1;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < W) {
-                a.mask[(int64_t)(c0 + i) * a.mask_stride + k] = w[k];
-                depth += __builtin_popcountll(w[k]);
-            }
+        for (int k = 0; k < W; ++k) {
+            a.mask[(int64_t)(c0 + i) * a.mask_stride + k] = w[k];
+            depth += __builtin_popcountll(w[k]);
+        }
         if (a.positions) a.positions[c0 + i] = base + depth;
     }
     // tokens that the mask has no bits for
-    for (int j = i + threads; j < n; j += threads) {
+    for (int j = i + kTokens; j < n; j += kTokens) {
         for (int k = 0; k < W; ++k) a.mask[(int64_t)(c0 + j) * a.mask_stride + k] = 0;
         if (a.positions) a.positions[c0 + j] = base;
     }
@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(256) keep_kernel(const KeepArgs a)
     const int layer = a.by_b.quotient(unit), b = unit - layer * a.B;
     const int n = (int)max((int64_t)0, min((int64_t)a.cu[b + 1] - a.cu[b], (int64_t)1 << 30));
     int len = a.lens[b], want = a.accepted[b];
+    int p = lane < a.most ? a.path[(int64_t)b * a.path_stride + lane] : -1;  // (asked for together with them)
     len = len < 0 ? 0 : len > a.capacity ? a.capacity : len;
     want = want < 0 ? 0 : want > a.most ? a.most : want;
     const int base = len - n;
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(256) keep_kernel(const KeepArgs a)
     for (int i0 = 0; i0 < want; i0 += 64) {
         // a lane per entry of the path: how far it grows, and where its rows lie
         const int i = i0 + lane;
-        const int p = i < want ? a.path[(int64_t)b * a.path_stride + i] : -1;
+        if (i0 > 0) p = i < want ? a.path[(int64_t)b * a.path_stride + i] : -1;
         int before = __shfl_up(p, 1);
         if (lane == 0) before = last;
         const uint64_t bad = __builtin_amdgcn_ballot_w64(!(i < want && p > before && p < n));
@@ -122,7 +123,11 @@ __global__ void __launch_bounds__(256) keep_kernel(const KeepArgs a)
 
 }  // namespace
 
-int launch_tree_mask(const TreeMaskArgs& a, hipStream_t st) { return (int)launch_kernel(tree_mask_kernel, dim3((unsigned)a.B), dim3(64 * a.words), 0, st, a); }
+int launch_tree_mask(const TreeMaskArgs& a, hipStream_t st)
+{
+    const auto kern = a.words == 1 ? tree_mask_kernel<1> : a.words == 2 ? tree_mask_kernel<2> : a.words == 3 ? tree_mask_kernel<3> : tree_mask_kernel<4>;
+    return (int)launch_kernel(kern, dim3((unsigned)a.B), dim3(64 * a.words), 0, st, a);
+}
 
 int launch_keep(const KeepArgs& p, hipStream_t st)
 {
