@@ -1604,45 +1604,49 @@ __global__ void __launch_bounds__(512, 2) scored_tall_kernel(const ScoredArgs a)
 // 128 rows, four waves that share tiles of 64 keys: a chunk of some thirty to 128 tokens times heads, as a tree of drafted tokens is, leaves half of a
 // 256-row work-group's waves without rows, and in 32-row ones each row block asks the L2 for the tiles by itself.  One barrier per tile: behind it the
 // tile is there, and the stage that the one NST - 1 tiles ahead goes to has been read.  Two stages leave room for two work-groups per CU at D = 128, whose
-// waves fill in for each other; with four a work-group is alone there, but has three tiles on their way.
-template <int D, int NSTAGES>
+// waves fill in for each other: one wave alone on a SIMD takes 1.45 us per tile, bound by the issue of its instructions (four stages: the same), two
+// take 2.0.  Where there is a CU for each work-group it has a second group of waves instead, with every other tile and stages of its own; the two merge in LDS.
+template <int D, int NSTAGES, int GROUPS>
 struct MidCfg {
-    static constexpr int kWaves = 4, NST = NSTAGES, STAGE = 2 * PagedTile<D>::BUF, SMEM = NST * STAGE;  // a stage: K, then V
+    static constexpr int kWaves = 4, NST = NSTAGES, STAGE = 2 * PagedTile<D>::BUF, SMEM = GROUPS * NST * STAGE;  // a stage: K, then V
     static_assert(kWaves * 32 * PagedTile<D>::ROW <= STAGE, "Q lies in the last stage at first, O in the first one at last");
+    static_assert(GROUPS == 1 || kWaves * 64 * 4 * (D / 2 + 2) <= SMEM, "the second group's results");
 };
 
-template <int D, int DU, int NSTAGES, bool kBf16, int kScores>
-__global__ void __launch_bounds__(256, 2) scored_mid_kernel(const ScoredArgs a)
+template <int D, int DU, int NSTAGES, int GROUPS, bool kBf16, int kScores>
+__global__ void __launch_bounds__(256 * GROUPS, 2) scored_mid_kernel(const ScoredArgs a)
 {
     using T = PagedTile<D>;
-    using C = MidCfg<D, NSTAGES>;
+    using C = MidCfg<D, NSTAGES, GROUPS>;
     using E = Elem<kBf16>;
-    constexpr int KS = DU / 16, MB = (DU + 31) / 32, BC = T::BC, NST = C::NST, NL = PagedRequests<D, C::kWaves>::NL;
+    constexpr int KS = DU / 16, MB = (DU + 31) / 32, BC = T::BC, NST = C::NST, NL = PagedRequests<D, C::kWaves>::NL, kThreads = 256 * GROUPS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    FA_LDS char* const stages = (FA_LDS char*)smem;
-    const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6), l32 = lane & 31, g = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6) & 3, grp = wave_uniform(tid >> 8), l32 = lane & 31, g = lane >> 5;
+    FA_LDS char* const stages = (FA_LDS char*)smem + grp * (C::NST * C::STAGE);  // of the group
 
     PagedItem it;
     if (!paged_item<kPagedMidRows>(a, lane, &it)) return;
-    paged_mark_missing<kPagedMidRows, 256>(a, it, tid);
+    paged_mark_missing<kPagedMidRows, kThreads>(a, it, tid);
     int kmin, kmax;
     paged_range<kPagedMidRows>(a, it, &kmin, &kmax);
     if (kmax <= kmin) {
-        paged_store_empty<kPagedMidRows, 256>(a, it, tid);
+        paged_store_empty<kPagedMidRows, kThreads>(a, it, tid);
         return;
     }
     const int tile0 = kmin >> 6, ntiles = ((kmax + 63) >> 6) - tile0;
     if (a.d != D) {  // columns that no request writes
         const v4u z = {0u, 0u, 0u, 0u};
-        for (int k = tid; k < C::SMEM / 16; k += 256) *reinterpret_cast<FA_LDS v4u*>(stages + 16 * k) = z;
+        for (int k = tid; k < C::SMEM / 16; k += kThreads) *reinterpret_cast<FA_LDS v4u*>((FA_LDS char*)smem + 16 * k) = z;
         paged_barrier();
     }
     const int first_row = it.row0 + wave * 32, r = first_row + l32;
 
-    // ---- Q, then the first NST - 1 tiles
+    // ---- Q, then the group's first NST - 1 tiles: grp, grp + GROUPS, ... in their order
+    const int mine = (ntiles - grp + GROUPS - 1) / GROUPS, steps = (ntiles + GROUPS - 1) / GROUPS;
+    auto tile_at = [&](int i) __attribute__((always_inline)) { return tile_of<kScores>(min(i * GROUPS + grp, ntiles - 1), ntiles); };
     PagedRequests<D, C::kWaves> req;
     req.set(a, it, tile0, wave, lane);
-    req.ask(a, tile_of<kScores>(0, ntiles));
+    req.ask(a, tile_at(0));
     FA_LDS char* const qst = stages + (NST - 1) * C::STAGE + wave * (32 * T::ROW);
 #pragma unroll
     for (int x = 0; x < 32 / T::RPB; ++x) {
@@ -1651,20 +1655,20 @@ __global__ void __launch_bounds__(256, 2) scored_mid_kernel(const ScoredArgs a)
         const int tok = row_token(a, it, row < it.rows ? row : it.rows - 1, &head);
         if (c * 8 < a.d) dma_kib_lanes<false>(a.Q + (size_t)tok * a.q_token + (size_t)head * a.q_head + c * 16, qst + x * 1024);
     }
-    auto request = [&](int t) __attribute__((always_inline)) {  // tile t, whose places have been asked for
-        FA_LDS char* const st = stages + (t % NST) * C::STAGE;
-        req.load(a, tile_of<kScores>(t, ntiles), st, st + T::BUF);
+    auto request = [&](int i) __attribute__((always_inline)) {  // the group's tile i, whose places have been asked for
+        FA_LDS char* const st = stages + (i % NST) * C::STAGE;
+        req.load(a, tile_at(i), st, st + T::BUF);
     };
 #pragma unroll
-    for (int t = 0; t < NST - 1; ++t) {
-        if (t < ntiles) {
-            if (t > 0) req.ask(a, tile_of<kScores>(t, ntiles));
-            request(t);
+    for (int i = 0; i < NST - 1; ++i) {
+        if (i < mine) {
+            if (i > 0) req.ask(a, tile_at(i));
+            request(i);
         }
     }
-    req.ask(a, tile_of<kScores>(NST - 1, ntiles));
+    req.ask(a, tile_at(NST - 1));
     RowScores<kScores> row;
-    if (a.tree && kmax > it.shift) tree_setup<256>(a, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
+    if (a.tree && kmax > it.shift) tree_setup<kThreads>(a, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
     int lo, hi;
     row.set(a, it, r, kmin, kmax, &lo, &hi);
     int lo_min = __builtin_amdgcn_readlane(lo, 0), hi_min = __builtin_amdgcn_readlane(hi, 0);
@@ -1680,16 +1684,16 @@ __global__ void __launch_bounds__(256, 2) scored_mid_kernel(const ScoredArgs a)
         for (int e = 0; e < 16; ++e) oacc[mb][e] = 0.0f;
     const float c2 = a.scale_log2, inv_c2 = __builtin_amdgcn_rcpf(c2);
     const int k_rd = T::k_lane(lane), v_rd = T::v_lane(lane);
-    for (int t = 0; t < ntiles; ++t) {
-        const int kb0 = (tile0 + tile_of<kScores>(t, ntiles)) * BC;
-        FA_LDS char* const kst = stages + (t % NST) * C::STAGE;
+    for (int i = 0; i < steps; ++i) {
+        const int kb0 = (tile0 + tile_at(i)) * BC;
+        FA_LDS char* const kst = stages + (i % NST) * C::STAGE;
         FA_LDS char* const vst = kst + T::BUF;
-        // tile t has landed when no more than the requests of those behind it are on their way (of each K and V, NL)
-        const int behind = min(NST - 2, ntiles - 1 - t);
+        // tile i has landed when no more than the requests of those behind it are on their way (of each K and V, NL)
+        const int behind = min(NST - 2, mine - 1 - i);
         if (NST > 3 && behind == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * NL) : "memory");
         else if (NST > 2 && behind == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (t == 0) {  // (Q came in front of it)
+        if (i == 0) {  // (Q came in front of it)
             const uint32_t qbase = fragment_base(qst, k_rd);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) qf[ks] = k_fragment<D>(qbase, ks, 0);
@@ -1697,10 +1701,11 @@ __global__ void __launch_bounds__(256, 2) scored_mid_kernel(const ScoredArgs a)
             for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
         }
         paged_barrier();
-        if (t + NST - 1 < ntiles) {
-            request(t + NST - 1);
-            req.ask(a, tile_of<kScores>(t + NST, ntiles));
+        if (i + NST - 1 < mine) {
+            request(i + NST - 1);
+            req.ask(a, tile_at(i + NST));
         }
+        if (i >= mine) continue;
         if (first_row >= it.rows || kb0 > hi_max || kb0 + BC <= lo_min) continue;  // nothing that this wave's rows see
         if (const int left = it.len - kb0; left < BC) paged_clear_past<D, kBf16>(vst, left, lane);
         v16f s[2];
@@ -1742,10 +1747,34 @@ __global__ void __launch_bounds__(256, 2) scored_mid_kernel(const ScoredArgs a)
         order_reads_and_mfmas<4 * MB, 2, MB, true>();
         __builtin_amdgcn_sched_barrier(0);
     }
+    if (first_row < it.rows && __builtin_expect(any_not_finite<MB>(oacc), 0))
+        paged_rescue<BC, MB, kBf16, kScores>(a, it, r, kmin, kmax, tile0, ntiles, last_first(kScores) ? (ntiles - 1 - grp) % GROUPS : grp, GROUPS, soft.m_ref, oacc, row);
     paged_barrier();  // every wave is done with the stages
+    FA_LDS char* ost = (FA_LDS char*)smem + wave * (32 * T::ROW);
+    if constexpr (GROUPS == 2) {
+        // the second group's results to the first, lane by lane: reference, sum, O
+        FA_LDS float* const x = (FA_LDS float*)smem + wave * (64 * (16 * MB + 2)) + lane;
+        ost = (FA_LDS char*)((FA_LDS float*)smem + wave * (64 * (16 * MB + 2)));  // (what the wave itself reads here)
+        if (grp == 1) {
+            x[0] = soft.m_ref, x[64] = soft.l_run;
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[64 * (2 + 16 * mb + e)] = oacc[mb][e];
+        }
+        paged_barrier();
+        if (grp == 1) return;
+        const float m1 = x[0], m = fmaxf(soft.m_ref, m1), f0 = fast_exp2(soft.m_ref - m), f1 = fast_exp2(m1 - m);
+        soft.l_run = f0 * soft.l_run + f1 * x[64];
+        soft.m_ref = m;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) oacc[mb][e] = f0 * oacc[mb][e] + f1 * x[64 * (2 + 16 * mb + e)];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before O goes there)
+    }
     if (first_row >= it.rows) return;
-    if (__builtin_expect(any_not_finite<MB>(oacc), 0)) paged_rescue<BC, MB, kBf16, kScores>(a, it, r, kmin, kmax, tile0, ntiles, 0, 1, soft.m_ref, oacc, row);
-    paged_store_rows<D, MB, kBf16, kScores>(a, it, first_row, r, lane, g, soft.m_ref, soft.l_run, oacc, stages + wave * (32 * T::ROW));
+    paged_store_rows<D, MB, kBf16, kScores>(a, it, first_row, r, lane, g, soft.m_ref, soft.l_run, oacc, ost);
 }
 
 // ---------------------------------------------------------------------------------------------- merge of splits
@@ -1860,12 +1889,12 @@ inline int launch_paged_bucket(const PagedArgs& a, bool bf16, int rows, long lon
 }
 
 template <int kRows>
-inline hipError_t launch_scored_kernel(void (*kern)(ScoredArgs), int tiles, DeviceFlags& attr_done, const ScoredArgs& a, long long blocks, hipStream_t st)
+inline hipError_t launch_scored_kernel(void (*kern)(ScoredArgs), int tiles, DeviceFlags& attr_done, const ScoredArgs& a, long long blocks, hipStream_t st, int threads = paged_threads(kRows))
 {
     if (hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), tiles + kTreeLds, attr_done); e != hipSuccess) return e;
-    return launch_kernel(kern, dim3((unsigned)blocks), dim3(paged_threads(kRows)), a.tree ? tiles + kTreeLds : tiles, st, a);
+    return launch_kernel(kern, dim3((unsigned)blocks), dim3(threads), a.tree ? tiles + kTreeLds : tiles, st, a);
 }
-template <int D, int DU, bool kBf16, int kScores, int kRows, int NSTAGES = 4>
+template <int D, int DU, bool kBf16, int kScores, int kRows, int NSTAGES = 4, int GROUPS = 1>
 inline hipError_t launch_scored_instance(const ScoredArgs& a, long long blocks, hipStream_t st)
 {
     static DeviceFlags attr_done;  // per instantiation and device
@@ -1873,8 +1902,8 @@ inline hipError_t launch_scored_instance(const ScoredArgs& a, long long blocks, 
         static_assert(2 * (FewCfg<D>::SMEM + kTreeLds) <= 160 * 1024, "two work-groups per CU");
         return launch_scored_kernel<kRows>(scored_few_kernel<D, kBf16, kScores>, FewCfg<D>::SMEM, attr_done, a, blocks, st);
     } else if constexpr (kRows == kPagedMidRows) {
-        static_assert((D == 128 && NSTAGES == 4 ? 1 : 2) * (MidCfg<D, NSTAGES>::SMEM + kTreeLds) <= 160 * 1024, "work-groups per CU");
-        return launch_scored_kernel<kRows>(scored_mid_kernel<D, DU, NSTAGES, kBf16, kScores>, MidCfg<D, NSTAGES>::SMEM, attr_done, a, blocks, st);
+        static_assert((3 - GROUPS) * (MidCfg<D, NSTAGES, GROUPS>::SMEM + kTreeLds) <= 160 * 1024, "two work-groups per CU, or one of two groups");
+        return launch_scored_kernel<kRows>(scored_mid_kernel<D, DU, NSTAGES, GROUPS, kBf16, kScores>, MidCfg<D, NSTAGES, GROUPS>::SMEM, attr_done, a, blocks, st, 256 * GROUPS);
     } else {
         static_assert(TallCfg<D>::SMEM + kTreeLds <= 160 * 1024, "a work-group per CU");
         return launch_scored_kernel<kRows>(scored_tall_kernel<D, DU, kBf16, kScores>, TallCfg<D>::SMEM, attr_done, a, blocks, st);
@@ -1887,8 +1916,12 @@ inline int launch_scored_type(const ScoredArgs& a, int rows, long long blocks, h
         return (int)(a.d <= 64 ? launch_scored_instance<64, 64, kBf16, kScores, kPagedFewRows>(a, blocks, st)
                                : launch_scored_instance<128, 128, kBf16, kScores, kPagedFewRows>(a, blocks, st));
     if (rows == kPagedMidRows) {
+        // a CU for each work-group: two groups of waves where there are tiles enough (one group / two, pieces of 10 to 30 tiles 1.21 on average, more than 30
+        // 1.39, 5 to 10 1.08, of one tile 0.92; a window of 1023 on 2900 keys H12 H_kv4 d64 29.8 -> 25.3 us)
+        if (blocks <= 256 && a.tiles_per_split >= 6)
+            return (int)(a.d <= 64 ? launch_scored_instance<64, 64, kBf16, kScores, kPagedMidRows, 4, 2>(a, blocks, st)
+                                   : launch_scored_instance<128, 128, kBf16, kScores, kPagedMidRows, 2, 2>(a, blocks, st));
         if (a.d <= 64) return (int)launch_scored_instance<64, 64, kBf16, kScores, kPagedMidRows>(a, blocks, st);
-        if (blocks <= 256) return (int)launch_scored_instance<128, 128, kBf16, kScores, kPagedMidRows, 4>(a, blocks, st);
         return (int)launch_scored_instance<128, 128, kBf16, kScores, kPagedMidRows, 2>(a, blocks, st);
     }
     if (a.d <= 64) return (int)launch_scored_instance<64, 64, kBf16, kScores, kPagedTallRows>(a, blocks, st);

@@ -283,7 +283,8 @@ int flash_append_paged(const flash_paged_params *p, void *stream);
 
 /* O = softmax(mask(Q K^T * scale)) V of every sequence's new tokens over its pages, down to one token per sequence, and LSE.  Rows that
  * see no key get O = 0 and LSE = -inf.  A value that is not finite in a row of V that a query does not see, or behind a
- * sequence's end, does not reach that query's O; one that it sees does (an infinity as NaN where its probability rounds to 0 in the caches' type). */
+ * sequence's end, does not reach that query's O; one that it sees does (an infinity as NaN where its probability rounds to 0 in the caches' type;
+ * where its weight is 0 in 32 bits, far behind a steep bias, it may not). */
 int flash_forward_paged(const flash_paged_params *p, void *stream);
 
 /* The split count that flash_forward_paged uses for p, and the bytes of its workspace (0 for one split).  They depend on the sizes (B, H, H_kv, d,

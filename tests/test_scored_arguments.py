@@ -178,7 +178,8 @@ for call in json.load(sys.stdin):
     rec.recorder_clear()
     assert L.flash_forward_paged(C.byref(p), None) == 0, call
     name = rec.recorder_name(0).decode()
-    res.append([re.search("scored_(few|mid|tall)_kernel", name).group(1), int(re.search("ELi(.)EEEv", name).group(1))])
+    paired = "Li2ELb" in name and "mid" in name  # (template arguments: D, columns, stages, groups of waves, bf16, kind)
+    res.append(["paired" if paired else re.search("scored_(few|mid|tall)_kernel", name).group(1), int(re.search("ELi(.)EEEv", name).group(1))])
 json.dump(res, sys.stdout)
 """
 
@@ -194,7 +195,7 @@ def launched(calls):
 def test_forms_of_the_gpu_tests():
     """The shapes of test_gpu_paged_scores.py reach the form that they are there for, and the calls the kernel of their kind."""
     calls, want = [], []
-    for shapes, form, dims in ((scores.FEW, "few", (8, 40, 64, 80, 128)), (scores.MID, "mid", (40, 64, 80, 128)), (scores.TALL[:1], "tall", (40, 64, 80, 128)), (scores.TALL[1:], "tall", (80, 128))):
+    for shapes, form, dims in ((scores.FEW, "few", (8, 40, 64, 80, 128)), (scores.MID, "mid", (40, 64, 80, 128)), (scores.PAIRED, "paired", (40, 64, 80, 128)), (scores.TALL[:1], "tall", (40, 64, 80, 128)), (scores.TALL[1:], "tall", (80, 128))):
         for news, lens, H, Hk, *splits in shapes:
             for d in dims:
                 for kind, number in (("cap", 2), ("slopes", 3), ("both", 4), ("prefix", 1), ("cap prefix", 2)):
@@ -206,7 +207,7 @@ def test_forms_of_the_gpu_tests():
                         extra["prefix_lens"] = 0xd00000
                     calls.append(paged_launches.call(news, lens, H, Hk, d, max_seqlen_q=max(news), causal=True, num_splits=splits[0] if splits else 1, **extra))
                     want.append([form, number])
-    for shapes, form, dims in ((scores.TREES_FEW, "few", (24, 64, 96, 128)), (scores.TREES_MID, "mid", (64, 80, 128)), (scores.TREES_TALL[:1], "tall", (40, 64, 80, 128)),
+    for shapes, form, dims in ((scores.TREES_FEW, "few", (24, 64, 96, 128)), (scores.TREES_MID, "mid", (64, 80, 128)), (scores.TREES_PAIRED, "paired", (40, 64, 80, 128)), (scores.TREES_TALL[:1], "tall", (40, 64, 80, 128)),
                                (scores.TREES_TALL[1:], "tall", (80, 128))):
         for news, lens, H, Hk, *splits in shapes:
             for d in dims:
