@@ -692,6 +692,7 @@ struct RowScores {
             for (int r = 0; r < 16; ++r) {
                 const int key = k0 + 32 * kb + 8 * (r >> 2) + (r & 3);
                 s[kb][r] -= slope * (__builtin_fabsf(distance(a, key)) + (float)(key - place));  // (0 for the others)
+                asm volatile("" : "+v"(s[kb][r]));  // (one after the other: 32 distances at once do not fit in the registers)
             }
     }
     // t of a product
