@@ -78,15 +78,17 @@ template <int kScores>
 __device__ __forceinline__ int tile_of(int t, int ntiles) { return last_first(kScores) ? max(ntiles - 1 - t, 0) : t; }
 
 constexpr int kTreeTokens = 256;  // drafted tokens of a sequence that a mask can name
-struct ScoredArgs : PagedArgs {
-    const float* slopes;        // [H]
-    const int32_t* prefix;      // [B], or null
+struct ScoredExtras {
     const uint64_t* tree;       // [tokens, tree_words], or null.  With a tree `causal` is 0 and `wr` is -1
+    const int32_t* prefix;      // [B], or null
+    const float* slopes;        // [H]
     int64_t tree_stride;
-    int tree_words;
     float cap_in, cap;          // exp2 of cap_in times a product is e^(2 score / cap)
     float slope_unit;           // of the slopes, to the units of what they are added to
+    int tree_words;
 };
+// (in front: the line of arguments that is read first has them, and nobody waits for another)
+struct ScoredArgs : ScoredExtras, PagedArgs {};
 template <int kScores>
 using ArgsOf = std::conditional_t<kScores == kScoresPlain, PagedArgs, ScoredArgs>;
 
