@@ -27,6 +27,7 @@ from .binding import (  # noqa: F401
 from .paged import (  # noqa: F401
     FLASH_MAX_SOFTCAP,
     FLASH_MAX_TREE_TOKENS,
+    FLASH_MIN_SOFTCAP,
     KeepParams,
     PagedParams,
     RotaryParams,

@@ -90,7 +90,7 @@ int validate_paged(const flash_paged_params* p, bool* empty)
 // what the forward has beside them: scores and masks of other kinds
 int validate_scores(const flash_paged_params* p)
 {
-    if (!(p->softcap >= 0.0f) || p->softcap > FLASH_MAX_SOFTCAP) return FLASH_EINVAL;
+    if (!(p->softcap >= 0.0f) || p->softcap > FLASH_MAX_SOFTCAP || (p->softcap > 0.0f && p->softcap < FLASH_MIN_SOFTCAP)) return FLASH_EINVAL;
     if (misaligned(p->alibi_slopes, 4) || misaligned(p->prefix_lens, 4) || misaligned(p->tree_mask, 8)) return FLASH_EALIGN;
     if (!p->tree_mask) return FLASH_OK;
     // (the mask says what the chunk's tokens see of each other)
@@ -377,20 +377,27 @@ bool ordered(const flash_paged_params* p, int br)
     return groups > kNumCU && groups <= (keys_of(p) > kShortKeys ? kOrderedGroups : kOrderedShort);
 }
 
+// products to the cap's argument (RowScores::capped), slopes to the units that the softmax goes by
+float cap_in_of(const flash_paged_params* p) { return (float)(2.0 * (double)fa::kLog2e * p->softmax_scale / p->softcap); }
+float slope_unit_of(const flash_paged_params* p) { return p->softcap > 0.0f ? 0.5f / p->softcap : 1.0f / p->softmax_scale; }
+// (an infinite one would make a NaN of a product or a distance of 0)
+bool units_finite(const flash_paged_params* p)
+{
+    return !(p->softcap > 0.0f && std::isinf(cap_in_of(p))) && !(p->alibi_slopes && std::isinf(slope_unit_of(p)));
+}
+
 // a has what every launch has
 int launch_scored(const flash_paged_params* p, fa::ScoredArgs& a, int br, long long blocks, hipStream_t st)
 {
     const bool bf16 = p->dtype == FLASH_BF16;
-    a.slopes = p->alibi_slopes, a.prefix = p->prefix_lens;
+    a.slopes = p->alibi_slopes, a.slope_unit = slope_unit_of(p), a.prefix = p->prefix_lens;
     a.tree = reinterpret_cast<const uint64_t*>(p->tree_mask), a.tree_stride = p->tree_stride, a.tree_words = p->tree_words;
     if (p->softcap > 0.0f) {
         a.cap = p->softcap;
-        a.cap_in = (float)(2.0 * (double)fa::kLog2e * p->softmax_scale / p->softcap);
+        a.cap_in = cap_in_of(p);
         a.scale_log2 = 2.0f * p->softcap * fa::kLog2e;
-        a.slope_unit = 0.5f / p->softcap;
         return a.slopes ? fa::launch_scored_both(a, bf16, br, blocks, st) : fa::launch_scored_capped(a, bf16, br, blocks, st);
     }
-    a.slope_unit = 1.0f / p->softmax_scale;
     return a.slopes ? fa::launch_scored_sloped(a, bf16, br, blocks, st) : fa::launch_scored_masked(a, bf16, br, blocks, st);
 }
 
@@ -401,6 +408,7 @@ int run_forward(const flash_paged_params* p, hipStream_t st)
     if (rc != FLASH_OK) return rc;
     if (!(p->softmax_scale > 0.0f) || std::isinf(p->softmax_scale)) return FLASH_EINVAL;
     if ((rc = validate_scores(p)) != FLASH_OK) return rc;
+    if (!units_finite(p)) return FLASH_EINVAL;
     if (empty) return FLASH_OK;
     if ((rc = validate_cache(p)) != FLASH_OK) return rc;
     if ((rc = rows_strides(p->q_token, p->q_head, p->Q)) != FLASH_OK || (rc = rows_strides(p->o_token, p->o_head, p->O)) != FLASH_OK) return rc;

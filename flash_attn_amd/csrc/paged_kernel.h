@@ -596,7 +596,7 @@ __device__ __forceinline__ uint64_t range_bits(int lo, int hi)
 // What a lane knows of its row, and its wave of its rows
 template <int kScores>
 struct RowScores {
-    TreeTable tree;
+    TreeTable tree = {nullptr, nullptr, 0};  // (none: keys in front of the chunk alone)
     int token, base;      // its index in the chunk; the chunk's first key
     int kmin, kmax;       // keys of the work-group
     int place;            // position

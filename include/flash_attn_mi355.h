@@ -261,8 +261,9 @@ typedef struct flash_paged_params {
     const void *positions;     /* NULL: the places in the sequence; otherwise [total_q], for the angles alone */
     int positions_64;
     /* forward: scores and masks beside the above */
-    float softcap;             /* > 0: scores x = scale q.k become softcap * tanh(x / softcap); up to FLASH_MAX_SOFTCAP.  0: they stay */
-    const float *alibi_slopes; /* fp32 [H], finite, or NULL: score -= slope[h] * |i - j| of the positions, behind the cap */
+    float softcap;             /* FLASH_MIN_SOFTCAP ... FLASH_MAX_SOFTCAP: scores x = scale q.k become softcap * tanh(x / softcap).  0: they stay */
+    const float *alibi_slopes; /* fp32 [H], or NULL: score -= slope[h] * |i - j| of the positions, behind the cap.  Finite, as has to be slope / softmax_scale,
+                                * with a cap slope / softcap; 1 / softmax_scale is checked, and softmax_scale / softcap */
     const int32_t *prefix_lens;   /* [B], or NULL: keys j < prefix_lens[b] are seen whatever is_causal and window_right say */
     const int64_t *tree_mask;  /* [total_q] rows of tree_words words, or NULL: the new tokens are a tree's, and bit j % 64 of word j / 64 of a token's row says
                                 * whether it sees new token j of its sequence (itself among them).  It takes the place of is_causal; window_right and
@@ -273,6 +274,7 @@ typedef struct flash_paged_params {
     int64_t tree_stride;       /* words from row to row */
 } flash_paged_params;
 
+#define FLASH_MIN_SOFTCAP 1e-6f
 #define FLASH_MAX_SOFTCAP 1000.0f
 #define FLASH_MAX_TREE_TOKENS 256
 

@@ -215,3 +215,14 @@ def test_forms_of_the_gpu_tests():
                 calls.append(paged_launches.call(news, lens, H, Hk, d, max_seqlen_q=max(news), num_splits=splits[0] if splits else 1, tree_mask=0xe00000, tree_words=words, tree_stride=words))
                 want.append([form, 1])
     assert launched(calls) == want
+
+
+@pytest.mark.parametrize("code,kw", [
+    (E_INVAL, {"softcap": 0.9e-6}), (E_INVAL, {"softcap": 1e-40}), (E_INVAL, {"softcap": 1e-6, "softmax_scale": 1e33}), (E_INVAL, {"alibi_slopes": 0x110000, "softmax_scale": 1e-39}),
+    (E_NODEVICE, {"softcap": 1e-6}), (E_NODEVICE, {"softcap": 1e-6, "alibi_slopes": 0x110000, "softmax_scale": 1e-39}), (E_NODEVICE, {"alibi_slopes": 0x110000, "softmax_scale": 1e-38}),
+    (E_NODEVICE, {"softmax_scale": 1e-39})])
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would launch with these pointers")
+def test_units_of_scores_are_finite(paged, code, kw):
+    """A cap below FLASH_MIN_SOFTCAP, and units in which a product or a distance of 0 would be 0 times infinity, are refused."""
+    assert paged.FLASH_MIN_SOFTCAP == 1e-6
+    assert paged._lib().flash_forward_paged(C.byref(paged_params(paged, **kw)), None) == code
