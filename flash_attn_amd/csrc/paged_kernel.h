@@ -92,6 +92,16 @@ struct ScoredArgs : ScoredExtras, PagedArgs {};
 template <int kScores>
 using ArgsOf = std::conditional_t<kScores == kScoresPlain, PagedArgs, ScoredArgs>;
 
+// A kernel's own arguments, read once more where they stand: what is used behind the loop, or seldom, would otherwise lie in scalar registers all along, of which there
+// are too few for all (60 of them went into lanes of a vector register and back: 250 instructions of the 1200 in front of the first product).
+__device__ __forceinline__ const PagedArgs& read_again(const PagedArgs& a) { return a; }
+__device__ __forceinline__ const ScoredArgs& read_again(const ScoredArgs&)
+{
+    uintptr_t at = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const ScoredArgs*)reinterpret_cast<const __attribute__((address_space(4))) ScoredArgs*>(at);
+}
+
 // What the merge needs of them (short arguments launch faster: common.h)
 struct PagedMergeArgs {
     char* O;
@@ -715,10 +725,11 @@ struct RowScores {
                     for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(slope, (float)(32 * kb + 8 * (r >> 2) + (r & 3)), s[kb][r]);
             }
         }
-        if (has_slopes(kScores) && __builtin_expect(kb0 + 32 * KB > bent, 0)) bend(a, s, kb0, g);
+        if (has_slopes(kScores) && __builtin_expect(kb0 + 32 * KB > bent, 0)) bend(read_again(a), s, kb0, g);
         if (__builtin_expect(sides != 0, 0)) {
-            if (a.tree) {
-                const uint64_t seen = (range_bits(lo - kb0, hi - kb0) | drafted_bits(a, kb0)) >> (4 * g);
+            const ScoredArgs& again = read_again(a);
+            if (again.tree) {
+                const uint64_t seen = (range_bits(lo - kb0, hi - kb0) | drafted_bits(again, kb0)) >> (4 * g);
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
                     const uint32_t bits = (uint32_t)(seen >> (32 * kb));
@@ -1017,9 +1028,10 @@ __device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
         }
     }
     if constexpr (kScores != kScoresPlain) {
-        if (a.tree && kmax > it.shift) tree_setup<256>(a, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
-        row.set(a, it, r, kmin, kmax, &lo, &hi);
-        lo_max = a.tree ? -rows_min(-lo) : __builtin_amdgcn_readlane(lo, 31);  // (a tree's bounds may fall)
+        const ScoredArgs& again = read_again(a);
+        if (again.tree && kmax > it.shift) tree_setup<256>(again, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
+        row.set(again, it, r, kmin, kmax, &lo, &hi);
+        lo_max = again.tree ? -rows_min(-lo) : __builtin_amdgcn_readlane(lo, 31);  // (a tree's bounds may fall)
         hi_min = __builtin_amdgcn_readlane(hi, 0);
     }
     const float c2 = a.scale_log2, inv_c2 = __builtin_amdgcn_rcpf(c2);
@@ -1074,7 +1086,7 @@ __device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
         if (more) request_v(t + 4);
     }
     if (wave < ntiles && __builtin_expect(any_not_finite<MB>(oacc), 0))
-        paged_rescue<BC, MB, kBf16, kScores>(a, it, r, kmin, kmax, tile0, ntiles, last_first(kScores) ? (ntiles - 1 - wave) & 3 : wave, 4, soft.m_ref, oacc, row);
+        paged_rescue<BC, MB, kBf16, kScores>(read_again(a), it, r, kmin, kmax, tile0, ntiles, last_first(kScores) ? (ntiles - 1 - wave) & 3 : wave, 4, soft.m_ref, oacc, row);
 
     // ---- merge of the four waves: reference of a row = the largest of theirs
     const int nrows = min(kPagedFewRows, it.rows - it.row0);
@@ -1099,6 +1111,7 @@ __device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
     }
     __syncthreads();
     constexpr int CO = D / 8;  // eight columns per thread
+    const ArgsOf<kScores>& end = read_again(a);
     for (int k = tid; k < nrows * CO; k += 256) {
         const int row = k / CO, c = (k % CO) * 8;
         float m = xm[row];
@@ -1114,23 +1127,23 @@ __device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
             for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf(f, src[e], o[e]);
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const float lse = l == 0.0f ? -INFINITY : lse_of<kScores>(a, m, l);
+        const float lse = l == 0.0f ? -INFINITY : lse_of<kScores>(end, m, l);
         int head;
-        const int tok = row_token(a, it, it.row0 + row, &head);
-        const size_t at = (size_t)tok * a.H + head;
-        if (c >= a.d) continue;
-        if (a.num_splits > 1) {
-            const size_t part = at * a.num_splits + it.split;
-            float* const op = a.O_partial + part * a.d + c;
+        const int tok = row_token(end, it, it.row0 + row, &head);
+        const size_t at = (size_t)tok * end.H + head;
+        if (c >= end.d) continue;
+        if (end.num_splits > 1) {
+            const size_t part = at * end.num_splits + it.split;
+            float* const op = end.O_partial + part * end.d + c;
             const v4f o0 = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv}, o1 = {o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv};
             *reinterpret_cast<v4f*>(op) = o0;
             *reinterpret_cast<v4f*>(op + 4) = o1;
-            if (c == 0) a.LSE_partial[part] = lse;
+            if (c == 0) end.LSE_partial[part] = lse;
         } else {
             const v4u w = {Elem<kBf16>::pack(o[0] * inv, o[1] * inv), Elem<kBf16>::pack(o[2] * inv, o[3] * inv),
                            Elem<kBf16>::pack(o[4] * inv, o[5] * inv), Elem<kBf16>::pack(o[6] * inv, o[7] * inv)};
-            *reinterpret_cast<v4u*>(a.O + (size_t)tok * a.o_token + (size_t)head * a.o_head + c * 2) = w;
-            if (c == 0) a.LSE[at] = lse;
+            *reinterpret_cast<v4u*>(end.O + (size_t)tok * end.o_token + (size_t)head * end.o_head + c * 2) = w;
+            if (c == 0) end.LSE[at] = lse;
         }
     }
 }
@@ -1512,13 +1525,14 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
     }
     req.ask(a, tile_of<kScores>(3, ntiles));  // (vnext: of tile 2)
     if constexpr (kScores != kScoresPlain) {
-        if (a.tree && kmax > it.shift) tree_setup<512>(a, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
-        row.set(a, it, r, kmin, kmax, &lo, &hi);
+        const ScoredArgs& again = read_again(a);
+        if (again.tree && kmax > it.shift) tree_setup<512>(again, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
+        row.set(again, it, r, kmin, kmax, &lo, &hi);
         lo_min = __builtin_amdgcn_readlane(lo, 0);
         hi_min = __builtin_amdgcn_readlane(hi, 0);
         lo_max = __builtin_amdgcn_readlane(lo, 31);
         hi_max = __builtin_amdgcn_readlane(hi, 31);
-        if (a.tree) lo_min = rows_min(lo), lo_max = -rows_min(-lo), hi_max = kmax - 1;  // (a tree's bounds may fall)
+        if (again.tree) lo_min = rows_min(lo), lo_max = -rows_min(-lo), hi_max = kmax - 1;  // (a tree's bounds may fall)
     }
     if (ntiles > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * NL) : "memory");
     else if (ntiles == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NL) : "memory");
@@ -1587,8 +1601,8 @@ __device__ __forceinline__ void tall_rows(const ArgsOf<kScores> a)
     if (first_row >= it.rows) return;
 
     // ---- epilogue
-    if (__builtin_expect(any_not_finite<MB>(oacc), 0)) paged_rescue<BC, MB, kBf16, kScores>(a, it, r, kmin, kmax, tile0, ntiles, 0, 1, soft.m_ref, oacc, row);
-    paged_store_rows<D, MB, kBf16, kScores>(a, it, first_row, r, lane, g, soft.m_ref, soft.l_run, oacc, Ks + wave * (32 * T::ROW));
+    if (__builtin_expect(any_not_finite<MB>(oacc), 0)) paged_rescue<BC, MB, kBf16, kScores>(read_again(a), it, r, kmin, kmax, tile0, ntiles, 0, 1, soft.m_ref, oacc, row);
+    paged_store_rows<D, MB, kBf16, kScores>(read_again(a), it, first_row, r, lane, g, soft.m_ref, soft.l_run, oacc, Ks + wave * (32 * T::ROW));
 }
 
 template <int D, int DU, bool kBf16>
@@ -1671,12 +1685,13 @@ __global__ void __launch_bounds__(256 * GROUPS, 2) scored_mid_kernel(const Score
     }
     req.ask(a, tile_at(NST - 1));
     RowScores<kScores> row;
-    if (a.tree && kmax > it.shift) tree_setup<kThreads>(a, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
+    const ScoredArgs& again = read_again(a);
+    if (again.tree && kmax > it.shift) tree_setup<kThreads>(again, it, tid, (FA_LDS char*)smem + C::SMEM, has_slopes(kScores), &row.tree);
     int lo, hi;
-    row.set(a, it, r, kmin, kmax, &lo, &hi);
+    row.set(again, it, r, kmin, kmax, &lo, &hi);
     int lo_min = __builtin_amdgcn_readlane(lo, 0), hi_min = __builtin_amdgcn_readlane(hi, 0);
     int lo_max = __builtin_amdgcn_readlane(lo, 31), hi_max = __builtin_amdgcn_readlane(hi, 31);  // (bounds do not fall from row to row)
-    if (a.tree) lo_min = rows_min(lo), lo_max = -rows_min(-lo), hi_max = kmax - 1;               // (but a tree's do)
+    if (again.tree) lo_min = rows_min(lo), lo_max = -rows_min(-lo), hi_max = kmax - 1;           // (but a tree's do)
 
     v8h qf[KS];
     v16f oacc[MB];
@@ -1751,7 +1766,7 @@ __global__ void __launch_bounds__(256 * GROUPS, 2) scored_mid_kernel(const Score
         __builtin_amdgcn_sched_barrier(0);
     }
     if (first_row < it.rows && __builtin_expect(any_not_finite<MB>(oacc), 0))
-        paged_rescue<BC, MB, kBf16, kScores>(a, it, r, kmin, kmax, tile0, ntiles, last_first(kScores) ? (ntiles - 1 - grp) % GROUPS : grp, GROUPS, soft.m_ref, oacc, row);
+        paged_rescue<BC, MB, kBf16, kScores>(read_again(a), it, r, kmin, kmax, tile0, ntiles, last_first(kScores) ? (ntiles - 1 - grp) % GROUPS : grp, GROUPS, soft.m_ref, oacc, row);
     paged_barrier();  // every wave is done with the stages
     FA_LDS char* ost = (FA_LDS char*)smem + wave * (32 * T::ROW);
     if constexpr (GROUPS == 2) {
@@ -1777,7 +1792,7 @@ __global__ void __launch_bounds__(256 * GROUPS, 2) scored_mid_kernel(const Score
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before O goes there)
     }
     if (first_row >= it.rows) return;
-    paged_store_rows<D, MB, kBf16, kScores>(a, it, first_row, r, lane, g, soft.m_ref, soft.l_run, oacc, ost);
+    paged_store_rows<D, MB, kBf16, kScores>(read_again(a), it, first_row, r, lane, g, soft.m_ref, soft.l_run, oacc, ost);
 }
 
 // ---------------------------------------------------------------------------------------------- merge of splits
