@@ -972,12 +972,25 @@ __device__ __forceinline__ void few_rows(const ArgsOf<kScores> a)
         const int kb0 = (tile0 + tile_of<kScores>(t, ntiles)) * BC;
         const bool whole = kb0 + BC <= len;
         if constexpr (kScores != kScoresPlain) {
-            if (__builtin_expect(whole && a.d == D, 1)) {  // (nearly all tiles: no branch per request)
+            if (__builtin_expect(whole && a.d == D, 1)) {  // (nearly all tiles, and nearly all others: no branch per request)
 #pragma unroll
                 for (int s = 0; s < GROUPS; ++s) {
                     const char* const at = place[s].in(a, head, page_bytes, row_bytes);
 #pragma unroll
                     for (int x = 0; x < kPer; ++x) dma_kib_nt(at, off[x], dst + (s * kPer + x) * 1024);
+                }
+                return;
+            }
+            if (__builtin_expect(a.d == D, 1)) {
+#pragma unroll
+                for (int s = 0; s < GROUPS; ++s) {
+                    const char* const at = place[s].in(a, head, page_bytes, row_bytes);
+#pragma unroll
+                    for (int x = 0; x < kPer; ++x) {
+                        const int r = T::RPB * x + lrow, past = r - (len - 1 - (kb0 + 16 * s));
+                        if constexpr (kIsV) dma_kib_lanes<true>(past <= 0 ? at + off[x] : reinterpret_cast<const char*>(&kPagedZeroes), dst + (s * kPer + x) * 1024);
+                        else dma_kib_nt(at, off[x] - (uint32_t)min(max(past, 0), r) * row_bytes, dst + (s * kPer + x) * 1024);
+                    }
                 }
                 return;
             }
