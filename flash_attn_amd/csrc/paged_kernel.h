@@ -1325,13 +1325,15 @@ struct TallCfg {
 
 // Rows of a tile of V from `left` on lie past the sequence's end and repeat the last key's.  Their probabilities are 0, but 0 times a value that is not
 // finite is not, and the wave's rows may see the last key: if it has such a value these rows become 0.  Each wave does so in front of its own reads, all
-// write the same.  (Requests that take the rows from a row of zeroes, as in the 32-row form, make the loop longer: 640 rows on 28339 keys B4 H5 H_kv1 d80
+// write the same, and all go by the last key's own row, which nobody writes: a row that another wave has cleared says nothing of those behind it.
+// (Requests that take the rows from a row of zeroes, as in the 32-row form, make the loop longer: 640 rows on 28339 keys B4 H5 H_kv1 d80
 // 113.1 -> 118.2 us; so 113.5.)
+__host__ __device__ constexpr int paged_asked_row(int left) { return left - 1; }
 template <int D, bool kBf16>
 __device__ __forceinline__ void paged_clear_past(FA_LDS char* stage, int left, int lane)
 {
     using T = PagedTile<D>;
-    const v4u row = *reinterpret_cast<FA_LDS const v4u*>(stage + left * T::ROW + (lane % T::CPR) * 16);
+    const v4u row = *reinterpret_cast<FA_LDS const v4u*>(stage + paged_asked_row(left) * T::ROW + (lane % T::CPR) * 16);
     bool odd = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) odd |= Elem<kBf16>::not_finite(row[e]);
