@@ -534,7 +534,7 @@ int run_keep(const flash_keep_params* p, hipStream_t st)
     a.v_layer = 2 * p->vc_layer, a.v_page = 2 * p->vc_page, a.v_head = 2 * p->vc_head, a.v_row = 2 * p->vc_row;
     a.table_stride = p->block_table_stride, a.path_stride = p->path_stride;
     a.B = p->B, a.layers = p->layers, a.Hk = p->H_kv, a.d = p->d, a.num_pages = p->num_pages, a.page = p->page_size;
-    a.capacity = p->num_pages > 0 ? p->page_size * p->max_pages : 0, a.most = p->max_path;
+    a.capacity = p->page_size * p->max_pages, a.most = p->max_path;  // (lengths do not depend on the pages that there are; rows on others are not moved)
     return record_hip(fa::launch_keep(a, st));
 }
 
