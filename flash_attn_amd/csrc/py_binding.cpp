@@ -499,6 +499,7 @@ PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t n)
         p.kc_layer = dims == 5 ? k.stride(0) : 0, p.kc_page = k.stride(-4), p.kc_head = k.stride(-3), p.kc_row = k.stride(-2);
         p.vc_layer = dims == 5 ? v.stride(0) : 0, p.vc_page = v.stride(-4), p.vc_head = v.stride(-3), p.vc_row = v.stride(-2);
         p.block_table_stride = table.stride(0), p.path_stride = path.stride(0);
+        if (p.layers == 0) p.layers = 1, p.num_pages = 0;  // (the lengths alone)
         const int rc = g_keep(&p, c10::hip::getCurrentHIPStream().stream());
         if (rc != FLASH_OK) return raise(rc, "flash_keep_paged");
         written({&k, &v, out});

@@ -614,6 +614,8 @@ def flash_keep_paged(k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, pat
         p.vc_page, p.vc_head, p.vc_row = v_cache.stride()[-4:-1]
         if many:
             p.kc_layer, p.vc_layer = k_cache.stride(0), v_cache.stride(0)
+        if p.layers == 0:  # (the lengths alone: one layer without pages)
+            p.layers, p.num_pages = 1, 0
         p.block_table_stride, p.path_stride = block_table.stride(0), path.stride(0)
         _raise(_lib().flash_keep_paged(C.byref(p), handle), "flash_keep_paged")
     _written(k_cache, v_cache, given)

@@ -326,7 +326,8 @@ typedef struct flash_keep_params {
     const int32_t *path;          /* [B, max_path] */
     const int32_t *accepted;      /* [B], cut to 0 ... max_path */
     int32_t *seqlens_out;         /* [B], none of the other tensors */
-    int B, H_kv, d, layers, num_pages, page_size, max_pages, max_path;   /* d: a multiple of 8 up to FLASH_MAX_HEAD_DIM */
+    int B, H_kv, d, layers, num_pages, page_size, max_pages, max_path;   /* d: a multiple of 8 up to FLASH_MAX_HEAD_DIM.  layers: of 0 the call is empty and
+                                   * writes nothing, seqlens_out neither; one layer of num_pages = 0 (no caches needed) gives the lengths alone */
     int64_t kc_layer, kc_page, kc_head, kc_row, vc_layer, vc_page, vc_head, vc_row;   /* elements, multiples of 8 */
     int64_t block_table_stride, path_stride;
 } flash_keep_params;
