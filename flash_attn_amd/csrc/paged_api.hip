@@ -516,10 +516,15 @@ int run_keep(const flash_keep_params* p, hipStream_t st)
     if (misaligned(p->seqlens_k, 4) || misaligned(p->cu_seqlens_q, 4) || misaligned(p->accepted, 4) || misaligned(p->seqlens_out, 4) || misaligned(p->path, 4) ||
         misaligned(p->block_table, 4))
         return FLASH_EALIGN;
-    // (other work-groups still read the lengths when the first one writes)
-    const int32_t *const o = p->seqlens_out, *const o_end = o + p->B;
-    auto apart_from = [&](const int32_t* t, long long n) { return n <= 0 || o_end <= t || t + n <= o; };
-    if (!apart_from(p->seqlens_k, p->B) || !apart_from(p->cu_seqlens_q, p->B + 1LL) || !apart_from(p->accepted, p->B)) return FLASH_EINVAL;
+    // (other work-groups still read the lengths, the path and the table when the first one writes)
+    auto apart_from = [&](const int32_t* t, int rows, int64_t stride, int n) {  // `rows` rows of n entries
+        const __int128 at = (reinterpret_cast<intptr_t>(p->seqlens_out) - reinterpret_cast<intptr_t>(t)) / 4;  // (in entries: all are aligned)
+        const __int128 row = at < n || stride == 0 ? 0 : (at - n) / stride + 1;                                // the first that ends behind it
+        return n <= 0 || row >= rows || row * stride + n <= at || row * stride >= at + p->B;
+    };
+    if (!apart_from(p->seqlens_k, 1, 0, p->B) || !apart_from(p->cu_seqlens_q, 1, 0, p->B + 1) || !apart_from(p->accepted, 1, 0, p->B) ||
+        !apart_from(p->path, p->B, p->path_stride, p->max_path) || !apart_from(p->block_table, p->B, p->block_table_stride, p->max_pages))
+        return FLASH_EINVAL;
     if (p->num_pages > 0) {
         if (!p->K_cache || !p->V_cache || p->K_cache == p->V_cache) return FLASH_EINVAL;
         if (misaligned(p->K_cache, 16) || misaligned(p->V_cache, 16)) return FLASH_EALIGN;
