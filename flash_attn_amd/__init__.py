@@ -25,6 +25,7 @@ from .binding import (  # noqa: F401
     lib,
 )
 from .paged import (  # noqa: F401
+    FLASH_MAX_SLOPE,
     FLASH_MAX_SOFTCAP,
     FLASH_MAX_TREE_TOKENS,
     FLASH_MIN_SOFTCAP,

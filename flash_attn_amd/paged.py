@@ -59,6 +59,7 @@ class PagedParams(C.Structure):
 
 
 FLASH_MIN_SOFTCAP, FLASH_MAX_SOFTCAP = 1e-6, 1000.0
+FLASH_MAX_SLOPE = 1024.0
 FLASH_MAX_TREE_TOKENS = 256
 
 
@@ -455,11 +456,12 @@ def flash_forward_paged(q, k_cache, v_cache, block_table, seqlens_k, cu_seqlens_
     Rows that belong to no sequence are left as they are (new memory where out and lse are not given).  For serving: tensors that require a gradient
     are refused while gradients are recorded.
 
-    softcap > 0: scores x become softcap * tanh(x / softcap), from FLASH_MIN_SOFTCAP to FLASH_MAX_SOFTCAP.  alibi_slopes: fp32 [H], finite, score -= slope[h] * |i - j| of
-    the positions, behind the cap.  prefix_lens: int32 [B], keys in front of it are seen by all of a sequence's tokens, whatever causal and a
-    right window say.  tree_mask: int64 [tokens, words] (flash_tree_mask): bit j % 64 of word j / 64 says whether a token sees new token j of its
-    sequence, in place of causal; with it max_seqlen_q is at most 64 * words, tokens stand at the chunk's begin plus their depth (bits less one), a right
-    window and a prefix are refused, and a left window must reach over a chunk."""
+    softcap > 0: scores x become softcap * tanh(x / softcap), from FLASH_MIN_SOFTCAP to FLASH_MAX_SOFTCAP.  alibi_slopes: fp32 [H], from
+    -FLASH_MAX_SLOPE to FLASH_MAX_SLOPE (device memory: not checked), score -= slope[h] * |i - j| of the positions, behind the cap.  prefix_lens:
+    int32 [B], keys in front of it are seen by all of a sequence's tokens, whatever causal and a right window say.  tree_mask: int64 [tokens, words]
+    (flash_tree_mask): bit j % 64 of word j / 64 says whether a token sees new token j of its sequence, in place of causal; with it max_seqlen_q is at
+    most 64 * words, tokens stand at the chunk's begin plus their depth (bits less one), a right window and a prefix are refused, and a left window
+    must reach over a chunk."""
     if stream is None:
         native = _native or _front_end()
         if softcap == 0 and alibi_slopes is None and prefix_lens is None and tree_mask is None:

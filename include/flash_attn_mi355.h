@@ -262,7 +262,8 @@ typedef struct flash_paged_params {
     int positions_64;
     /* forward: scores and masks beside the above */
     float softcap;             /* FLASH_MIN_SOFTCAP ... FLASH_MAX_SOFTCAP: scores x = scale q.k become softcap * tanh(x / softcap).  0: they stay */
-    const float *alibi_slopes; /* fp32 [H], or NULL: score -= slope[h] * |i - j| of the positions, behind the cap.  Finite, as has to be slope / softmax_scale,
+    const float *alibi_slopes; /* fp32 [H], or NULL: score -= slope[h] * |i - j| of the positions, behind the cap.  |slope| at most FLASH_MAX_SLOPE: a score's
+                                * rounding grows by up to (d + 11) 2^-24 * 64 |slope|.  slope / softmax_scale has to be finite,
                                 * with a cap slope / softcap; 1 / softmax_scale is checked, and softmax_scale / softcap */
     const int32_t *prefix_lens;   /* [B], or NULL: keys j < prefix_lens[b] are seen whatever is_causal and window_right say */
     const int64_t *tree_mask;  /* [total_q] rows of tree_words words, or NULL: the new tokens are a tree's, and bit j % 64 of word j / 64 of a token's row says
@@ -276,6 +277,7 @@ typedef struct flash_paged_params {
 
 #define FLASH_MIN_SOFTCAP 1e-6f
 #define FLASH_MAX_SOFTCAP 1000.0f
+#define FLASH_MAX_SLOPE 1024.0f   /* (device memory: not checked) */
 #define FLASH_MAX_TREE_TOKENS 256
 
 /* New rows of K, turned as by flash_rotary, and of V into their pages; Q, if it is given, turned into O by the same launch.  Rows whose place

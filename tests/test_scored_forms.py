@@ -1,5 +1,6 @@
-"""Every case of test_gpu_scored_forms.py gets the form that it is there for, and the kernel of its scores.  No GPU needed."""
+"""Every case of test_gpu_scored_forms.py and test_gpu_steep_slopes.py gets the form that it is there for, and the kernel of its scores.  No GPU needed."""
 import test_gpu_scored_forms as forms
+import test_gpu_steep_slopes as steep
 from test_scored_arguments import launched
 
 KINDS = {"": 1, "prefix": 1, "cap": 2, "cap prefix": 2, "slopes": 3, "slopes prefix": 3, "both": 4, "both prefix": 4}
@@ -29,3 +30,14 @@ def test_every_form_has_every_kind():
             if (form, name) != ("tall", "causal"):  # (test_gpu_paged_scores.py: unsplit and in splits)
                 assert {c[7] for c in mine if is_one(c[6])} == set(forms.SCORES), (form, name)
         assert {c[5] > 1 for c in mine} == {False, True}
+
+
+def test_forms_of_steep_slopes():
+    calls, want = [], []
+    for form, news, lens, H, Hk, splits in steep.SHAPES:
+        for mask in steep.MASKS:
+            for d in steep.DIMS:
+                for kind in ("slopes", "both"):
+                    calls.append(forms.arguments(news, lens, H, Hk, d, splits, mask, kind))
+                    want.append([form, KINDS[kind]])
+    assert launched(calls) == want
