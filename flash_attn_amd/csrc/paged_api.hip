@@ -16,7 +16,7 @@ using fa::device_usable;
 using fa::misaligned;
 using fa::record_hip;
 
-constexpr int kNumCU = 256;  // MI355X
+constexpr int kNumCU = fa::kPagedCus;
 constexpr int kMostTokens = 1 << 25;
 constexpr long long kMostOfToken = 1LL << 30;  // elements of a token's heads: the kernels count them in an int, with a launch's step on top
 

@@ -43,6 +43,7 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kPagedTallRows = 256, kPagedMidRows = 128, kPagedFewRows = 32;  // rows of a work-group
+constexpr int kPagedCus = 256;                                                      // of an MI355X
 constexpr int paged_threads(int rows) { return rows == kPagedTallRows ? 512 : 256; }
 
 struct PagedArgs {
@@ -550,10 +551,11 @@ struct PagedSoftmax {
 // A cap turns a score x into c tanh(x / c).  tanh(z) = 1 + 2 t with t = -1 / (1 + e^(2 z)), which grows with z from -1 to 0: the softmax goes by t in place
 // of the product, in units of 2 c log2 e, and the constant c that is missing is added to the LSE.  That is a product, two transcendental
 // instructions and a subtraction per score in front of the usual fma and exp2, 24 cycles of a SIMD beside the 24 that a plain score takes and the 32 of its
-// MFMAs at d = 128.  t is off by at most 3 half steps of 2^-24 (v_exp_f32, the subtraction and v_rcp_f32 one each), a score by 6 c 2^-24; a
-// polynomial for small z that stays relative takes as many cycles (measured: v_exp_f32 and v_rcp_f32 8 cycles a wave, other instructions 4).
+// MFMAs at d = 128.  t is off by at most 4.5 half steps of 2^-24 (the argument's two roundings and v_exp_f32, of which at most a quarter arrives, below 1.5; the
+// subtraction 1; v_rcp_f32 2), a score by 9 c 2^-24, 16 c 2^-24 with what the softmax rounds behind it; a polynomial for small z that
+// stays relative takes as many cycles (measured: v_exp_f32 and v_rcp_f32 8 cycles a wave, other instructions 4).
 // A bias by distance, -slope |p - j|, begins as slope (j - p), which a product of its own and an offset of the tile work out; tiles with keys that stand
-// otherwise and may be seen get the difference.  Behind a cap it is added to t, one instruction per score.
+// otherwise and may be seen get the difference.  The sums of a score begin with slope (j - first of the tile), so that what they round grows with 64 |slope|.  Behind a cap it is added to t, one instruction per score.
 // A tree's tokens see the keys in front of the chunk, and of the chunk's those whose bit is set; they stand at the chunk's begin plus their depth, the number
 // of tokens that they see in the chunk less one.  The masks of the sequence's tokens and the depths lie in LDS; all they touch is the last tile or
 // the last few of a sequence, which take a mask of 64 bits per row.
@@ -1951,7 +1953,7 @@ inline int launch_scored_type(const ScoredArgs& a, int rows, long long blocks, h
     if (rows == kPagedMidRows) {
         // a CU for each work-group: two groups of waves where there are tiles enough (one group / two, pieces of 10 to 30 tiles 1.21 on average, more than 30
         // 1.39, 5 to 10 1.08, of one tile 0.92; a window of 1023 on 2900 keys H12 H_kv4 d64 29.8 -> 25.3 us)
-        if (blocks <= 256 && a.tiles_per_split >= 6)
+        if (blocks <= kPagedCus && a.tiles_per_split >= 6)
             return (int)(a.d <= 64 ? launch_scored_instance<64, 64, kBf16, kScores, kPagedMidRows, 4, 2>(a, blocks, st)
                                    : launch_scored_instance<128, 128, kBf16, kScores, kPagedMidRows, 2, 2>(a, blocks, st));
         if (a.d <= 64) return (int)launch_scored_instance<64, 64, kBf16, kScores, kPagedMidRows>(a, blocks, st);

@@ -541,7 +541,8 @@ def flash_tree_mask(parents, cu_seqlens_q, seqlens_k=None, max_seqlen_q=0, mask=
     A parent stands in front of its children; a number that is not below the token's own, or negative, says that it has none and hangs on the keys in
     front of the chunk.  A token's row has the bits of the tokens on its path, its own among them, and it stands at seqlens_k - n + (tokens on the
     path) - 1, without seqlens_k counted from the chunk's begin.  max_seqlen_q: at least the longest chunk (0: the number of tokens), which
-    decides the words, 64 tokens each, up to FLASH_MAX_TREE_TOKENS.  mask, positions: where to."""
+    decides the words, 64 tokens each, up to FLASH_MAX_TREE_TOKENS.  mask, positions: where to; rows of no sequence are left as they are (new memory
+    where these are not given)."""
     if stream is None:
         res = (_native or _front_end()).tree_mask(parents, cu_seqlens_q, seqlens_k, max_seqlen_q, mask, positions)
         if res is not NotImplemented:
@@ -581,7 +582,7 @@ def flash_keep_paged(k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, pat
     Caches [pages,H_kv,page_size,d], or [layers,pages,H_kv,page_size,d] for all layers at once.  path: int32 [B, L], the path's tokens by their numbers in
     the chunk, which grow; accepted: int32 [B], how many of them stay.  Row path[b, i] of the chunk goes to its row i; a path ends in front of the
     first number that does not grow or is not a token of the chunk.  Returned: seqlens_k - n + tokens that stay, in `out` if that is given, which cannot
-    be seqlens_k itself."""
+    lie in one of the other index tensors."""
     if stream is None:
         res = (_native or _front_end()).keep(k_cache, v_cache, block_table, seqlens_k, cu_seqlens_q, path, accepted, out)
         if res is not NotImplemented:

@@ -302,7 +302,7 @@ int flash_forward_paged_workspace_bytes(const flash_paged_params *p, size_t *o_p
  * graph serves all steps. */
 
 /* Masks and positions from the parents of a tree's tokens: row i of a sequence's n has the bits of the tokens on its path from the root, its own
- * among them, and stands at seqlens_k[b] - n + (tokens on the path) - 1. */
+ * among them, and stands at seqlens_k[b] - n + (tokens on the path) - 1.  Rows of no sequence are not written. */
 typedef struct flash_tree_params {
     const int32_t *parents;       /* [total_q]: index of a token's parent within the chunk.  Parents stand in front of their children: a number that is
                                    * not below the token's own, or below 0, is none, and the token hangs on the keys in front of the chunk */
@@ -327,7 +327,7 @@ typedef struct flash_keep_params {
     const int32_t *block_table, *seqlens_k, *cu_seqlens_q;   /* as in flash_paged_params, of all layers */
     const int32_t *path;          /* [B, max_path] */
     const int32_t *accepted;      /* [B], cut to 0 ... max_path */
-    int32_t *seqlens_out;         /* [B], none of the other tensors */
+    int32_t *seqlens_out;         /* [B], in none of the other tensors (the five above are checked) */
     int B, H_kv, d, layers, num_pages, page_size, max_pages, max_path;   /* d: a multiple of 8 up to FLASH_MAX_HEAD_DIM.  layers: of 0 the call is empty and
                                    * writes nothing, seqlens_out neither; one layer of num_pages = 0 (no caches needed) gives the lengths alone */
     int64_t kc_layer, kc_page, kc_head, kc_row, vc_layer, vc_page, vc_head, vc_row;   /* elements, multiples of 8 */
